@@ -334,6 +334,104 @@ int jt_ipc_open_handle(const void* handle, void** ptr);
 int jt_ipc_close_handle(void* ptr);
 
 /*
+ * Block tables, slot maps and positions of a round, from request lengths (no counterpart
+ * kernel in the reference, whose scheduler builds them on the host:
+ * nanovllm/engine/block_manager.py, nanovllm/engine/model_runner.py prepare_prefill /
+ * prepare_decode).  Request r has cached_lens[r] tokens in the cache and writes new_lens[r];
+ * the pages it needs beyond ceil(cached / block_size) are the next entries of free_pages, in
+ * request order, written into block_tables in place.  Token i of the round (requests in
+ * order): slot_mapping[i] = page * block_size + offset, positions[i] = cached + index,
+ * token_to_request[i].  Entries from the round's total to max_tokens are padding (slot -1,
+ * position 0, request -1).  pages_taken[0] is the demand: when it exceeds num_free, the
+ * pages past the list are -1 in the table and their tokens' slots are -1, and so are those of
+ * tokens past table_width pages.  A negative length counts as zero and sets device error
+ * bit 0.
+ */
+typedef struct JtRequestMapsParams {
+  int32_t* block_tables;       /* [num_requests, table_width], row stride below  */
+  const int32_t* cached_lens;  /* [num_requests]                                  */
+  const int32_t* new_lens;     /* [num_requests]                                  */
+  const int32_t* free_pages;   /* [num_free]                                      */
+  int64_t* slot_mapping;       /* [max_tokens]                                    */
+  int64_t* positions;          /* [max_tokens]                                    */
+  int32_t* token_to_request;   /* [max_tokens]                                    */
+  int32_t* cu_seqlens;         /* [num_requests + 1]                              */
+  int32_t* context_lens;       /* [num_requests] cached + new                     */
+  int32_t* pages_taken;        /* [1]                                             */
+  int64_t table_stride0;
+  int32_t num_requests, table_width, block_size, num_free, max_tokens;
+} JtRequestMapsParams;
+
+int jt_request_maps_launch(const JtRequestMapsParams* params, cudaStream_t stream);
+
+/*
+ * RMS norm of every query and key head, then the half-split position rotation, in fp32 with
+ * one rounding, and optionally the K / V rows into the paged cache:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight;  out = [y1 cos - y2 sin, y2 cos + y1 sin]
+ * store 0: rotated K to k_out (v, slots and the pools unused).  store 1: rotated K and V to
+ * the pools [pages, page_size, kv_heads, dim] of the operand type.  store 2: both to e4m3
+ * pools of that shape with one power-of-two scale byte (e8m0, bias 127) per (page, head,
+ * offset): scale 2^e, e the smallest with max|row| <= 448 * 2^e; a row with a non-finite
+ * element gets scale byte 255 (NaN) and zero codes.  Rows with a negative slot are not
+ * written; a slot or position out of range sets device error bit 0 (the slot is skipped, the
+ * position read as 0).  q_out may be q, k_out may be k.  Replaces the head norms of
+ * nanovllm/models/qwen3.py:223-225 with rope_scatter or store_kvcache after them (which
+ * round between the steps).  Strides in elements; last dimensions contiguous.
+ */
+typedef struct JtQkNormRopeParams {
+  const void* q;             /* [rows, q_heads, dim]                                   */
+  const void* k;             /* [rows, kv_heads, dim]                                  */
+  const void* v;             /* [rows, kv_heads, dim]                                  */
+  const void* q_weight;      /* [dim]                                                  */
+  const void* k_weight;      /* [dim]                                                  */
+  const void* positions;     /* [rows] int32 or int64                                  */
+  const void* cos_sin_cache; /* [max_position, dim] (cos | sin)                        */
+  const void* slots;         /* [rows] int32 or int64                                  */
+  void* q_out;               /* [rows, q_heads, dim]                                   */
+  void* k_out;               /* [rows, kv_heads, dim], store 0                         */
+  void* k_pool;
+  void* v_pool;
+  void* k_scale;             /* [pages, kv_heads, page_size] bytes, store 2            */
+  void* v_scale;
+  int64_t num_pages, max_position;
+  int64_t q_stride0, q_stride1, k_stride0, k_stride1, v_stride0, v_stride1;
+  int64_t qo_stride0, qo_stride1, ko_stride0, ko_stride1;
+  int64_t kp_stride0, kp_stride1, kp_stride2, vp_stride0, vp_stride1, vp_stride2;
+  int64_t ks_stride0, ks_stride1, vs_stride0, vs_stride1;
+  int64_t positions_stride, slots_stride, cache_stride0;
+  float eps;
+  int32_t rows, q_heads, kv_heads, head_dim, page_size;
+  int32_t dtype;             /* q, k, v, outputs, store-1 pools: JT_BF16, JT_F16, JT_F32 */
+  int32_t weight_dtype, cache_dtype;
+  int32_t store;             /* 0, 1 or 2                                              */
+  int32_t positions_is_int64, slots_is_int64;
+} JtQkNormRopeParams;
+
+int jt_qk_norm_rope_launch(const JtQkNormRopeParams* params, cudaStream_t stream);
+
+/*
+ * jt_kv_commit_launch's copy for an 8-bit cache: e4m3 rows of kv_pool [2, layers, blocks,
+ * block_size, kv_heads, head_dim] and their bytes of kv_scale [2, layers, blocks, kv_heads,
+ * block_size], gather before scatter.  Strides in bytes; rows 16-byte aligned, head_dim a
+ * multiple of 16, the scale's last dimension contiguous.  At most
+ * jt_kv_fp8_commit_max_slots() slots per call.  A slot out of range is skipped and sets
+ * device error bit 0.
+ */
+typedef struct JtKvFp8CommitParams {
+  void* kv_pool;
+  void* kv_scale;
+  const void* source_slots;       /* [num_slots] int32 or int64 */
+  const void* destination_slots;  /* [num_slots] int32 or int64 */
+  int64_t num_blocks;
+  int64_t stride_axis, stride_layer, stride_block, stride_offset, stride_head;
+  int64_t scale_axis, scale_layer, scale_block, scale_head;
+  int32_t slot_is_int64, num_slots, num_layers, num_kv_heads, head_dim, block_size;
+} JtKvFp8CommitParams;
+
+int jt_kv_fp8_commit_launch(const JtKvFp8CommitParams* params, cudaStream_t stream);
+int32_t jt_kv_fp8_commit_max_slots(void);
+
+/*
  * Failure detection without a GPU fault: runs one thread that waits, with the kernels'
  * bounded-wait routine and a limit of limit_cycles, on an mbarrier nothing arrives on.
  * Synchronous (diagnostics).  out[0] = 1 if the wait claimed completion (a failure),

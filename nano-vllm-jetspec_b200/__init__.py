@@ -21,7 +21,10 @@ from ._lib import KernelLaunchError, LibraryMissingError, load_library, read_dev
 from . import ops  # noqa: F401  (registers the jetspec_b200:: custom operators)
 from .accept import accept_batch, accept_walk
 from .attention import store_kvcache
+from .fp8_cache import alloc_fp8_kv_cache, copy_accepted_kv_fp8, dequantize_kv
 from .packed_metadata import PackedTreeMetadata, ancestor_mask_from_parents
+from .qk_norm_rope import qk_norm_rope, qk_norm_rope_store
+from .request_maps import RequestMaps, build_request_maps
 from .row_linear import RowParallelLinear, row_parallel_linear
 from .paged_backend import packed_tree_attention, packed_tree_attention_reference
 from .sharding import KvHeadShard, shard_for_rank
@@ -35,5 +38,7 @@ __all__ = [
     "packed_tree_attention", "packed_tree_attention_reference", "KvHeadShard",
     "shard_for_rank", "copy_accepted_kv", "scatter_tree_kv", "rope_scatter",
     "rope_scatter_prevalidated", "packed_tree_attention_gqa", "accept_batch", "accept_walk",
-    "RowParallelLinear", "row_parallel_linear",
+    "RowParallelLinear", "row_parallel_linear", "RequestMaps", "build_request_maps",
+    "qk_norm_rope", "qk_norm_rope_store", "alloc_fp8_kv_cache", "copy_accepted_kv_fp8",
+    "dequantize_kv",
 ]

@@ -41,6 +41,10 @@ EXPORTED_SYMBOLS = (
     "jt_ipc_open_handle",
     "jt_ipc_close_handle",
     "jt_kv_commit_max_slots",
+    "jt_request_maps_launch",
+    "jt_qk_norm_rope_launch",
+    "jt_kv_fp8_commit_launch",
+    "jt_kv_fp8_commit_max_slots",
     "jt_abi_version",
     "jt_last_error",
     "jt_read_device_errors",
@@ -155,6 +159,40 @@ class JtRowLinearParams(ctypes.Structure):
     ]
 
 
+def _fields(kind, names):
+    return [(name, kind) for name in names.split()]
+
+
+class JtRequestMapsParams(ctypes.Structure):
+    _fields_ = (
+        _fields(c_void_p, "block_tables cached_lens new_lens free_pages slot_mapping positions "
+                          "token_to_request cu_seqlens context_lens pages_taken")
+        + _fields(c_i64, "table_stride0")
+        + _fields(c_i32, "num_requests table_width block_size num_free max_tokens"))
+
+
+class JtQkNormRopeParams(ctypes.Structure):
+    _fields_ = (
+        _fields(c_void_p, "q k v q_weight k_weight positions cos_sin_cache slots q_out k_out "
+                          "k_pool v_pool k_scale v_scale")
+        + _fields(c_i64, "num_pages max_position q_stride0 q_stride1 k_stride0 k_stride1 "
+                         "v_stride0 v_stride1 qo_stride0 qo_stride1 ko_stride0 ko_stride1 "
+                         "kp_stride0 kp_stride1 kp_stride2 vp_stride0 vp_stride1 vp_stride2 "
+                         "ks_stride0 ks_stride1 vs_stride0 vs_stride1 positions_stride "
+                         "slots_stride cache_stride0")
+        + _fields(ctypes.c_float, "eps")
+        + _fields(c_i32, "rows q_heads kv_heads head_dim page_size dtype weight_dtype "
+                         "cache_dtype store positions_is_int64 slots_is_int64"))
+
+
+class JtKvFp8CommitParams(ctypes.Structure):
+    _fields_ = (
+        _fields(c_void_p, "kv_pool kv_scale source_slots destination_slots")
+        + _fields(c_i64, "num_blocks stride_axis stride_layer stride_block stride_offset "
+                         "stride_head scale_axis scale_layer scale_block scale_head")
+        + _fields(c_i32, "slot_is_int64 num_slots num_layers num_kv_heads head_dim block_size"))
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -198,6 +236,14 @@ def _declare(lib):
     lib.jt_ipc_close_handle.restype = ctypes.c_int
     lib.jt_kv_commit_max_slots.argtypes = []
     lib.jt_kv_commit_max_slots.restype = c_i32
+    lib.jt_request_maps_launch.argtypes = [P(JtRequestMapsParams), c_void_p]
+    lib.jt_request_maps_launch.restype = ctypes.c_int
+    lib.jt_qk_norm_rope_launch.argtypes = [P(JtQkNormRopeParams), c_void_p]
+    lib.jt_qk_norm_rope_launch.restype = ctypes.c_int
+    lib.jt_kv_fp8_commit_launch.argtypes = [P(JtKvFp8CommitParams), c_void_p]
+    lib.jt_kv_fp8_commit_launch.restype = ctypes.c_int
+    lib.jt_kv_fp8_commit_max_slots.argtypes = []
+    lib.jt_kv_fp8_commit_max_slots.restype = c_i32
     lib.jt_abi_version.argtypes = []
     lib.jt_abi_version.restype = c_i32
     lib.jt_last_error.argtypes = []

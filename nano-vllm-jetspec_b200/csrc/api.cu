@@ -45,6 +45,13 @@ extern "C" int jt_read_device_errors(uint32_t* errors) {
   uint32_t g = 0;
   rc = jt_read_errors_f32(&g);
   if (rc != JT_OK) return rc;
-  *errors = a | b | c | d | e | f | g;
+  uint32_t h = 0, i = 0, j = 0;
+  rc = jt_read_errors_maps(&h);
+  if (rc != JT_OK) return rc;
+  rc = jt_read_errors_norm(&i);
+  if (rc != JT_OK) return rc;
+  rc = jt_read_errors_fp8_commit(&j);
+  if (rc != JT_OK) return rc;
+  *errors = a | b | c | d | e | f | g | h | i | j;
   return JT_OK;
 }

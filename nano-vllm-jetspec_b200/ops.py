@@ -13,10 +13,15 @@ functionalisation sees exactly which buffers they write.
 * ``jetspec_b200::kv_store_``       - k_cache / v_cache rows <- key / value
 * ``jetspec_b200::kv_commit_``      - kv_pool accepted rows moved to their destinations
 * ``jetspec_b200::rope_scatter_``   - out <- rope(q); k_pool / v_pool <- rope(k) / v
+* ``jetspec_b200::request_maps_``   - block tables, slots, positions <- request lengths
+* ``jetspec_b200::qk_norm_rope_``   - q_out / k_out <- rotated normed heads
+* ``jetspec_b200::qk_norm_rope_store_`` - q_out and the cache rows <- rotated normed heads
+* ``jetspec_b200::kv_fp8_commit_``  - kv_pool / kv_scale accepted rows moved
 """
 from __future__ import annotations
 
 from types import SimpleNamespace
+from typing import Optional
 
 import torch
 
@@ -90,6 +95,71 @@ def rope_scatter_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
 
 @rope_scatter_.register_fake
 def _(q, k, v, positions, cos_sin_cache, k_pool, v_pool, node_slots, out):
+    return None
+
+
+@torch.library.custom_op(f"{NAMESPACE}::request_maps_",
+                         mutates_args=("block_tables", "slots", "positions", "owners", "cu",
+                                       "lens", "taken"))
+def request_maps_(block_tables: torch.Tensor, cached_lens: torch.Tensor, new_lens: torch.Tensor,
+                  free_pages: torch.Tensor, block_size: int, slots: torch.Tensor,
+                  positions: torch.Tensor, owners: torch.Tensor, cu: torch.Tensor,
+                  lens: torch.Tensor, taken: torch.Tensor) -> None:
+    from .request_maps import _launch_maps
+
+    _launch_maps(block_tables, cached_lens, new_lens, free_pages, block_size, slots, positions,
+                 owners, cu, lens, taken)
+
+
+@request_maps_.register_fake
+def _(block_tables, cached_lens, new_lens, free_pages, block_size, slots, positions, owners, cu,
+      lens, taken):
+    return None
+
+
+@torch.library.custom_op(f"{NAMESPACE}::qk_norm_rope_", mutates_args=("q_out", "k_out"))
+def qk_norm_rope_(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
+                  k_weight: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor,
+                  eps: float, q_out: torch.Tensor, k_out: torch.Tensor) -> None:
+    from .qk_norm_rope import _launch_norm
+
+    _launch_norm(q, k, q_weight, k_weight, positions, cos_sin_cache, eps, q_out, k_out)
+
+
+@qk_norm_rope_.register_fake
+def _(q, k, q_weight, k_weight, positions, cos_sin_cache, eps, q_out, k_out):
+    return None
+
+
+@torch.library.custom_op(f"{NAMESPACE}::qk_norm_rope_store_",
+                         mutates_args=("k_pool", "v_pool", "k_scale", "v_scale", "q_out"))
+def qk_norm_rope_store_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                        q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
+                        cos_sin_cache: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                        slots: torch.Tensor, eps: float, k_scale: Optional[torch.Tensor],
+                        v_scale: Optional[torch.Tensor], q_out: torch.Tensor) -> None:
+    from .qk_norm_rope import _launch_norm
+
+    _launch_norm(q, k, q_weight, k_weight, positions, cos_sin_cache, eps, q_out, None, v, k_pool,
+                 v_pool, slots, k_scale, v_scale)
+
+
+@qk_norm_rope_store_.register_fake
+def _(q, k, v, q_weight, k_weight, positions, cos_sin_cache, k_pool, v_pool, slots, eps, k_scale,
+      v_scale, q_out):
+    return None
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv_fp8_commit_", mutates_args=("kv_pool", "kv_scale"))
+def kv_fp8_commit_(kv_pool: torch.Tensor, kv_scale: torch.Tensor, source_slots: torch.Tensor,
+                   destination_slots: torch.Tensor) -> None:
+    from .fp8_cache import _launch_commit
+
+    _launch_commit(kv_pool, kv_scale, source_slots, destination_slots)
+
+
+@kv_fp8_commit_.register_fake
+def _(kv_pool, kv_scale, source_slots, destination_slots):
     return None
 
 
