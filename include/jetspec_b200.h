@@ -432,6 +432,53 @@ int jt_kv_fp8_commit_launch(const JtKvFp8CommitParams* params, cudaStream_t stre
 int32_t jt_kv_fp8_commit_max_slots(void);
 
 /*
+ * Packed tree attention over an 8-bit paged cache: jt_tree_attn_launch's semantics and
+ * metadata with K / V rows held as e4m3 codes times a power-of-two scale per (slot, KV head):
+ * value = code * 2^(byte - 127), scale byte 255 = NaN.  A single-token decode step is a tree
+ * of one node.  Scores, softmax statistics and sums in fp32; probabilities rounded to bf16
+ * for the PV product, or kept to 16 bits (hi + lo) when the output is f16 or fp32.  A query
+ * row that sees no key gives zeros; a row that sees a key whose K or V scale is NaN gives
+ * NaN; keys a row does not see never reach it, whatever their bytes hold.  Requests with no
+ * nodes are allowed.  Strides of the pools and scales in bytes, of q and out in elements,
+ * last dimensions contiguous; pool rows 16-byte aligned (head_dim a multiple of 16, at most
+ * 128), at most 1024 nodes per tree (larger: device error bit 1, rows not written).
+ */
+typedef struct JtTreeAttnFp8Params {
+  void* out;                       /* [total_queries, q_heads, head_dim], out_dtype      */
+  const void* q;                   /* [total_queries, q_heads, head_dim], dtype          */
+  const void* k_pool;              /* [num_blocks, block_size, kv_heads, head_dim] e4m3 */
+  const void* v_pool;
+  const void* k_scale;             /* [num_blocks, kv_heads, block_size] bytes           */
+  const void* v_scale;
+  const int32_t* cu_seqlens_q;     /* [num_requests + 1]                                */
+  const int32_t* query_to_request; /* [total_queries]                                   */
+  const int32_t* query_local_row;  /* [total_queries]                                   */
+  const int32_t* prefix_lens;      /* [num_requests]                                    */
+  const int32_t* node_counts;      /* [num_requests]                                    */
+  const int32_t* block_tables;     /* [num_requests, table_width] (row stride below)     */
+  const int64_t* tree_slots;       /* [total_queries]                                   */
+  const float* qq_bias;            /* [sum T_r^2] 0 / -inf                              */
+  const int64_t* qq_bias_offsets;  /* [num_requests + 1]                                */
+  void* workspace;                 /* device scratch, zeroed once when allocated         */
+  int64_t workspace_bytes;
+  int64_t num_blocks;
+  int64_t q_stride0, q_stride1, out_stride0, out_stride1, table_stride0;
+  int64_t k_stride0, k_stride1, k_stride2, v_stride0, v_stride1, v_stride2;
+  int64_t ks_stride0, ks_stride1, vs_stride0, vs_stride1;
+  float scale;                     /* > 0                                               */
+  int32_t num_requests, total_queries, num_kv_heads, groups, head_dim, block_size;
+  int32_t table_width;
+  int32_t dtype;                   /* JT_BF16 or JT_F16                                 */
+  int32_t out_dtype;               /* dtype or JT_F32                                   */
+} JtTreeAttnFp8Params;
+
+int jt_tree_attn_fp8_launch(const JtTreeAttnFp8Params* params, cudaStream_t stream);
+/* Bytes of workspace for this geometry (0: none needed), -1 for an invalid one. */
+int64_t jt_tree_attn_fp8_workspace_size(int32_t num_requests, int32_t total_queries,
+                                        int32_t num_kv_heads, int32_t groups,
+                                        int32_t head_dim);
+
+/*
  * Failure detection without a GPU fault: runs one thread that waits, with the kernels'
  * bounded-wait routine and a limit of limit_cycles, on an mbarrier nothing arrives on.
  * Synchronous (diagnostics).  out[0] = 1 if the wait claimed completion (a failure),

@@ -29,6 +29,7 @@ from .row_linear import RowParallelLinear, row_parallel_linear
 from .paged_backend import packed_tree_attention, packed_tree_attention_reference
 from .sharding import KvHeadShard, shard_for_rank
 from .state import _slots_for_blocks, copy_accepted_kv
+from .tree_fp8 import packed_tree_attention_fp8
 from .tree_fusion import rope_scatter, rope_scatter_prevalidated, scatter_tree_kv
 from .tree_gqa import packed_tree_attention_gqa
 
@@ -40,5 +41,5 @@ __all__ = [
     "rope_scatter_prevalidated", "packed_tree_attention_gqa", "accept_batch", "accept_walk",
     "RowParallelLinear", "row_parallel_linear", "RequestMaps", "build_request_maps",
     "qk_norm_rope", "qk_norm_rope_store", "alloc_fp8_kv_cache", "copy_accepted_kv_fp8",
-    "dequantize_kv",
+    "dequantize_kv", "packed_tree_attention_fp8",
 ]

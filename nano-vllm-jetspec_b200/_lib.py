@@ -45,6 +45,8 @@ EXPORTED_SYMBOLS = (
     "jt_qk_norm_rope_launch",
     "jt_kv_fp8_commit_launch",
     "jt_kv_fp8_commit_max_slots",
+    "jt_tree_attn_fp8_launch",
+    "jt_tree_attn_fp8_workspace_size",
     "jt_abi_version",
     "jt_last_error",
     "jt_read_device_errors",
@@ -193,6 +195,19 @@ class JtKvFp8CommitParams(ctypes.Structure):
         + _fields(c_i32, "slot_is_int64 num_slots num_layers num_kv_heads head_dim block_size"))
 
 
+class JtTreeAttnFp8Params(ctypes.Structure):
+    _fields_ = (
+        _fields(c_void_p, "out q k_pool v_pool k_scale v_scale cu_seqlens_q query_to_request "
+                          "query_local_row prefix_lens node_counts block_tables tree_slots "
+                          "qq_bias qq_bias_offsets workspace")
+        + _fields(c_i64, "workspace_bytes num_blocks q_stride0 q_stride1 out_stride0 "
+                         "out_stride1 table_stride0 k_stride0 k_stride1 k_stride2 v_stride0 "
+                         "v_stride1 v_stride2 ks_stride0 ks_stride1 vs_stride0 vs_stride1")
+        + _fields(ctypes.c_float, "scale")
+        + _fields(c_i32, "num_requests total_queries num_kv_heads groups head_dim block_size "
+                         "table_width dtype out_dtype"))
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -244,6 +259,10 @@ def _declare(lib):
     lib.jt_kv_fp8_commit_launch.restype = ctypes.c_int
     lib.jt_kv_fp8_commit_max_slots.argtypes = []
     lib.jt_kv_fp8_commit_max_slots.restype = c_i32
+    lib.jt_tree_attn_fp8_launch.argtypes = [P(JtTreeAttnFp8Params), c_void_p]
+    lib.jt_tree_attn_fp8_launch.restype = ctypes.c_int
+    lib.jt_tree_attn_fp8_workspace_size.argtypes = [c_i32] * 5
+    lib.jt_tree_attn_fp8_workspace_size.restype = c_i64
     lib.jt_abi_version.argtypes = []
     lib.jt_abi_version.restype = c_i32
     lib.jt_last_error.argtypes = []

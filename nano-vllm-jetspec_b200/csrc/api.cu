@@ -52,6 +52,9 @@ extern "C" int jt_read_device_errors(uint32_t* errors) {
   if (rc != JT_OK) return rc;
   rc = jt_read_errors_fp8_commit(&j);
   if (rc != JT_OK) return rc;
-  *errors = a | b | c | d | e | f | g | h | i | j;
+  uint32_t k = 0;
+  rc = jt_read_errors_attn_fp8(&k);
+  if (rc != JT_OK) return rc;
+  *errors = a | b | c | d | e | f | g | h | i | j | k;
   return JT_OK;
 }

@@ -26,6 +26,7 @@ int jt_read_errors_f32(uint32_t* bits);
 int jt_read_errors_maps(uint32_t* bits);
 int jt_read_errors_norm(uint32_t* bits);
 int jt_read_errors_fp8_commit(uint32_t* bits);
+int jt_read_errors_attn_fp8(uint32_t* bits);
 
 // fp32-operand tree attention (tree_attn_f32.cu), for parameters the entry point checked.
 int jt_tree_attn_f32_launch(const JtTreeAttnParams& p, cudaStream_t stream);

@@ -17,6 +17,7 @@ functionalisation sees exactly which buffers they write.
 * ``jetspec_b200::qk_norm_rope_``   - q_out / k_out <- rotated normed heads
 * ``jetspec_b200::qk_norm_rope_store_`` - q_out and the cache rows <- rotated normed heads
 * ``jetspec_b200::kv_fp8_commit_``  - kv_pool / kv_scale accepted rows moved
+* ``jetspec_b200::tree_attention_fp8_`` - out <- tree attention over the 8-bit cache
 """
 from __future__ import annotations
 
@@ -160,6 +161,31 @@ def kv_fp8_commit_(kv_pool: torch.Tensor, kv_scale: torch.Tensor, source_slots: 
 
 @kv_fp8_commit_.register_fake
 def _(kv_pool, kv_scale, source_slots, destination_slots):
+    return None
+
+
+@torch.library.custom_op(f"{NAMESPACE}::tree_attention_fp8_", mutates_args=("out",))
+def tree_attention_fp8_(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor,
+                        v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                        cu_seqlens_q: torch.Tensor, query_to_request: torch.Tensor,
+                        query_local_row: torch.Tensor, prefix_lens: torch.Tensor,
+                        node_counts: torch.Tensor, block_tables: torch.Tensor,
+                        tree_slots: torch.Tensor, qq_bias: torch.Tensor,
+                        qq_bias_offsets: torch.Tensor, scale: float, groups: int) -> None:
+    from .tree_fp8 import _launch_attention
+
+    metadata = SimpleNamespace(
+        cu_seqlens_q=cu_seqlens_q, query_to_request=query_to_request,
+        query_local_row=query_local_row, prefix_lens=prefix_lens, node_counts=node_counts,
+        block_tables=block_tables, tree_slots=tree_slots, qq_bias=qq_bias,
+        qq_bias_offsets=qq_bias_offsets)
+    _launch_attention(out, q, k_pool, v_pool, k_scale, v_scale, metadata, scale, groups)
+
+
+@tree_attention_fp8_.register_fake
+def _(out, q, k_pool, v_pool, k_scale, v_scale, cu_seqlens_q, query_to_request, query_local_row,
+      prefix_lens, node_counts, block_tables, tree_slots, qq_bias, qq_bias_offsets, scale,
+      groups):
     return None
 
 
