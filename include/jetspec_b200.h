@@ -438,7 +438,8 @@ int32_t jt_kv_fp8_commit_max_slots(void);
  * of one node.  Scores, softmax statistics and sums in fp32; probabilities rounded to bf16
  * for the PV product, or kept to 16 bits (hi + lo) when the output is f16 or fp32.  A query
  * row that sees no key gives zeros; a row that sees a key whose K or V scale is NaN gives
- * NaN; keys a row does not see never reach it, whatever their bytes hold.  Requests with no
+ * NaN; keys a row does not see never reach it, whatever their bytes hold.  V values past
+ * bf16's range saturate.  Requests with no
  * nodes are allowed.  Strides of the pools and scales in bytes, of q and out in elements,
  * last dimensions contiguous; pool rows 16-byte aligned (head_dim a multiple of 16, at most
  * 128), at most 1024 nodes per tree (larger: device error bit 1, rows not written).
@@ -459,7 +460,7 @@ typedef struct JtTreeAttnFp8Params {
   const int64_t* tree_slots;       /* [total_queries]                                   */
   const float* qq_bias;            /* [sum T_r^2] 0 / -inf                              */
   const int64_t* qq_bias_offsets;  /* [num_requests + 1]                                */
-  void* workspace;                 /* device scratch, zeroed once when allocated         */
+  void* workspace;                 /* device scratch, 256-byte aligned                     */
   int64_t workspace_bytes;
   int64_t num_blocks;
   int64_t q_stride0, q_stride1, out_stride0, out_stride1, table_stride0;
@@ -473,7 +474,7 @@ typedef struct JtTreeAttnFp8Params {
 } JtTreeAttnFp8Params;
 
 int jt_tree_attn_fp8_launch(const JtTreeAttnFp8Params* params, cudaStream_t stream);
-/* Bytes of workspace for this geometry (0: none needed), -1 for an invalid one. */
+/* Bytes of workspace for this geometry, -1 for an invalid one. */
 int64_t jt_tree_attn_fp8_workspace_size(int32_t num_requests, int32_t total_queries,
                                         int32_t num_kv_heads, int32_t groups,
                                         int32_t head_dim);

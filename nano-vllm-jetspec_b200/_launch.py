@@ -36,10 +36,8 @@ def stream_handle(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(raw_stream(device))
 
 
-def workspace(device: torch.device, nbytes: int, stream: int | None = None, *,
-              zeroed: bool = False) -> torch.Tensor:
-    """Device scratch of at least ``nbytes`` reserved per (device, stream, size), filled with
-    zeros when it is allocated if ``zeroed`` (such scratch is kept apart).
+def workspace(device: torch.device, nbytes: int, stream: int | None = None) -> torch.Tensor:
+    """Device scratch of at least ``nbytes`` reserved per (device, stream, size).
 
     Workspaces are never freed or resized: a CUDA graph that captured a launch keeps
     pointing at the same bytes for as long as the process lives.  Launches on one
@@ -47,12 +45,11 @@ def workspace(device: torch.device, nbytes: int, stream: int | None = None, *,
     """
     if stream is None:
         stream = raw_stream(device)
-    key = (device.index, stream, int(nbytes), zeroed)
+    key = (device.index, stream, int(nbytes))
     with _workspace_lock:
         buffer = _workspaces.get(key)
         if buffer is None:
-            allocate = torch.zeros if zeroed else torch.empty
-            buffer = allocate(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+            buffer = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
             _workspaces[key] = buffer
     return buffer
 

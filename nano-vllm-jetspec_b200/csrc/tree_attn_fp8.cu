@@ -1,108 +1,1447 @@
-// Packed tree attention over an 8-bit paged cache (e4m3 codes, power-of-two row scales).
+// Packed tree attention over an 8-bit paged cache (e4m3 codes, power-of-two row scales) on
+// tcgen05 tensor cores.
 //
 // For query row i (node j, head hq) of request r: keys are positions 0..P+T-1 (prefix pages,
 // then the T tree nodes), visible when the position is below P, or is node n <= j with zero
-// bias.  s = scale * sum_d q_d k_d, p = exp(s - max), out = sum p v / sum p, with
-// k = code * 2^(kbyte - 127) and v likewise.
-#include "common.cuh"
+// bias.  With k = K 2^e, v = V 2^f (K, V codes):
+//   s = scale * 2^e * sum_d q_d K_d,   p = exp(s - max),   out = sum p 2^f V / sum p
+// * Scores on 8-bit operands without loss: a bf16 query element, scaled by the row's power of
+//   two, is the sum of two e4m3 values (4 significant bits each, the second one signed: 8
+//   bits), an f16 one of three.  Q enters as two or three e4m3 tiles against the same K tile
+//   (kind::f8f6f4 runs at twice the bf16 rate, so two terms cost what one bf16 product
+//   would), and K goes from HBM to the tensor core untouched.  2^e multiplies the score
+//   column in the softmax.  Elements below 2^-10 of the row's largest lose low bits, at most
+//   2^-18 of that largest.
+// * PV runs in bf16: a warpgroup expands the V codes (exact in bf16, 2^f folded in) into the
+//   swizzled tile the MMA reads.  P is rounded to bf16 (8 bits, as in the 16-bit cache's
+//   kernel); f16 and fp32 outputs take P as hi + lo bf16 (16 bits).
+//
+// Work: an item is (request, KV head, m-block), an m-block one or two 128-row query tiles;
+// the items' 128-key tiles, weighted by their tensor time, form one line that is cut into
+// equal parts, one per CTA, so every SM streams the same amount whatever the lengths.  Every
+// CTA scans the lengths itself and finds its part: no plan kernel, no queue.  An item cut
+// between CTAs leaves unnormalised fp32 partials that a second small kernel merges (a
+// programmatic dependent; it returns at once when nothing was cut).
+//
+// Two softmax streams per CTA keep the tensor core busy while the other one works.  With two
+// query tiles (trees of more than 128 rows) each stream owns a tile and both use every K / V
+// tile; with one, the streams take alternate key tiles of the same rows and their (max, sum,
+// O) are merged at the end.
+//
+//   warp 0       MMA issuer, TMEM owner (S0, S1, O0, O1: 128 columns each)
+//   warp 1       work pieces; TMA loads of K, V and scale bytes for prefix tiles
+//   warps 2-3    scale factors of every tile; cp.async gathers of tiles that touch tree nodes
+//                or pages TMA cannot box
+//   warps 4-7    queries -> e4m3 terms; V codes -> bf16 tile
+//   warps 8-15   softmax + epilogue, one warpgroup per stream, one thread per row
+//
+// Every mbarrier wait is bounded; one that runs out sets JT_DEVERR_TIMEOUT and the CTA's
+// abort flag, all roles leave their loops, drain what they started and free the TMEM.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
-#include <cuda_fp8.h>
+#include <algorithm>
+
+#include "common.cuh"
 
 namespace {
 
 __device__ uint32_t g_attn_fp8_errors;
 
-constexpr int kThreads = 128;
+constexpr int kN = 128;               // keys per tile
+constexpr int kM = 128;               // rows per query tile
+constexpr int kD = 128;               // head dim in shared memory (shorter heads: zeros)
+constexpr int kThreads = 512;
+constexpr int kKRing = 3, kVRing = 2, kScaleRing = 4;
+constexpr int kTile8 = kN * kD;       // bytes of a code tile
+constexpr int kTile16 = 2 * kTile8;   // bytes of a bf16 tile: two 64-dim halves
+constexpr int kHalf16 = kTile8;
+constexpr int kMaxCtas = 160;         // workspace slots are sized for this many SMs
+constexpr int kMaxNodes = 1024;
+// Costs in units of one 128-row, 128-key tile: an item's fixed cost (query load, pipeline
+// fill, epilogue), and the least part worth a CTA of its own.
+constexpr int kItemCost = 3;
+constexpr int kMinPart = 6;
+constexpr int kMinTiles = 2;          // cuts closer than this to an item's end move to it
+constexpr long long kWaitLimit = 4000000000ll;  // cycles (~2 s) per wait
 
-__device__ __forceinline__ float code_value(uint8_t c) {
-  __nv_fp8_e4m3 v;
-  v.__x = c;
-  return static_cast<float>(v);
+// ---- shared memory ------------------------------------------------------------------
+template <bool kWide>
+struct Smem {
+  static constexpr int kTerms = kWide ? 3 : 2;   // e4m3 terms of a query element
+  static constexpr int kTiles = kWide ? 1 : 2;   // query tiles per item
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + kTiles * kTerms * kTile8;
+  static constexpr int kV8 = kK + kKRing * kTile8;
+  static constexpr int kV16 = kV8 + kVRing * kTile8;
+  static constexpr int kScale = kV16 + 2 * kTile16;          // [kScaleRing][K, V][128] bytes
+  static constexpr int kKf = kScale + kScaleRing * 256;       // [2][128] float
+  static constexpr int kVm = kKf + 2 * kN * 4;                // [2][128] uint2
+  static constexpr int kQfac = kVm + 2 * kN * 8;              // [2][2][128] float
+  static constexpr int kX = kQfac + 4 * kM * 4;               // [2][128] float2: max, sum
+  static constexpr int kItem = kX + 2 * kM * 8;               // [2][16] int
+  static constexpr int kFlag = kItem + 2 * 64;                // [2][2] int
+  static constexpr int kMisc = kFlag + 32;                    // TMEM base, abort
+  static constexpr int kBar = kMisc + 32;
+  static constexpr int kBytes = kBar + 8 * 32 + 1024;         // + alignment slack
+  static_assert(kBytes <= 227 * 1024, "shared memory per CTA");
+};
+
+// ---- barriers -------------------------------------------------------------------------
+constexpr int kBarKFull = 0;     // [3] TMA (arrive_tx + arrive) or two gather warps
+constexpr int kBarKEmpty = 3;    // [3] commit after the tile's last QK
+constexpr int kBarVFull = 6;     // [2] TMA or two gather warps
+constexpr int kBarVEmpty = 8;    // [2] 4 converter warps
+constexpr int kBarFac = 10;      // [2] 2 gather warps: the tile's factors are written
+constexpr int kBarBFull = 12;    // [2] 4 converter warps: the tile's bf16 V is written
+constexpr int kBarBEmpty = 14;   // [2] commit after the tile's last PV
+constexpr int kBarQFull = 16;    // [2] 4 converter warps, by piece parity
+constexpr int kBarQEmpty = 18;   // commit after a piece's last QK
+constexpr int kBarSFull = 19;    // [2] commit per QK, by stream
+constexpr int kBarPFull = 21;    // [2] 4 softmax warps, by stream
+constexpr int kBarODone = 23;    // commit after a piece's last PV
+constexpr int kBarOFree = 24;    // 8 softmax warps: the epilogue has read O
+constexpr int kBarX = 25;        // 8 softmax warps: (max, sum) exchanged
+constexpr int kBarItemFull = 26;   // [2] publisher
+constexpr int kBarItemEmpty = 28;  // [2] every warp
+constexpr int kBarDrain = 30;
+constexpr int kNumBars = 31;
+static_assert(kNumBars <= 32, "barrier area");
+
+__device__ __forceinline__ uint32_t bar_count(int i) {
+  if (i < kBarKEmpty) return 2;
+  if (i < kBarVFull) return 1;
+  if (i < kBarVEmpty) return 2;
+  if (i < kBarFac) return 4;
+  if (i < kBarBFull) return 2;
+  if (i < kBarBEmpty) return 4;
+  if (i < kBarQFull) return 1;
+  if (i < kBarQEmpty) return 4;
+  if (i < kBarPFull) return 1;   // QEmpty, SFull
+  if (i < kBarODone) return 4;
+  if (i == kBarODone) return 1;
+  if (i < kBarItemFull) return 8;
+  if (i < kBarItemEmpty) return 1;
+  if (i < kBarDrain) return kThreads / 32;
+  return 1;
 }
+
+// TMEM columns.
+__device__ __forceinline__ constexpr uint32_t col_s(int s) { return 128u * s; }
+__device__ __forceinline__ constexpr uint32_t col_o(int s) { return 256u + 128u * s; }
+
+// ---- PTX ------------------------------------------------------------------------------
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
+                                            bool abortable) {
+  const long long start = clock64();
+  for (;;) {
+    if (mbar_try(bar, parity)) return true;
+    if (abortable && *abort) return false;
+    if (clock64() - start > kWaitLimit) {
+      *abort = 1;
+      atomicOr(&g_attn_fp8_errors, JT_DEVERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort,
+                                          bool abortable = true) {
+  if (mbar_try(bar, parity)) return true;
+  return mbar_wait_slow(bar, parity, abort, abortable);
+}
+__device__ __forceinline__ void warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  mbar_wait(bar, parity, abort);
+  __syncwarp();
+}
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+__device__ __forceinline__ void fence_proxy_async() {
+  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+}
+// Warp-wide forms: elect.sync picks the one issuing lane (always the same for a full warp).
+__device__ __forceinline__ void commit_warp(uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
+          bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f8_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                            uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts_warp(uint32_t d, uint32_t a_tmem, uint64_t b,
+                                            uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
+}
+// Shared-memory matrix descriptor, 128-byte swizzle (sm_100 descriptor version 1).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  uint64_t d = static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
+  d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32;
+  d |= 1ull << 46;
+  d |= 2ull << 61;
+  return d;
+}
+// Instruction descriptors, M128 N128, fp32 accumulator: e4m3 x e4m3 (both K-major), and
+// bf16 x bf16 with an MN-major B.
+constexpr uint32_t kIdescQK = (1u << 4) | (static_cast<uint32_t>(kN >> 3) << 17) |
+                              (static_cast<uint32_t>(kM >> 4) << 24);
+constexpr uint32_t kIdescPV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
+                              (static_cast<uint32_t>(kD >> 3) << 17) |
+                              (static_cast<uint32_t>(kM >> 4) << 24);
+
+#define JT_LD32_REGS(v)                                                                      \
+  "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),        \
+      "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),             \
+      "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),          \
+      "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),          \
+      "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),          \
+      "=r"(v[31])
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : JT_LD32_REGS(v)
+      : "r"(taddr));
+}
+#undef JT_LD32_REGS
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+      "%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+      "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+      "%13,%14,%15,%16};\n" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1,
+                                            int c2, int c3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::
+          "r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+template <int kRegs>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegs));
+}
+// Registers per thread of the four warpgroups: 88 + 72 + 2 x 176 = 512 = 4 x the 128 of the
+// launch, so every increase is covered by the decreases.
+constexpr int kRegsLoad = 88, kRegsConvert = 72, kRegsSoftmax = 176;
+static_assert(kRegsLoad + kRegsConvert + 2 * kRegsSoftmax <= 4 * (65536 / kThreads), "registers");
+
+// ---- numbers --------------------------------------------------------------------------
 // 2^(byte - 127); byte 255 is NaN, byte 0 the subnormal 2^-127.
-__device__ __forceinline__ float scale_value(uint8_t b) {
-  if (b == 255) return __uint_as_float(0x7fc00000u);
-  return b == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(static_cast<uint32_t>(b) << 23);
+__device__ __forceinline__ float scale_value(uint32_t b) {
+  if (b == 255u) return __uint_as_float(0x7fc00000u);
+  return b == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(b << 23);
+}
+// Multipliers that take a code widened by widen() to its value in bf16: 2^(120 + byte - 127),
+// as a product of two where that exceeds bf16's range.  A NaN scale gives zero: the V row is
+// kept out of the product, and the key's score is NaN for the rows that see it.
+__device__ __forceinline__ uint2 v_multipliers(uint32_t b) {
+  if (b == 255u) return make_uint2(0u, 0x3f803f80u);
+  const int k = static_cast<int>(b) - 7;  // 120 + b - 127
+  const int e1 = min(k, 127), e2 = k - e1;
+  const uint32_t m1 = static_cast<uint32_t>(e1 + 127) << 7, m2 = static_cast<uint32_t>(e2 + 127) << 7;
+  return make_uint2(m1 | (m1 << 16), m2 | (m2 << 16));
+}
+// Four e4m3 codes as bf16 pairs of value * 2^-120: the code's exponent and mantissa fields
+// dropped into bf16's (subnormal codes become bf16 subnormals of the same value).  The code
+// 0x7f (NaN), which no row of this cache holds, reads as 480: finite, so bytes of keys no row
+// sees never reach the product.
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t a = __byte_perm(w, 0u, 0x1404), b = __byte_perm(w, 0u, 0x3424);
+  lo = ((a >> 4) & 0x07f007f0u) | (a & 0x80008000u);
+  hi = ((b >> 4) & 0x07f007f0u) | (b & 0x80008000u);
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t clamp_bf16x2(uint32_t a) {
+  uint32_t r;
+  asm("{\n .reg .b32 t;\n min.bf16x2 t, %1, %2;\n max.bf16x2 %0, t, %3;\n}\n"
+      : "=r"(r)
+      : "r"(a), "r"(0x7f7f7f7fu), "r"(0xff7fff7fu));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_e4m3(uint32_t pair) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"(static_cast<uint16_t>(pair)));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  return jt::MmaOp<__nv_bfloat16>::pack(lo, hi);
 }
 
-// One CTA per (packed node, query head): 128 keys at a time, a score per thread, then an
-// output element per thread.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) tree_attn_fp8_kernel(const JtTreeAttnFp8Params p) {
-  __shared__ float sq[128], prob[kThreads], red[kThreads / 32];
-  __shared__ int64_t place[kThreads], vplace[kThreads];
-  const int node = blockIdx.x, hq = blockIdx.y, h = hq / p.groups, tid = threadIdx.x;
-  const int r = p.query_to_request[node], j = p.query_local_row[node];
-  const int P = max(p.prefix_lens[r], 0), T_r = p.node_counts[r], q0 = p.cu_seqlens_q[r];
-  if (T_r > 1024) {
-    if (tid == 0) atomicOr(&g_attn_fp8_errors, JT_DEVERR_TREE_TOO_LARGE);
+// exp2 of a score pair on the FMA pipe, relieving the special-function unit: 2^x = 2^j 2^f with
+// j = rint(x) from the float rounding trick and 2^f, |f| <= 1/2, from a cubic fitted to the
+// least relative error on that interval (8.4e-5, below the bf16 rounding of P).
+__device__ __forceinline__ float2 exp2_poly2(float2 x) {
+  x = make_float2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
+  const float2 t = __fadd2_rn(x, make_float2(12582912.f, 12582912.f));
+  const float2 j = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = __fadd2_rn(x, make_float2(-j.x, -j.y));
+  float2 q = __ffma2_rn(make_float2(0.05521299f, 0.05521299f), f,
+                        make_float2(0.24271414f, 0.24271414f));
+  q = __ffma2_rn(q, f, make_float2(0.69326216f, 0.69326216f));
+  q = __ffma2_rn(q, f, make_float2(0.9999196f, 0.9999196f));
+  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+}
+
+// ---- the work line ----------------------------------------------------------------------
+struct Geometry {
+  int groups, npt, npi;  // nodes per query tile, per item
+};
+struct ItemInfo {
+  int key_end, n, weight, cost;
+};
+__device__ __forceinline__ ItemInfo item_info(const Geometry& ge, int P, int T, int mb) {
+  const int first = mb * ge.npi, last = min(T, first + ge.npi);
+  ItemInfo it;
+  it.key_end = P + last;
+  it.n = (it.key_end + kN - 1) / kN;
+  it.weight = last - first > ge.npt ? 2 : 1;
+  it.cost = it.n * it.weight + kItemCost;
+  return it;
+}
+// A request as the kernel takes it: no nodes when it has none or is refused.
+__device__ __forceinline__ void load_request(const JtTreeAttnFp8Params& p, int r, int& P, int& T,
+                                             bool flag) {
+  P = __ldg(p.prefix_lens + r);
+  T = __ldg(p.node_counts + r);
+  const int64_t capacity = static_cast<int64_t>(p.table_width) * p.block_size;
+  if (T > kMaxNodes) {
+    if (flag) atomicOr(&g_attn_fp8_errors, JT_DEVERR_TREE_TOO_LARGE);
+    T = 0;
+  }
+  if (P < 0 || P > capacity) {
+    if (flag) atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
+    P = P < 0 ? 0 : static_cast<int>(capacity);
+  }
+  T = max(T, 0);
+}
+__device__ __forceinline__ int64_t head_cost(const Geometry& ge, int P, int T) {
+  int64_t c = 0;
+  for (int mb = 0; mb * ge.npi < T; ++mb) c += item_info(ge, P, T, mb).cost;
+  return c;
+}
+// Tile of an item at which a cut at line position x falls.
+__device__ __forceinline__ int cut_tile(const ItemInfo& it, int64_t start, int64_t x) {
+  if (x <= start) return 0;
+  if (x >= start + it.cost) return it.n;
+  const int t = static_cast<int>((x - start) / it.weight);
+  if (t < kMinTiles) return 0;
+  if (it.n - t < kMinTiles) return it.n;
+  return t;
+}
+
+struct Piece {
+  int r, h, mb, P, T, q_start, t0, n, key_end, two, slot, last;
+};
+// A piece's partial slot in the workspace, or -1 for a whole item.
+struct PieceMeta {
+  int valid, finishes, r, h, mb, pad[3];
+};
+struct Workspace {
+  PieceMeta* meta;   // [2 * kMaxCtas]
+  float2* ml;        // [slot][tile][128] max (log2 units), sum
+  float4* o;         // [slot][tile][32 groups of 4 columns][128]
+};
+constexpr int64_t kMetaBytes = 2 * kMaxCtas * sizeof(PieceMeta);
+constexpr int64_t kMlBytes = 2ll * kMaxCtas * 2 * kM * sizeof(float2);
+constexpr int64_t kPartBytes = 2ll * kMaxCtas * 2 * kM * kD * sizeof(float);
+static_assert(kMetaBytes % 256 == 0 && kMlBytes % 256 == 0, "workspace alignment");
+__host__ __device__ __forceinline__ Workspace carve(void* base) {
+  char* b = static_cast<char*>(base);
+  return Workspace{reinterpret_cast<PieceMeta*>(b), reinterpret_cast<float2*>(b + kMetaBytes),
+                   reinterpret_cast<float4*>(b + kMetaBytes + kMlBytes)};
+}
+
+// How tiles reach shared memory, decided on the host from the layout.
+struct LoadPlan {
+  int tma;   // prefix tiles by TMA boxes of `box` keys, their scale bytes by bulk copies
+  int box;
+};
+
+// Visibility words of the 128 keys at kb for this lane's row: bit b of word w is key
+// kb + 32 w + b.  Each warp builds its rows' words node by node: lane b reads the bias of its
+// key, a ballot collects the word, and the lanes of that node keep it.
+__device__ __forceinline__ void mask_words(const float* bias, int kb, int P, int T, int key_end,
+                                           int j, bool ok, uint32_t (&mw)[4]) {
+  const int lane = threadIdx.x & 31;
+  mw[0] = mw[1] = mw[2] = mw[3] = 0u;
+  const int lo = __reduce_min_sync(0xffffffffu, ok ? j : 0x7fffffff);
+  const int hi = __reduce_max_sync(0xffffffffu, ok ? j : -1);
+  for (int base = lo; base <= hi; base += 4) {
+    float b[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int node = base + i, key = kb + 32 * w + lane - P;
+        b[i][w] = -INFINITY;
+        if (node <= hi && kb + 32 * w + lane < key_end) {
+          if (key < 0)
+            b[i][w] = 0.f;
+          else if (key <= node)
+            b[i][w] = __ldg(bias + static_cast<int64_t>(node) * T + key);
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t bits = __ballot_sync(0xffffffffu, b[i][w] == 0.f);
+        if (ok && j == base + i) mw[w] = bits;
+      }
+  }
+}
+
+// Softmax of one row of a 128-key tile: scores from TMEM, scaled by the keys' factors, the
+// lazy running maximum (moved only when a tile exceeds it by 2^8, so P stays below 2^8 and O
+// is rarely rescaled), P to the S columns it came from.  kCareful (masked tiles, tiles with a
+// NaN row): masked scores are -inf and every exponential is exp2, which keeps a NaN.
+template <bool kWide, bool kCareful>
+__device__ __forceinline__ void softmax_row(uint32_t s_addr, const float* kf, float c_row,
+                                            const uint32_t (&mw)[4], float& m_run, float& l_run,
+                                            float& alpha) {
+  uint32_t v[4][32];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + 32 * q, v[q]);
+  tmem_wait_ld();
+  float mx4[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float4* f4 = reinterpret_cast<const float4*>(kf + 32 * q);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float4 f = f4[k];
+      const float2 a = __fmul2_rn(make_float2(__uint_as_float(v[q][4 * k]), __uint_as_float(v[q][4 * k + 1])),
+                                  make_float2(f.x, f.y));
+      const float2 b = __fmul2_rn(make_float2(__uint_as_float(v[q][4 * k + 2]), __uint_as_float(v[q][4 * k + 3])),
+                                  make_float2(f.z, f.w));
+      v[q][4 * k] = __float_as_uint(a.x);
+      v[q][4 * k + 1] = __float_as_uint(a.y);
+      v[q][4 * k + 2] = __float_as_uint(b.x);
+      v[q][4 * k + 3] = __float_as_uint(b.y);
+    }
+    if constexpr (kCareful) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k)
+        if (!((mw[q] >> k) & 1u)) v[q][k] = 0xff800000u;
+    }
+    float m8[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      m8[k] = fmaxf(fmaxf(__uint_as_float(v[q][k]), __uint_as_float(v[q][k + 8])),
+                    fmaxf(__uint_as_float(v[q][k + 16]), __uint_as_float(v[q][k + 24])));
+    mx4[q] = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
+                   fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+  }
+  const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * c_row;
+  alpha = 1.f;
+  if (mx > m_run + 8.f) {
+    if (m_run != -INFINITY) alpha = jt::fast_exp2(m_run - mx);
+    m_run = mx;
+  }
+  const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+  const float2 c2 = make_float2(c_row, c_row), n2 = make_float2(neg_m, neg_m);
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t ph[16], pl[kWide ? 16 : 1];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float2 x = __ffma2_rn(
+          make_float2(__uint_as_float(v[q][2 * k]), __uint_as_float(v[q][2 * k + 1])), c2, n2);
+      float2 e;
+      if (!kCareful && !kWide && (k & 3) == 3)
+        e = exp2_poly2(x);
+      else
+        e = make_float2(jt::fast_exp2(x.x), jt::fast_exp2(x.y));
+      sum[k & 1] = __fadd2_rn(sum[k & 1], e);
+      ph[k] = pack_bf16(e.x, e.y);
+      if constexpr (kWide) {
+        const float2 h = jt::MmaOp<__nv_bfloat16>::unpack(ph[k]);
+        pl[k] = pack_bf16(e.x - h.x, e.y - h.y);
+      }
+    }
+    tmem_st16(s_addr + 16 * q, ph);
+    if constexpr (kWide) tmem_st16(s_addr + 64 + 16 * q, pl);
+  }
+  l_run = l_run * alpha + ((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y));
+}
+
+// 32 output columns of one row.
+__device__ __forceinline__ void store_columns(const JtTreeAttnFp8Params& p, int64_t at,
+                                              const float (&o)[32], int columns) {
+  if (p.out_dtype == JT_F32) {
+    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (4 * k < columns) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
     return;
   }
-  const int D = p.head_dim;
-  const T* q = static_cast<const T*>(p.q) + node * p.q_stride0 + hq * p.q_stride1;
-  if (tid < D) sq[tid] = static_cast<float>(q[tid]);
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (8 * k >= columns) continue;
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w[e] = p.out_dtype == JT_BF16 ? pack_bf16(o[8 * k + 2 * e], o[8 * k + 2 * e + 1])
+                                    : jt::MmaOp<__half>::pack(o[8 * k + 2 * e], o[8 * k + 2 * e + 1]);
+    dst[k] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <bool kWide>
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_attn_fp8_kernel(const __grid_constant__ JtTreeAttnFp8Params p,
+                         const __grid_constant__ CUtensorMap kmap,
+                         const __grid_constant__ CUtensorMap vmap, const LoadPlan plan) {
+  using L = Smem<kWide>;
+  constexpr int kTerms = L::kTerms;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = jt::smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  unsigned char* sbase = smem_raw + (base - raw);
+  const uint32_t bar0 = base + L::kBar;
+#define JT_BAR(i) (bar0 + 8u * static_cast<uint32_t>(i))
+  volatile int* misc = reinterpret_cast<volatile int*>(sbase + L::kMisc);
+  volatile int* abort = misc + 1;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Geometry ge{p.groups, kM / p.groups, (kM / p.groups) * L::kTiles};
+
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  if (tid < kNumBars) mbar_init(JT_BAR(tid), bar_count(tid));
+  if (tid == 0) {
+    misc[1] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(
+                     base + L::kMisc)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+
+  // This CTA's part of the work line: a block-wide scan of the requests' costs (a contiguous
+  // run of requests per thread), then the request that holds the part's start.
+  int64_t* scan = reinterpret_cast<int64_t*>(sbase + L::kV16);  // not in use yet
+  const int R = p.num_requests, per = (R + kThreads - 1) / kThreads;
+  const int r_lo = min(tid * per, R), r_hi = min(r_lo + per, R);
+  int64_t mine = 0;
+  for (int r = r_lo; r < r_hi; ++r) {
+    int P, T;
+    load_request(p, r, P, T, blockIdx.x == 0);
+    mine += head_cost(ge, P, T) * p.num_kv_heads;
+  }
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) scan[warp] = incl;
   __syncthreads();
-  const int32_t* table = p.block_tables + r * p.table_stride0;
-  const float* bias = p.qq_bias + p.qq_bias_offsets[r] + static_cast<int64_t>(j) * T_r;
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int k0 = 0; k0 < P + j + 1; k0 += kThreads) {
-    const int pos = k0 + tid;
-    int64_t slot = -1;
-    if (pos < P) {
-      const int col = pos / p.block_size;
-      if (col < p.table_width) slot = static_cast<int64_t>(table[col]) * p.block_size + pos % p.block_size;
-    } else if (pos <= P + j && bias[pos - P] == 0.f) {
-      slot = p.tree_slots[q0 + pos - P];
+  int64_t before = 0, total = 0;
+  for (int k = 0; k < kThreads / 32; ++k) {
+    if (k < warp) before += scan[k];
+    total += scan[k];
+  }
+  const int64_t my_start = before + incl - mine;
+  const int parts = static_cast<int>(
+      max(static_cast<int64_t>(1), min(static_cast<int64_t>(gridDim.x), total / kMinPart)));
+  const bool has_part = static_cast<int>(blockIdx.x) < parts && total > 0;
+  const int64_t x0 = has_part ? total * blockIdx.x / parts : 0;
+  const int64_t x1 = has_part ? total * (blockIdx.x + 1) / parts : 0;
+  if (has_part && mine > 0 && my_start <= x0 && x0 < my_start + mine) {
+    int64_t s = my_start;
+    for (int r = r_lo; r < r_hi; ++r) {
+      int P, T;
+      load_request(p, r, P, T, false);
+      const int64_t c = head_cost(ge, P, T) * p.num_kv_heads;
+      if (x0 < s + c) {
+        scan[32] = r;
+        scan[33] = s;
+        break;
+      }
+      s += c;
     }
-    const bool want = pos < P || (pos <= P + j && bias[pos - P] == 0.f);
-    if (slot < 0 || slot >= p.num_blocks * p.block_size) {
-      if (want) atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
-      slot = -1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = static_cast<uint32_t>(misc[0]);
+  const int r_start = has_part ? static_cast<int>(scan[32]) : R;
+  const int64_t s_start = has_part ? scan[33] : 0;
+  __syncthreads();  // the scan area is free
+
+  // Pieces: a two-entry ring in shared memory, filled one piece ahead by warp 1's first lane.
+  volatile int* item_ring = reinterpret_cast<volatile int*>(sbase + L::kItem);
+  auto next_piece = [&](uint32_t seq, Piece& it) -> bool {
+    const int slot = seq & 1;
+    int ok = 0;
+    if (mbar_wait(JT_BAR(kBarItemFull + slot), (seq >> 1) & 1, abort) && !*abort) {
+      volatile int* e = item_ring + 16 * slot;
+      it.r = e[0]; it.h = e[1]; it.mb = e[2]; it.P = e[3]; it.T = e[4]; it.q_start = e[5];
+      it.t0 = e[6]; it.n = e[7]; it.key_end = e[8]; it.two = e[9]; it.slot = e[10];
+      it.last = e[11];
+      ok = e[12];
     }
-    float s = -INFINITY, vf = 0.f;
-    place[tid] = -1;
-    if (slot >= 0) {
-      const int64_t page = slot / p.block_size, off = slot % p.block_size;
-      const uint8_t* k = static_cast<const uint8_t*>(p.k_pool) + page * p.k_stride0 +
-                         off * p.k_stride1 + h * p.k_stride2;
-      s = 0.f;
-      for (int d = 0; d < D; ++d) s += sq[d] * code_value(k[d]);
-      s *= scale_value(static_cast<const uint8_t*>(p.k_scale)[page * p.ks_stride0 + h * p.ks_stride1 + off]);
-      s *= p.scale;
-      vf = scale_value(static_cast<const uint8_t*>(p.v_scale)[page * p.vs_stride0 + h * p.vs_stride1 + off]);
-      place[tid] = page * p.v_stride0 + off * p.v_stride1 + h * p.v_stride2;
+    ok = __all_sync(0xffffffffu, ok != 0);
+    if (lane == 0) mbar_arrive(JT_BAR(kBarItemEmpty + slot));
+    return ok != 0;
+  };
+
+  if (warp < 4) {
+    regs_dec<kRegsLoad>();
+    if (warp == 0) {
+      // ---------------------------------------------------------------- MMA issuer
+      // QK of a stream's next tile is issued right behind the PV that reads P out of the same
+      // S buffer: MMAs of one thread execute in order.
+      uint32_t g0 = 0, seq = 0;
+      uint32_t p_phase[2] = {0, 0};
+      const uint64_t q_desc = smem_desc(base + L::kQ, 16, 1024);
+      const uint64_t k_desc = smem_desc(base + L::kK, 16, 1024);
+      const uint64_t v_desc = smem_desc(base + L::kV16, kHalf16, 1024);
+      auto wait_k = [&](uint32_t g) {
+        mbar_wait(JT_BAR(kBarKFull + g % kKRing), (g / kKRing) & 1, abort);
+        tc_fence_after();
+      };
+      auto qk = [&](uint32_t g, int s, int tile) {
+        const uint64_t kd = k_desc + (g % kKRing) * (kTile8 >> 4);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+          for (int kk = 0; kk < kD / 32; ++kk)
+            mma_f8_warp(tmem + col_s(s), q_desc + ((tile * kTerms + term) * kTile8 + kk * 32) / 16,
+                        kd + kk * 2, kIdescQK, (term | kk) != 0 ? 1u : 0u);
+        commit_warp(JT_BAR(kBarSFull + s));
+      };
+      auto pv = [&](uint32_t g, int s, bool acc) {
+        mbar_wait(JT_BAR(kBarPFull + s), p_phase[s], abort);
+        p_phase[s] ^= 1u;
+        tc_fence_after();
+        const uint64_t vd = v_desc + (g & 1) * (kTile16 >> 4);
+#pragma unroll
+        for (int kk = 0; kk < kN / 16; ++kk) {
+          mma_ts_warp(tmem + col_o(s), tmem + col_s(s) + 8 * kk, vd + kk * (2048 / 16), kIdescPV,
+                      acc || kk > 0 ? 1u : 0u);
+          if constexpr (kWide)
+            mma_ts_warp(tmem + col_o(s), tmem + col_s(s) + 64 + 8 * kk, vd + kk * (2048 / 16),
+                        kIdescPV, 1u);
+        }
+      };
+      for (;; ++seq) {
+        Piece it;
+        if (!next_piece(seq, it)) break;
+        const int n = it.n;
+        mbar_wait(JT_BAR(kBarQFull + (seq & 1)), (seq >> 1) & 1, abort);
+        tc_fence_after();
+        auto k_done = [&](uint32_t g, int t) {
+          commit_warp(JT_BAR(kBarKEmpty + g % kKRing));
+          if (t == n - 1) commit_warp(JT_BAR(kBarQEmpty));
+        };
+        if (it.two) {
+          wait_k(g0);
+          qk(g0, 0, 0);
+          qk(g0, 1, 1);
+          k_done(g0, 0);
+        } else {
+          for (int t = 0; t < min(2, n); ++t) {
+            wait_k(g0 + t);
+            qk(g0 + t, t, 0);
+            k_done(g0 + t, t);
+          }
+        }
+        for (int t = 0; t < n; ++t) {
+          const uint32_t g = g0 + t;
+          mbar_wait(JT_BAR(kBarBFull + (g & 1)), (g >> 1) & 1, abort);
+          if (t == 0 && seq > 0) mbar_wait(JT_BAR(kBarOFree), (seq - 1) & 1, abort);
+          if (it.two) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              pv(g, s, t > 0);
+              if (s == 1) commit_warp(JT_BAR(kBarBEmpty + (g & 1)));
+              if (t + 1 < n) {
+                if (s == 0) wait_k(g + 1);
+                qk(g + 1, s, s);
+                if (s == 1) k_done(g + 1, t + 1);
+              }
+            }
+          } else {
+            const int s = t & 1;
+            pv(g, s, t > 1);
+            commit_warp(JT_BAR(kBarBEmpty + (g & 1)));
+            if (t + 2 < n) {
+              wait_k(g + 2);
+              qk(g + 2, s, 0);
+              k_done(g + 2, t + 2);
+            }
+          }
+        }
+        commit_warp(JT_BAR(kBarODone));
+        g0 += n;
+      }
+      commit_warp(JT_BAR(kBarDrain));
+      mbar_wait(JT_BAR(kBarDrain), 0, abort, false);
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- pieces and TMA
+      // The whole warp follows the pieces; its first lane does the work.
+      int r = r_start, h = 0, mb = 0, P = 0, T = 0;
+      int64_t s_item = s_start;
+      bool more = has_part;
+      int meta_valid[2] = {0, 0};
+      if (lane == 0 && more) {
+        load_request(p, r, P, T, false);
+        const int64_t ch = head_cost(ge, P, T);
+        h = static_cast<int>((x0 - s_item) / ch);
+        s_item += ch * h;
+        for (;;) {
+          const ItemInfo it = item_info(ge, P, T, mb);
+          if (x0 < s_item + it.cost) break;
+          s_item += it.cost;
+          ++mb;
+        }
+      }
+      auto publish = [&](uint32_t seq) {
+        const int slot = seq & 1;
+        if (seq >= 2) mbar_wait(JT_BAR(kBarItemEmpty + slot), ((seq >> 1) - 1) & 1, abort);
+        volatile int* e = item_ring + 16 * slot;
+        e[12] = 0;
+        while (more && !*abort) {
+          const ItemInfo it = item_info(ge, P, T, mb);
+          const int tb = cut_tile(it, s_item, x0), te = cut_tile(it, s_item, x1);
+          const bool found = te > tb;
+          if (found) {
+            const bool whole = tb == 0 && te == it.n;
+            const int which = tb == 0 ? 1 : 0;
+            const int part = whole ? -1 : 2 * static_cast<int>(blockIdx.x) + which;
+            e[0] = r; e[1] = h; e[2] = mb; e[3] = P; e[4] = T;
+            e[5] = __ldg(p.cu_seqlens_q + r);
+            e[6] = tb; e[7] = te - tb; e[8] = it.key_end; e[9] = it.weight == 2 ? 1 : 0;
+            e[10] = part; e[11] = te == it.n; e[12] = 1;
+            if (!whole) {
+              PieceMeta* m = carve(p.workspace).meta + part;
+              m->finishes = te == it.n;
+              m->r = r;
+              m->h = h;
+              m->mb = mb;
+              meta_valid[which] = 1;
+            }
+          }
+          // On to the next item of the line.
+          s_item += it.cost;
+          if (s_item >= x1) {
+            more = false;
+          } else {
+            ++mb;
+            if (mb * ge.npi >= T) {
+              mb = 0;
+              if (++h == p.num_kv_heads) {
+                h = 0;
+                do {
+                  ++r;
+                  if (r < R) load_request(p, r, P, T, false);
+                } while (r < R && T == 0);
+                if (r >= R) more = false;
+              }
+            }
+          }
+          if (found) break;
+        }
+        mbar_arrive(JT_BAR(kBarItemFull + slot));
+      };
+      uint32_t g0 = 0, k_used = 0, v_used = 0;
+      if (lane == 0) publish(0);
+      const char* ksc = static_cast<const char*>(p.k_scale);
+      const char* vsc = static_cast<const char*>(p.v_scale);
+      uint32_t last_k[kKRing], last_v[kVRing];
+#pragma unroll
+      for (int i = 0; i < kKRing; ++i) last_k[i] = 0;
+#pragma unroll
+      for (int i = 0; i < kVRing; ++i) last_v[i] = 0;
+      for (uint32_t seq = 0;; ++seq) {
+        Piece it;
+        if (!next_piece(seq, it)) break;
+        const int n = it.n;
+        const int32_t* table = p.block_tables + static_cast<int64_t>(it.r) * p.table_stride0;
+        auto load = [&](bool is_v, int t) {
+          const int kb = (it.t0 + t) * kN;
+          const uint32_t g = g0 + t;
+          const int ring = is_v ? kVRing : kKRing;
+          const int slot = g % ring;
+          if (!plan.tma || kb + kN > it.P) {
+            // Gathered by warps 2-3, which wait for the slot's last TMA fill to be consumed.
+            (is_v ? v_used : k_used) &= ~(1u << slot);
+            return;
+          }
+          const uint32_t full = JT_BAR((is_v ? kBarVFull : kBarKFull) + slot);
+          if (g >= static_cast<uint32_t>(ring))
+            mbar_wait(JT_BAR((is_v ? kBarVEmpty : kBarKEmpty) + slot), ((g / ring) & 1) ^ 1, abort);
+          if (*abort) return;
+          const uint32_t dst = base + (is_v ? L::kV8 : L::kK) + slot * kTile8;
+          mbar_arrive_tx(full, is_v ? kTile8 : kTile8 + 2 * kN);
+          for (int i = 0; i < kN; i += plan.box) {
+            const int pos = kb + i, off = pos % p.block_size;
+            int page = __ldg(table + pos / p.block_size);
+            if (page < 0 || page >= p.num_blocks) {
+              atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
+              page = -1;
+            }
+            // Page -1 lies outside the map: the box is filled with zeros.
+            tma_load_4d(dst + i * kD, is_v ? &vmap : &kmap, 0, it.h, off, page, full);
+            if (!is_v) {
+              const int64_t pg = max(page, 0);
+              const uint32_t sdst = base + L::kScale + (g % kScaleRing) * 256 + i;
+              bulk_load(sdst, ksc + pg * p.ks_stride0 + it.h * p.ks_stride1 + off, plan.box, full);
+              bulk_load(sdst + kN, vsc + pg * p.vs_stride0 + it.h * p.vs_stride1 + off, plan.box, full);
+            }
+          }
+          mbar_arrive(full);
+          if (is_v) { last_v[slot] = g / ring + 1; v_used |= 1u << slot; }
+          else { last_k[slot] = g / ring + 1; k_used |= 1u << slot; }
+        };
+        if (lane == 0) {
+          load(false, 0);
+          if (n > 1) load(false, 1);
+          for (int t = 0; t < n; ++t) {
+            if (t == max(0, n - 3)) publish(seq + 1);
+            load(true, t);
+            if (t + 2 < n) load(false, t + 2);
+          }
+        }
+        __syncwarp();
+        g0 += n;
+      }
+      if (lane == 0) {
+        // The copies this lane started have landed before the CTA exits.
+#pragma unroll
+        for (int i = 0; i < kKRing; ++i)
+          if (k_used & (1u << i)) mbar_wait(JT_BAR(kBarKFull + i), (last_k[i] - 1) & 1, abort, false);
+#pragma unroll
+        for (int i = 0; i < kVRing; ++i)
+          if (v_used & (1u << i)) mbar_wait(JT_BAR(kBarVFull + i), (last_v[i] - 1) & 1, abort, false);
+        PieceMeta* m = carve(p.workspace).meta + 2 * blockIdx.x;
+        m[0].valid = meta_valid[0];
+        m[1].valid = meta_valid[1];
+      }
+    } else {
+      // ---------------------------------------------------------------- factors and gathers
+      const int gt = tid - 64;  // two keys per thread
+      uint32_t g0 = 0;
+      float* kf = reinterpret_cast<float*>(sbase + L::kKf);
+      uint2* vm = reinterpret_cast<uint2*>(sbase + L::kVm);
+      volatile int* flag = reinterpret_cast<volatile int*>(sbase + L::kFlag);
+      const int64_t pool_slots = p.num_blocks * static_cast<int64_t>(p.block_size);
+      const int chunks = p.head_dim / 16;
+      for (uint32_t seq = 0;; ++seq) {
+        Piece it;
+        if (!next_piece(seq, it)) break;
+        const int32_t* table = p.block_tables + static_cast<int64_t>(it.r) * p.table_stride0;
+        for (int t = 0; t < it.n; ++t) {
+          const uint32_t g = g0 + t;
+          const int kb = (it.t0 + t) * kN;
+          const bool by_tma = plan.tma && kb + kN <= it.P;
+          uint32_t kbyte[2], vbyte[2];
+          int64_t page[2], off[2];
+          if (by_tma) {
+            warp_wait(JT_BAR(kBarKFull + g % kKRing), (g / kKRing) & 1, abort);
+            const unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256;
+            const uint32_t k2 = *reinterpret_cast<const uint16_t*>(sc + 2 * gt);
+            const uint32_t v2 = *reinterpret_cast<const uint16_t*>(sc + kN + 2 * gt);
+            kbyte[0] = k2 & 0xff; kbyte[1] = k2 >> 8;
+            vbyte[0] = v2 & 0xff; vbyte[1] = v2 >> 8;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int pos = kb + 2 * gt + i;
+              int64_t slot = -1;
+              page[i] = -1;
+              off[i] = 0;
+              if (pos < it.key_end) {
+                if (pos < it.P) {
+                  const int col = pos / p.block_size;
+                  slot = static_cast<int64_t>(__ldg(table + col)) * p.block_size + pos % p.block_size;
+                } else {
+                  slot = __ldg(p.tree_slots + it.q_start + (pos - it.P));
+                }
+                if (slot >= 0 && slot < pool_slots) {
+                  page[i] = slot / p.block_size;
+                  off[i] = slot - page[i] * p.block_size;
+                } else {
+                  atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
+                }
+              }
+              kbyte[i] = vbyte[i] = 127;
+              if (page[i] >= 0) {
+                kbyte[i] = __ldg(static_cast<const uint8_t*>(p.k_scale) + page[i] * p.ks_stride0 +
+                                 it.h * p.ks_stride1 + off[i]);
+                vbyte[i] = __ldg(static_cast<const uint8_t*>(p.v_scale) + page[i] * p.vs_stride0 +
+                                 it.h * p.vs_stride1 + off[i]);
+              }
+            }
+            if (g >= kKRing)
+              warp_wait(JT_BAR(kBarKEmpty + g % kKRing), ((g / kKRing) & 1) ^ 1, abort);
+            const uint32_t dst = base + L::kK + (g % kKRing) * kTile8;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int row = 2 * gt + i;
+              const char* src = static_cast<const char*>(p.k_pool);
+              if (page[i] >= 0) src += page[i] * p.k_stride0 + off[i] * p.k_stride1 + it.h * p.k_stride2;
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                const bool live = page[i] >= 0 && c < chunks;
+                jt::cp_async_16(dst + row * 128 + ((c ^ (row & 7)) << 4), live ? src + 16 * c : src,
+                                live ? 16 : 0);
+              }
+            }
+            asm volatile("cp.async.wait_all;\n" ::: "memory");
+            fence_proxy_async();
+            warp_arrive(JT_BAR(kBarKFull + g % kKRing));
+          }
+          // The factor buffers of tile g - 2 are free once its last PV has completed.
+          if (g >= 2) warp_wait(JT_BAR(kBarBEmpty + (g & 1)), ((g >> 1) & 1) ^ 1, abort);
+          int seen = 0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int at = (g & 1) * kN + 2 * gt + i;
+            kf[at] = vbyte[i] == 255u ? scale_value(255u) : scale_value(kbyte[i]);
+            vm[at] = v_multipliers(vbyte[i]);
+            if (kbyte[i] == 255u || vbyte[i] == 255u) seen |= 1;  // a NaN row
+            if (vbyte[i] > 134u) seen |= 2;                        // a second V multiplier
+          }
+          seen = __reduce_or_sync(0xffffffffu, seen);
+          if (lane == 0) flag[(g & 1) * 2 + (warp - 2)] = seen;
+          warp_arrive(JT_BAR(kBarFac + (g & 1)));
+          if (!by_tma) {
+            if (g >= kVRing)
+              warp_wait(JT_BAR(kBarVEmpty + g % kVRing), ((g / kVRing) & 1) ^ 1, abort);
+            const uint32_t dst = base + L::kV8 + (g % kVRing) * kTile8;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int row = 2 * gt + i;
+              const char* src = static_cast<const char*>(p.v_pool);
+              if (page[i] >= 0) src += page[i] * p.v_stride0 + off[i] * p.v_stride1 + it.h * p.v_stride2;
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                const bool live = page[i] >= 0 && c < chunks;
+                jt::cp_async_16(dst + row * 128 + ((c ^ (row & 7)) << 4), live ? src + 16 * c : src,
+                                live ? 16 : 0);
+              }
+            }
+            asm volatile("cp.async.wait_all;\n" ::: "memory");
+            warp_arrive(JT_BAR(kBarVFull + g % kVRing));
+          }
+        }
+        g0 += it.n;
+      }
     }
-    float mx = s;
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
-    __syncthreads();
-    const float top = fmaxf(fmaxf(red[0], red[1]), fmaxf(fmaxf(red[2], red[3]), m));
-    const float ref = top == -INFINITY ? 0.f : top;
-    const float w = slot >= 0 ? expf(s - ref) : 0.f;
-    const float keep = m == -INFINITY ? 0.f : expf(m - ref);
+  } else if (warp < 8) {
+    // ------------------------------------------------------------------ converters
+    regs_dec<kRegsConvert>();
+    const int ct = tid - 128;  // query row; V chunk index
+    uint32_t g0 = 0;
+    float* qfac = reinterpret_cast<float*>(sbase + L::kQfac);
+    const uint2* vm = reinterpret_cast<const uint2*>(sbase + L::kVm);
+    const volatile int* flag = reinterpret_cast<const volatile int*>(sbase + L::kFlag);
+    // V: eight lanes of a warp take four 16-byte chunks of rows r and r ^ 5, so that both the
+    // swizzled loads and the swizzled stores of the eight touch different banks.
+    const int quad = lane >> 3, sub = lane & 7;
+    for (uint32_t seq = 0;; ++seq) {
+      Piece it;
+      if (!next_piece(seq, it)) break;
+      if (seq > 0) warp_wait(JT_BAR(kBarQEmpty), (seq - 1) & 1, abort);
+      for (int tile = 0; tile < (it.two ? 2 : 1); ++tile) {
+        // One row per thread: its largest magnitude, then e4m3 terms of row / 2^e.
+        const int local = ct / ge.groups;
+        const int j = it.mb * ge.npi + tile * ge.npt + local;
+        const bool ok = local < ge.npt && j < it.T;
+        const uint4* src = nullptr;
+        if (ok)
+          src = reinterpret_cast<const uint4*>(
+              static_cast<const uint16_t*>(p.q) + (static_cast<int64_t>(it.q_start) + j) * p.q_stride0 +
+              (static_cast<int64_t>(it.h) * ge.groups + (ct - local * ge.groups)) * p.q_stride1);
+        const bool is_bf16 = p.dtype == JT_BF16;
+        auto unpack2 = [&](uint32_t w) {
+          return is_bf16 ? jt::MmaOp<__nv_bfloat16>::unpack(w) : jt::MmaOp<__half>::unpack(w);
+        };
+        const int words = p.head_dim / 8;
+        uint32_t top = 0;
+        if (ok) {
+#pragma unroll 4
+          for (int i = 0; i < words; ++i) {
+            const uint4 w = __ldg(src + i);
+            const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = unpack2(a[k]);
+              top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+            }
+          }
+        }
+        const bool finite = top < 0x7f800000u;
+        int e = 0;
+        if (top != 0 && finite)
+          e = max(static_cast<int>(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u), -126);
+        const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        const uint32_t dst = base + L::kQ + tile * kTerms * kTile8 + ct * 128;
+#pragma unroll 1
+        for (int c = 0; c < 8; ++c) {
+          uint32_t term[kTerms][4];
+#pragma unroll
+          for (int k = 0; k < kTerms; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) term[k][i] = 0u;
+          if (ok && finite && 2 * c < words) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint4 w = __ldg(src + 2 * c + half);
+              const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                float2 x = unpack2(a[k]);
+                x.x *= inv;
+                x.y *= inv;
+#pragma unroll
+                for (int m = 0; m < kTerms; ++m) {
+                  const uint32_t pair = pack_e4m3(x.x, x.y);
+                  term[m][2 * half + (k >> 1)] |= pair << (16 * (k & 1));
+                  const float2 y = unpack_e4m3(pair);
+                  x.x -= y.x;
+                  x.y -= y.y;
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int m = 0; m < kTerms; ++m)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(
+                             dst + m * kTile8 + ((c ^ (ct & 7)) << 4)),
+                         "r"(term[m][0]), "r"(term[m][1]), "r"(term[m][2]), "r"(term[m][3])
+                         : "memory");
+        }
+        qfac[((seq & 1) * 2 + tile) * kM + ct] =
+            finite ? p.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23)
+                   : __uint_as_float(0x7fc00000u);
+      }
+      fence_proxy_async();
+      warp_arrive(JT_BAR(kBarQFull + (seq & 1)));
+      for (int t = 0; t < it.n; ++t) {
+        const uint32_t g = g0 + t;
+        // The factors of tile g are written after the last PV of tile g - 2, whose bf16 tile
+        // is therefore free too.
+        warp_wait(JT_BAR(kBarFac + (g & 1)), (g >> 1) & 1, abort);
+        warp_wait(JT_BAR(kBarVFull + g % kVRing), (g / kVRing) & 1, abort);
+        const bool big = ((flag[(g & 1) * 2] | flag[(g & 1) * 2 + 1]) & 2) != 0;
+        const uint32_t src = base + L::kV8 + (g % kVRing) * kTile8;
+        const uint32_t dst = base + L::kV16 + (g & 1) * kTile16;
+        // 1024 chunks: each of the warp's 8 rounds covers 4 row pairs x 4 chunks.  Row pairs
+        // (r, r ^ 5) over r in {0, 1, 2, 3} (+ 8 per group of rows).
+#pragma unroll 2
+        for (int i = 0; i < 8; ++i) {
+          const int unit = (warp - 4) * 32 + i * 4 + quad;  // [0, 128): row group, pair, half
+          const int half = unit & 1, pair = (unit >> 1) & 3, rows8 = unit >> 3;
+          const int row = rows8 * 8 + ((sub & 4) ? (pair ^ 5) : pair);
+          const int c = half * 4 + (sub & 3);
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(src + row * 128 + ((c ^ (row & 7)) << 4)));
+          const uint2 m = vm[(g & 1) * kN + row];
+          uint32_t o[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            widen(w[k], o[2 * k], o[2 * k + 1]);
+            o[2 * k] = mul_bf16x2(o[2 * k], m.x);
+            o[2 * k + 1] = mul_bf16x2(o[2 * k + 1], m.x);
+          }
+          if (big) {
+            // Saturating: an infinity would reach rows that do not see this key.
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = clamp_bf16x2(mul_bf16x2(o[k], m.y));
+          }
+          const uint32_t row_dst = dst + (c >> 2) * kHalf16 + row * 128;
+          const int c0 = (2 * c) & 7;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(
+                           row_dst + ((c0 ^ (row & 7)) << 4)),
+                       "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
+                       : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(
+                           row_dst + (((c0 + 1) ^ (row & 7)) << 4)),
+                       "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
+                       : "memory");
+        }
+        fence_proxy_async();
+        warp_arrive(JT_BAR(kBarBFull + (g & 1)));
+        if (lane == 0) mbar_arrive(JT_BAR(kBarVEmpty + g % kVRing));
+      }
+      g0 += it.n;
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax + epilogue
+    regs_inc<kRegsSoftmax>();
+    const int s = (warp - 8) >> 2;           // stream
+    const int row = tid - 256 - s * 128;     // query-tile row, TMEM lane
+    const uint32_t lanes = static_cast<uint32_t>((row >> 5) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + col_s(s);
+    const float* kf = reinterpret_cast<const float*>(sbase + L::kKf);
+    const float* qfac = reinterpret_cast<const float*>(sbase + L::kQfac);
+    const volatile int* flag = reinterpret_cast<const volatile int*>(sbase + L::kFlag);
+    float2* xch = reinterpret_cast<float2*>(sbase + L::kX);
+    const int local = row / ge.groups, head_in = row - local * ge.groups;
+    uint32_t g0 = 0, step = 0, x_phase = 0;
+    for (uint32_t seq = 0;; ++seq) {
+      Piece it;
+      if (!next_piece(seq, it)) break;
+      const int n = it.n;
+      const int j = it.mb * ge.npi + (it.two ? s * ge.npt : 0) + local;
+      const bool ok = local < ge.npt && j < it.T;
+      const bool live = __any_sync(0xffffffffu, ok);
+      const float* bias = p.qq_bias + __ldg(p.qq_bias_offsets + it.r);
+      const int t_first = it.two ? 0 : s, t_step = it.two ? 1 : 2;
+      // Words of the next tile that needs a mask, built ahead of it.
+      uint32_t mw[4] = {0u, 0u, 0u, 0u};
+      // First masked tile of this stream: tiles below floor(P / 128) need none.
+      int t_mask = max(0, it.P / kN - it.t0);
+      if (!it.two && ((t_mask ^ s) & 1)) ++t_mask;
+      if (live && t_mask < n)
+        mask_words(bias, (it.t0 + t_mask) * kN, it.P, it.T, it.key_end, j, ok, mw);
+      float m_run = -INFINITY, l_run = 0.f, c_row = 0.f;
+      for (int t = t_first; t < n; t += t_step) {
+        const uint32_t g = g0 + t;
+        if (t == t_first) {
+          warp_wait(JT_BAR(kBarQFull + (seq & 1)), (seq >> 1) & 1, abort);
+          c_row = qfac[((seq & 1) * 2 + (it.two ? s : 0)) * kM + row];
+        }
+        warp_wait(JT_BAR(kBarFac + (g & 1)), (g >> 1) & 1, abort);
+        warp_wait(JT_BAR(kBarSFull + s), step & 1, abort);
+        ++step;
+        tc_fence_after();
+        if (live) {
+          const bool masked = t >= t_mask;
+          const bool nan_row = ((flag[(g & 1) * 2] | flag[(g & 1) * 2 + 1]) & 1) != 0;
+          float alpha;
+          if (!masked && nan_row) mw[0] = mw[1] = mw[2] = mw[3] = 0xffffffffu;
+          if (masked || nan_row)
+            softmax_row<kWide, true>(s_addr, kf + (g & 1) * kN, c_row, mw, m_run, l_run, alpha);
+          else
+            softmax_row<kWide, false>(s_addr, kf + (g & 1) * kN, c_row, mw, m_run, l_run, alpha);
+          // The scores of this tile were issued behind the previous PV of the stream, so that
+          // PV has completed: O can be rescaled at once.
+          if (t != t_first && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tmem + lanes + col_o(s) + 32 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+              tmem_st32(tmem + lanes + col_o(s) + 32 * c, o);
+            }
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          warp_arrive(JT_BAR(kBarPFull + s));
+          // The masks of the next masked tile, behind this tile's product.
+          const int t_next = masked ? t + t_step : t_mask;
+          if ((masked || nan_row) && t_next < n)
+            mask_words(bias, (it.t0 + t_next) * kN, it.P, it.T, it.key_end, j, ok, mw);
+        } else {
+          // No live row in this warp: its rows of P are never read out.
+          tc_fence_before();
+          warp_arrive(JT_BAR(kBarPFull + s));
+        }
+      }
+      // Epilogue, once the piece's last PV has completed.
+      warp_wait(JT_BAR(kBarODone), seq & 1, abort);
+      tc_fence_after();
+      const Workspace w = carve(p.workspace);
+      const int64_t out_row =
+          (static_cast<int64_t>(it.q_start) + j) * p.out_stride0 +
+          (static_cast<int64_t>(it.h) * ge.groups + head_in) * p.out_stride1;
+      if (it.two) {
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        if (live) {
+          if (it.slot >= 0 && ok)
+            w.ml[(it.slot * 2ll + s) * kM + row] = make_float2(m_run, l_run);
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            __syncwarp();
+            tmem_ld32(tmem + lanes + col_o(s) + 32 * c, o);
+            tmem_wait_ld();
+            if (!ok) continue;
+            if (it.slot >= 0) {
+              float4* dst = w.o + ((it.slot * 2ll + s) * 32 + 8 * c) * kM + row;
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                dst[k * kM] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                          __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+            } else if (32 * c < p.head_dim) {
+              float f[32];
+#pragma unroll
+              for (int k = 0; k < 32; ++k) f[k] = l_run == 0.f ? 0.f : __uint_as_float(o[k]) * inv;
+              store_columns(p, out_row + 32 * c, f, p.head_dim - 32 * c);
+            }
+          }
+        }
+      } else {
+        // The streams' rows meet: each warpgroup merges and writes 64 of the columns.
+        xch[s * kM + row] = make_float2(m_run, l_run);
+        warp_arrive(JT_BAR(kBarX));
+        warp_wait(JT_BAR(kBarX), x_phase, abort);
+        x_phase ^= 1u;
+        if (live) {
+          const float2 a = xch[row], b = n > 1 ? xch[kM + row] : make_float2(-INFINITY, 0.f);
+          const float m = fmaxf(a.x, b.x);
+          const float fa = a.x == -INFINITY ? 0.f : jt::fast_exp2(a.x - m);
+          const float fb = b.x == -INFINITY ? 0.f : jt::fast_exp2(b.x - m);
+          const float l = a.y * (a.x == -INFINITY ? 1.f : fa) + (n > 1 ? b.y * (b.x == -INFINITY ? 1.f : fb) : 0.f);
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          if (it.slot >= 0 && ok && s == 0) w.ml[it.slot * 2ll * kM + row] = make_float2(m, l);
+#pragma unroll 1
+          for (int c = 2 * s; c < 2 * s + 2; ++c) {
+            uint32_t o0[32], o1[32];
+            __syncwarp();
+            tmem_ld32(tmem + lanes + col_o(0) + 32 * c, o0);
+            if (n > 1) {
+              tmem_ld32(tmem + lanes + col_o(1) + 32 * c, o1);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o1[k] = 0u;
+            }
+            tmem_wait_ld();
+            if (!ok) continue;
+            float f[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              f[k] = __uint_as_float(o0[k]) * fa + __uint_as_float(o1[k]) * fb;
+            if (it.slot >= 0) {
+              float4* dst = w.o + (it.slot * 2ll * 32 + 8 * c) * kM + row;
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                dst[k * kM] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+            } else if (32 * c < p.head_dim) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) f[k] = l == 0.f ? 0.f : f[k] * inv;
+              store_columns(p, out_row + 32 * c, f, p.head_dim - 32 * c);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      tc_fence_before();
+      warp_arrive(JT_BAR(kBarOFree));
+      g0 += n;
+    }
+  }
+#undef JT_BAR
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+}
+
+// Merge of items cut between CTAs: block (c, q) takes 16 columns of the item that begins in
+// CTA c's part and ends in a later one, a row per thread.  Its pieces are slot 2c + 1, then
+// slots 2(c + 1), 2(c + 2), ... up to the one that finishes it.
+template <bool kWide>
+__global__ void __launch_bounds__(kM) tree_attn_fp8_merge_kernel(
+    const __grid_constant__ JtTreeAttnFp8Params p, const int parts) {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const Workspace w = carve(p.workspace);
+  const int c = blockIdx.x, tile = blockIdx.y >> 3, cg0 = (blockIdx.y & 7) * 4, row = threadIdx.x;
+  const PieceMeta first = w.meta[2 * c + 1];
+  if (!first.valid || first.finishes || 4 * cg0 >= p.head_dim) return;
+  const int npt = kM / p.groups, npi = npt * Smem<kWide>::kTiles;
+  const int T = p.node_counts[first.r];
+  const int local = row / p.groups;
+  const int j = first.mb * npi + tile * npt + local;
+  if (local >= npt || j >= T) return;
+  float acc[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) acc[k] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  for (int i = c; i < parts; ++i) {
+    const int slot = i == c ? 2 * c + 1 : 2 * i;
+    if (i != c && !w.meta[slot].valid) continue;  // a part shorter than the least cut
+    const float2 ml = w.ml[(slot * 2ll + tile) * kM + row];
+    float4 o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = w.o[((slot * 2ll + tile) * 32 + cg0 + k) * kM + row];
+    const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top;
+    const float fa = m == -INFINITY ? 0.f : jt::fast_exp2(m - ref);
+    const float fb = ml.x == -INFINITY ? 0.f : jt::fast_exp2(ml.x - ref);
+    // A row whose keys were all NaN has no maximum but a NaN sum, which has to stay.
+    l = l * (m == -INFINITY ? 1.f : fa) + ml.y * (ml.x == -INFINITY ? 1.f : fb);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      acc[4 * k] = acc[4 * k] * fa + o[k].x * fb;
+      acc[4 * k + 1] = acc[4 * k + 1] * fa + o[k].y * fb;
+      acc[4 * k + 2] = acc[4 * k + 2] * fa + o[k].z * fb;
+      acc[4 * k + 3] = acc[4 * k + 3] * fa + o[k].w * fb;
+    }
     m = top;
-    float sum = w;
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    __syncthreads();
-    if ((tid & 31) == 0) red[tid >> 5] = sum;
-    prob[tid] = w * vf;
-    __syncthreads();
-    l = l * keep + (red[0] + red[1] + red[2] + red[3]);
-    acc *= keep;
-    if (tid < D)
-      for (int i = 0; i < kThreads; ++i)
-        if (place[i] >= 0)
-          acc += prob[i] * code_value(static_cast<const uint8_t*>(p.v_pool)[place[i] + tid]);
-    __syncthreads();
+    if (i != c && w.meta[slot].finishes) break;
   }
-  if (tid < D) {
-    const float o = l == 0.f ? 0.f : acc / l;
-    const int64_t at = node * p.out_stride0 + hq * p.out_stride1 + tid;
-    if (p.out_dtype == JT_F32)
-      static_cast<float*>(p.out)[at] = o;
-    else
-      static_cast<T*>(p.out)[at] = T(o);
-  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int h = first.h * p.groups + (row - local * p.groups);
+  const int64_t at = (static_cast<int64_t>(p.cu_seqlens_q[first.r]) + j) * p.out_stride0 +
+                     h * p.out_stride1 + 4 * cg0;
+  float f[32];
+#pragma unroll
+  for (int k = 0; k < 32; ++k) f[k] = k < 16 && l != 0.f ? acc[k & 15] * inv : 0.f;
+  store_columns(p, at, f, 16);
+}
+
+bool al16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult query{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &query) ==
+            cudaSuccess &&
+        query == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    return static_cast<PFN_cuTensorMapEncodeTiled_v12000>(nullptr);
+  }();
+  return fn;
+}
+
+// [blocks, block_size, heads, head_dim] bytes; a box is `box` keys of one head, 128 bytes wide
+// (zeros past head_dim), in the MMA operands' 128-byte swizzle.
+bool encode_pool(CUtensorMap* map, const JtTreeAttnFp8Params& p, const void* pool, int64_t s0,
+                 int64_t s1, int64_t s2, int box) {
+  auto encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.head_dim),
+                              static_cast<cuuint64_t>(p.num_kv_heads),
+                              static_cast<cuuint64_t>(p.block_size),
+                              static_cast<cuuint64_t>(p.num_blocks)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(s2), static_cast<cuuint64_t>(s1),
+                                 static_cast<cuuint64_t>(s0)};
+  const cuuint32_t boxes[4] = {kD, 1, static_cast<cuuint32_t>(box), 1};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(pool), dims, strides,
+                boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool kWide>
+int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
+  LoadPlan plan{};
+  // TMA where a tile is whole boxes of whole pages: pages of whole tiles, or powers of two
+  // from 16 keys (a bulk copy of scale bytes is at least 16), with 16-byte scale rows.
+  const int bs = p.block_size;
+  plan.box = bs % kN == 0 ? kN : bs;
+  plan.tma = (bs % kN == 0 || (bs >= 16 && kN % bs == 0)) && al16(p.k_scale) && al16(p.v_scale) &&
+             (p.ks_stride0 | p.ks_stride1 | p.vs_stride0 | p.vs_stride1) % 16 == 0;
+  CUtensorMap kmap{}, vmap{};
+  if (plan.tma &&
+      (!encode_pool(&kmap, p, p.k_pool, p.k_stride0, p.k_stride1, p.k_stride2, plan.box) ||
+       !encode_pool(&vmap, p, p.v_pool, p.v_stride0, p.v_stride1, p.v_stride2, plan.box)))
+    plan.tma = 0;  // a layout the encoder refuses: gathered like any other page size
+  auto kernel = tree_attn_fp8_kernel<kWide>;
+  int rc = jt_cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                              Smem<kWide>::kBytes),
+                         "tree_attn_fp8 smem attribute");
+  if (rc != JT_OK) return rc;
+  const int grid = std::min(sms, kMaxCtas);
+  kernel<<<grid, kThreads, Smem<kWide>::kBytes, stream>>>(p, kmap, vmap, plan);
+  rc = jt_cuda_check(cudaGetLastError(), "tree_attn_fp8 launch");
+  if (rc != JT_OK) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid, 8 * Smem<kWide>::kTiles);
+  cfg.blockDim = dim3(kM);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return jt_cuda_check(cudaLaunchKernelEx(&cfg, tree_attn_fp8_merge_kernel<kWide>, p, grid),
+                       "tree_attn_fp8 merge launch");
 }
 
 }  // namespace
@@ -121,15 +1460,16 @@ extern "C" int64_t jt_tree_attn_fp8_workspace_size(int32_t num_requests, int32_t
                                                    int32_t head_dim) {
   if (num_requests < 1 || total_queries < 1 || num_kv_heads < 1 || groups < 1 || head_dim < 1)
     return -1;
-  return 0;
+  return kMetaBytes + kMlBytes + kPartBytes;
 }
 
 extern "C" int jt_tree_attn_fp8_launch(const JtTreeAttnFp8Params* p, cudaStream_t stream) {
   if (p == nullptr) return jt_fail(JT_ERR_INVALID, "tree_attn_fp8: null params");
   if (p->num_requests < 1 || p->total_queries < 1 || p->num_kv_heads < 1 || p->groups < 1 ||
-      p->groups > 128 || p->block_size < 1 || p->num_blocks < 1 || p->table_width < 1)
+      p->groups > kM || p->block_size < 1 || p->num_blocks < 1 || p->num_blocks > 0x7fffffff ||
+      p->table_width < 1)
     return jt_fail(JT_ERR_INVALID, "tree_attn_fp8: invalid geometry");
-  if (p->head_dim < 16 || p->head_dim > 128 || p->head_dim % 16 != 0)
+  if (p->head_dim < 16 || p->head_dim > kD || p->head_dim % 16 != 0)
     return jt_fail(JT_ERR_UNSUPPORTED, "tree_attn_fp8: head_dim %d is not a multiple of 16 up to 128",
                    p->head_dim);
   if (p->dtype != JT_BF16 && p->dtype != JT_F16)
@@ -142,10 +1482,21 @@ extern "C" int jt_tree_attn_fp8_launch(const JtTreeAttnFp8Params* p, cudaStream_
       !p->cu_seqlens_q || !p->query_to_request || !p->query_local_row || !p->prefix_lens ||
       !p->node_counts || !p->block_tables || !p->tree_slots || !p->qq_bias || !p->qq_bias_offsets)
     return jt_fail(JT_ERR_INVALID, "tree_attn_fp8: null tensor pointer");
-  const dim3 grid(p->total_queries, p->num_kv_heads * p->groups);
-  if (p->dtype == JT_BF16)
-    tree_attn_fp8_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(*p);
-  else
-    tree_attn_fp8_kernel<__half><<<grid, kThreads, 0, stream>>>(*p);
-  return jt_cuda_check(cudaGetLastError(), "tree_attn_fp8 launch");
+  if (!al16(p->q) || !al16(p->out) || !al16(p->k_pool) || !al16(p->v_pool) ||
+      (p->q_stride0 | p->q_stride1 | p->out_stride0 | p->out_stride1) % 8 != 0 ||
+      (p->k_stride0 | p->k_stride1 | p->k_stride2 | p->v_stride0 | p->v_stride1 | p->v_stride2) % 16 != 0)
+    return jt_fail(JT_ERR_INVALID,
+                   "tree_attn_fp8: queries, output and pool rows must start on 16 bytes");
+  const int64_t need = kMetaBytes + kMlBytes + kPartBytes;
+  if (p->workspace == nullptr || p->workspace_bytes < need ||
+      (reinterpret_cast<uintptr_t>(p->workspace) & 255u) != 0)
+    return jt_fail(JT_ERR_WORKSPACE, "tree_attn_fp8: workspace of %lld bytes required (got %lld)",
+                   static_cast<long long>(need), static_cast<long long>(p->workspace_bytes));
+  int dev = 0, sms = 0;
+  int rc = jt_cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc != JT_OK) return rc;
+  rc = jt_cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "SM count");
+  if (rc != JT_OK) return rc;
+  return p->dtype == JT_BF16 && p->out_dtype == JT_BF16 ? launch<false>(*p, sms, stream)
+                                                        : launch<true>(*p, sms, stream);
 }
