@@ -151,7 +151,7 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
+__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
                                             bool abortable) {
   const long long start = clock64();
   for (;;) {
@@ -252,6 +252,15 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
       "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15}, [%16];\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
@@ -283,19 +292,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
-template <int kRegs>
-__device__ __forceinline__ void regs_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegs));
-}
-template <int kRegs>
-__device__ __forceinline__ void regs_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegs));
-}
-// Registers per thread of the four warpgroups: 88 + 72 + 2 x 176 = 512 = 4 x the 128 of the
-// launch, so every increase is covered by the decreases.
-constexpr int kRegsLoad = 88, kRegsConvert = 72, kRegsSoftmax = 176;
-static_assert(kRegsLoad + kRegsConvert + 2 * kRegsSoftmax <= 4 * (65536 / kThreads), "registers");
-
 // ---- numbers --------------------------------------------------------------------------
 // 2^(byte - 127); byte 255 is NaN, byte 0 the subnormal 2^-127.
 __device__ __forceinline__ float scale_value(uint32_t b) {
@@ -374,16 +370,14 @@ __device__ __forceinline__ ItemInfo item_info(const Geometry& ge, int P, int T, 
   const int first = mb * ge.npi, last = min(T, first + ge.npi);
   ItemInfo it;
   it.key_end = P + last;
-  it.n = (it.key_end + kN - 1) / kN;
+  it.n = (it.key_end + kN - 1) >> 7;
   it.weight = last - first > ge.npt ? 2 : 1;
   it.cost = it.n * it.weight + kItemCost;
   return it;
 }
 // A request as the kernel takes it: no nodes when it has none or is refused.
-__device__ __forceinline__ void load_request(const JtTreeAttnFp8Params& p, int r, int& P, int& T,
-                                             bool flag) {
-  P = __ldg(p.prefix_lens + r);
-  T = __ldg(p.node_counts + r);
+__device__ __noinline__ int2 load_request(const JtTreeAttnFp8Params& p, int r, bool flag) {
+  int P = __ldg(p.prefix_lens + r), T = __ldg(p.node_counts + r);
   const int64_t capacity = static_cast<int64_t>(p.table_width) * p.block_size;
   if (T > kMaxNodes) {
     if (flag) atomicOr(&g_attn_fp8_errors, JT_DEVERR_TREE_TOO_LARGE);
@@ -393,10 +387,11 @@ __device__ __forceinline__ void load_request(const JtTreeAttnFp8Params& p, int r
     if (flag) atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
     P = P < 0 ? 0 : static_cast<int>(capacity);
   }
-  T = max(T, 0);
+  return make_int2(P, max(T, 0));
 }
-__device__ __forceinline__ int64_t head_cost(const Geometry& ge, int P, int T) {
+__device__ __noinline__ int64_t head_cost(const Geometry ge, int P, int T) {
   int64_t c = 0;
+#pragma unroll 1
   for (int mb = 0; mb * ge.npi < T; ++mb) c += item_info(ge, P, T, mb).cost;
   return c;
 }
@@ -404,7 +399,7 @@ __device__ __forceinline__ int64_t head_cost(const Geometry& ge, int P, int T) {
 __device__ __forceinline__ int cut_tile(const ItemInfo& it, int64_t start, int64_t x) {
   if (x <= start) return 0;
   if (x >= start + it.cost) return it.n;
-  const int t = static_cast<int>((x - start) / it.weight);
+  const int t = static_cast<int>(x - start) >> (it.weight - 1);
   if (t < kMinTiles) return 0;
   if (it.n - t < kMinTiles) return it.n;
   return t;
@@ -432,6 +427,38 @@ __host__ __device__ __forceinline__ Workspace carve(void* base) {
                    reinterpret_cast<float4*>(b + kMetaBytes + kMlBytes)};
 }
 
+// Page and offset of key position `pos` of a piece, page -1 past its keys or out of the pool.
+struct KeyPlace {
+  int64_t page;
+  int off;
+};
+__device__ __noinline__ KeyPlace locate_key(const JtTreeAttnFp8Params& p, const int32_t* table,
+                                            int pos, int P, int key_end, int q_start) {
+  KeyPlace k{-1, 0};
+  if (pos >= key_end) return k;
+  int64_t slot;
+  if (pos < P) {
+    const int col = pos / p.block_size;
+    slot = static_cast<int64_t>(__ldg(table + col)) * p.block_size + (pos - col * p.block_size);
+  } else {
+    slot = __ldg(p.tree_slots + q_start + (pos - P));
+  }
+  if (slot >= 0 && slot < p.num_blocks * static_cast<int64_t>(p.block_size)) {
+    k.page = slot / p.block_size;
+    k.off = static_cast<int>(slot - k.page * p.block_size);
+  } else {
+    atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
+  }
+  return k;
+}
+// One row's 16-byte chunks into a swizzled code tile (zeros past `chunks` or without a page).
+__device__ __noinline__ void gather_row(uint32_t dst, int row, const char* src, int chunks) {
+#pragma unroll 1
+  for (int c = 0; c < 8; ++c)
+    jt::cp_async_16(dst + row * 128 + ((c ^ (row & 7)) << 4), c < chunks ? src + 16 * c : src,
+                    c < chunks ? 16 : 0);
+}
+
 // How tiles reach shared memory, decided on the host from the layout.
 struct LoadPlan {
   int tma;   // prefix tiles by TMA boxes of `box` keys, their scale bytes by bulk copies
@@ -441,12 +468,13 @@ struct LoadPlan {
 // Visibility words of the 128 keys at kb for this lane's row: bit b of word w is key
 // kb + 32 w + b.  Each warp builds its rows' words node by node: lane b reads the bias of its
 // key, a ballot collects the word, and the lanes of that node keep it.
-__device__ __forceinline__ void mask_words(const float* bias, int kb, int P, int T, int key_end,
-                                           int j, bool ok, uint32_t (&mw)[4]) {
+__device__ __noinline__ uint4 mask_words(const float* bias, int kb, int P, int T, int key_end,
+                                         int j, bool ok) {
   const int lane = threadIdx.x & 31;
-  mw[0] = mw[1] = mw[2] = mw[3] = 0u;
+  uint32_t mw[4] = {0u, 0u, 0u, 0u};
   const int lo = __reduce_min_sync(0xffffffffu, ok ? j : 0x7fffffff);
   const int hi = __reduce_max_sync(0xffffffffu, ok ? j : -1);
+#pragma unroll 1
   for (int base = lo; base <= hi; base += 4) {
     float b[4][4];
 #pragma unroll
@@ -470,51 +498,74 @@ __device__ __forceinline__ void mask_words(const float* bias, int kb, int P, int
         if (ok && j == base + i) mw[w] = bits;
       }
   }
+  return make_uint4(mw[0], mw[1], mw[2], mw[3]);
 }
 
-// Softmax of one row of a 128-key tile: scores from TMEM, scaled by the keys' factors, the
-// lazy running maximum (moved only when a tile exceeds it by 2^8, so P stays below 2^8 and O
-// is rarely rescaled), P to the S columns it came from.  kCareful (masked tiles, tiles with a
-// NaN row): masked scores are -inf and every exponential is exp2, which keeps a NaN.
-template <bool kWide, bool kCareful>
-__device__ __forceinline__ void softmax_row(uint32_t s_addr, const float* kf, float c_row,
-                                            const uint32_t (&mw)[4], float& m_run, float& l_run,
-                                            float& alpha) {
-  uint32_t v[4][32];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + 32 * q, v[q]);
+// Columns of P inside an S buffer: keys 16 kk .. 16 kk + 15 (8 columns of bf16 pairs).  Each
+// half tile's P lies in the columns of the scores it came from, the low parts 32 columns on.
+__device__ __forceinline__ constexpr uint32_t col_p(int kk) {
+  return kk < 4 ? 8u * kk : 64u + 8u * (kk - 4);
+}
+
+// 64 scores of a row from TMEM, times the keys' factors (and -inf where masked).
+template <bool kCareful>
+__device__ __forceinline__ void load_scores(uint32_t s_addr, const float* kf, uint32_t m0,
+                                            uint32_t m1, uint32_t (&v)[64]) {
+  tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(v));
+  tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
   tmem_wait_ld();
-  float mx4[4];
+  const float4* f4 = reinterpret_cast<const float4*>(kf);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const float4* f4 = reinterpret_cast<const float4*>(kf + 32 * q);
+  for (int k = 0; k < 16; ++k) {
+    const float4 f = f4[k];
+    const float2 a = __fmul2_rn(make_float2(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1])),
+                                make_float2(f.x, f.y));
+    const float2 b = __fmul2_rn(make_float2(__uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3])),
+                                make_float2(f.z, f.w));
+    v[4 * k] = __float_as_uint(a.x);
+    v[4 * k + 1] = __float_as_uint(a.y);
+    v[4 * k + 2] = __float_as_uint(b.x);
+    v[4 * k + 3] = __float_as_uint(b.y);
+  }
+  if constexpr (kCareful) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float4 f = f4[k];
-      const float2 a = __fmul2_rn(make_float2(__uint_as_float(v[q][4 * k]), __uint_as_float(v[q][4 * k + 1])),
-                                  make_float2(f.x, f.y));
-      const float2 b = __fmul2_rn(make_float2(__uint_as_float(v[q][4 * k + 2]), __uint_as_float(v[q][4 * k + 3])),
-                                  make_float2(f.z, f.w));
-      v[q][4 * k] = __float_as_uint(a.x);
-      v[q][4 * k + 1] = __float_as_uint(a.y);
-      v[q][4 * k + 2] = __float_as_uint(b.x);
-      v[q][4 * k + 3] = __float_as_uint(b.y);
+    for (int k = 0; k < 32; ++k) {
+      if (!((m0 >> k) & 1u)) v[k] = 0xff800000u;
+      if (!((m1 >> k) & 1u)) v[32 + k] = 0xff800000u;
     }
-    if constexpr (kCareful) {
-#pragma unroll
-      for (int k = 0; k < 32; ++k)
-        if (!((mw[q] >> k) & 1u)) v[q][k] = 0xff800000u;
-    }
+  }
+}
+
+// Softmax of one row of a 128-key tile, in two passes over half tiles (the scores are read
+// from TMEM twice rather than held: 128 live scores would leave too few registers for the
+// 16 warps, and the loops keep the code small enough for the instruction cache).  The running
+// maximum is lazy: it moves only when a tile exceeds it by 2^8, so P stays below 2^8 and O
+// is rarely rescaled.  kCareful (masked tiles, tiles with a NaN row): masked scores are -inf
+// and every exponential is exp2, which keeps a NaN.
+struct RowState {
+  float m, l, alpha;  // running maximum (log2 units) and sum; the factor older sums and O take
+};
+template <bool kWide, bool kCareful>
+__device__ __forceinline__ RowState softmax_body(uint32_t s_addr, const float* kf, float c_row,
+                                                 uint4 mw, float m_run, float l_run) {
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    uint32_t v[64];
+    load_scores<kCareful>(s_addr + 64 * h, kf + 64 * h, h ? mw.z : mw.x, h ? mw.w : mw.y, v);
     float m8[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      m8[k] = fmaxf(fmaxf(__uint_as_float(v[q][k]), __uint_as_float(v[q][k + 8])),
-                    fmaxf(__uint_as_float(v[q][k + 16]), __uint_as_float(v[q][k + 24])));
-    mx4[q] = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
-                   fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+    for (int k = 0; k < 8; ++k) m8[k] = fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 8]));
+#pragma unroll
+    for (int q = 16; q < 64; q += 16)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        m8[k] = fmaxf(m8[k], fmaxf(__uint_as_float(v[q + k]), __uint_as_float(v[q + k + 8])));
+    mx = fmaxf(mx, fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
+                         fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))));
   }
-  const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * c_row;
-  alpha = 1.f;
+  mx *= c_row;
+  float alpha = 1.f;
   if (mx > m_run + 8.f) {
     if (m_run != -INFINITY) alpha = jt::fast_exp2(m_run - mx);
     m_run = mx;
@@ -522,50 +573,63 @@ __device__ __forceinline__ void softmax_row(uint32_t s_addr, const float* kf, fl
   const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
   const float2 c2 = make_float2(c_row, c_row), n2 = make_float2(neg_m, neg_m);
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    uint32_t v[64];
+    load_scores<kCareful>(s_addr + 64 * h, kf + 64 * h, h ? mw.z : mw.x, h ? mw.w : mw.y, v);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint32_t ph[16], pl[kWide ? 16 : 1];
+    for (int q = 0; q < 2; ++q) {
+      uint32_t ph[16], pl[kWide ? 16 : 1];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float2 x = __ffma2_rn(
-          make_float2(__uint_as_float(v[q][2 * k]), __uint_as_float(v[q][2 * k + 1])), c2, n2);
-      float2 e;
-      if (!kCareful && !kWide && (k & 3) == 3)
-        e = exp2_poly2(x);
-      else
-        e = make_float2(jt::fast_exp2(x.x), jt::fast_exp2(x.y));
-      sum[k & 1] = __fadd2_rn(sum[k & 1], e);
-      ph[k] = pack_bf16(e.x, e.y);
-      if constexpr (kWide) {
-        const float2 h = jt::MmaOp<__nv_bfloat16>::unpack(ph[k]);
-        pl[k] = pack_bf16(e.x - h.x, e.y - h.y);
+      for (int k = 0; k < 16; ++k) {
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[32 * q + 2 * k]),
+                                                __uint_as_float(v[32 * q + 2 * k + 1])), c2, n2);
+        float2 e;
+        if (!kCareful && !kWide && (k & 3) == 3)
+          e = exp2_poly2(x);
+        else
+          e = make_float2(jt::fast_exp2(x.x), jt::fast_exp2(x.y));
+        sum[k & 1] = __fadd2_rn(sum[k & 1], e);
+        ph[k] = pack_bf16(e.x, e.y);
+        if constexpr (kWide) {
+          const float2 f = jt::MmaOp<__nv_bfloat16>::unpack(ph[k]);
+          pl[k] = pack_bf16(e.x - f.x, e.y - f.y);
+        }
       }
+      tmem_st16(s_addr + 64 * h + 16 * q, ph);
+      if constexpr (kWide) tmem_st16(s_addr + 64 * h + 32 + 16 * q, pl);
     }
-    tmem_st16(s_addr + 16 * q, ph);
-    if constexpr (kWide) tmem_st16(s_addr + 64 + 16 * q, pl);
   }
-  l_run = l_run * alpha + ((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y));
+  return RowState{m_run, l_run * alpha + ((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)), alpha};
 }
 
-// 32 output columns of one row.
+// Masked tiles (the last one or two of an item) run a copy of their own, out of line.
+template <bool kWide>
+__device__ __noinline__ RowState softmax_masked(uint32_t s_addr, const float* kf, float c_row,
+                                                uint4 mw, float m_run, float l_run) {
+  return softmax_body<kWide, true>(s_addr, kf, c_row, mw, m_run, l_run);
+}
+
+// 16 output columns of one row.  The narrow kernel's output is bf16.
+template <bool kWide>
 __device__ __forceinline__ void store_columns(const JtTreeAttnFp8Params& p, int64_t at,
-                                              const float (&o)[32], int columns) {
-  if (p.out_dtype == JT_F32) {
+                                              const float (&o)[16]) {
+  if (kWide && p.out_dtype == JT_F32) {
     float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (4 * k < columns) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+    for (int k = 0; k < 4; ++k)
+      dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
     return;
   }
   uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (8 * k >= columns) continue;
+  for (int k = 0; k < 2; ++k) {
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      w[e] = p.out_dtype == JT_BF16 ? pack_bf16(o[8 * k + 2 * e], o[8 * k + 2 * e + 1])
-                                    : jt::MmaOp<__half>::pack(o[8 * k + 2 * e], o[8 * k + 2 * e + 1]);
+      w[e] = !kWide || p.out_dtype == JT_BF16
+                 ? pack_bf16(o[8 * k + 2 * e], o[8 * k + 2 * e + 1])
+                 : jt::MmaOp<__half>::pack(o[8 * k + 2 * e], o[8 * k + 2 * e + 1]);
     dst[k] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
@@ -608,9 +672,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int r_lo = min(tid * per, R), r_hi = min(r_lo + per, R);
   int64_t mine = 0;
   for (int r = r_lo; r < r_hi; ++r) {
-    int P, T;
-    load_request(p, r, P, T, blockIdx.x == 0);
-    mine += head_cost(ge, P, T) * p.num_kv_heads;
+    const int2 q = load_request(p, r, blockIdx.x == 0);
+    mine += head_cost(ge, q.x, q.y) * p.num_kv_heads;
   }
   int64_t incl = mine;
 #pragma unroll
@@ -634,9 +697,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (has_part && mine > 0 && my_start <= x0 && x0 < my_start + mine) {
     int64_t s = my_start;
     for (int r = r_lo; r < r_hi; ++r) {
-      int P, T;
-      load_request(p, r, P, T, false);
-      const int64_t c = head_cost(ge, P, T) * p.num_kv_heads;
+      const int2 q = load_request(p, r, false);
+      const int64_t c = head_cost(ge, q.x, q.y) * p.num_kv_heads;
       if (x0 < s + c) {
         scan[32] = r;
         scan[33] = s;
@@ -671,89 +733,61 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   if (warp < 4) {
-    regs_dec<kRegsLoad>();
     if (warp == 0) {
       // ---------------------------------------------------------------- MMA issuer
       // QK of a stream's next tile is issued right behind the PV that reads P out of the same
       // S buffer: MMAs of one thread execute in order.
       uint32_t g0 = 0, seq = 0;
-      uint32_t p_phase[2] = {0, 0};
+      uint32_t p_phase = 0;  // bit s: stream s
       const uint64_t q_desc = smem_desc(base + L::kQ, 16, 1024);
       const uint64_t k_desc = smem_desc(base + L::kK, 16, 1024);
       const uint64_t v_desc = smem_desc(base + L::kV16, kHalf16, 1024);
-      auto wait_k = [&](uint32_t g) {
-        mbar_wait(JT_BAR(kBarKFull + g % kKRing), (g / kKRing) & 1, abort);
-        tc_fence_after();
-      };
-      auto qk = [&](uint32_t g, int s, int tile) {
-        const uint64_t kd = k_desc + (g % kKRing) * (kTile8 >> 4);
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term)
-#pragma unroll
-          for (int kk = 0; kk < kD / 32; ++kk)
-            mma_f8_warp(tmem + col_s(s), q_desc + ((tile * kTerms + term) * kTile8 + kk * 32) / 16,
-                        kd + kk * 2, kIdescQK, (term | kk) != 0 ? 1u : 0u);
-        commit_warp(JT_BAR(kBarSFull + s));
-      };
-      auto pv = [&](uint32_t g, int s, bool acc) {
-        mbar_wait(JT_BAR(kBarPFull + s), p_phase[s], abort);
-        p_phase[s] ^= 1u;
-        tc_fence_after();
-        const uint64_t vd = v_desc + (g & 1) * (kTile16 >> 4);
-#pragma unroll
-        for (int kk = 0; kk < kN / 16; ++kk) {
-          mma_ts_warp(tmem + col_o(s), tmem + col_s(s) + 8 * kk, vd + kk * (2048 / 16), kIdescPV,
-                      acc || kk > 0 ? 1u : 0u);
-          if constexpr (kWide)
-            mma_ts_warp(tmem + col_o(s), tmem + col_s(s) + 64 + 8 * kk, vd + kk * (2048 / 16),
-                        kIdescPV, 1u);
-        }
-      };
       for (;; ++seq) {
         Piece it;
         if (!next_piece(seq, it)) break;
-        const int n = it.n;
+        const int n = it.n, two = it.two;
         mbar_wait(JT_BAR(kBarQFull + (seq & 1)), (seq >> 1) & 1, abort);
         tc_fence_after();
-        auto k_done = [&](uint32_t g, int t) {
-          commit_warp(JT_BAR(kBarKEmpty + g % kKRing));
-          if (t == n - 1) commit_warp(JT_BAR(kBarQEmpty));
-        };
-        if (it.two) {
-          wait_k(g0);
-          qk(g0, 0, 0);
-          qk(g0, 1, 1);
-          k_done(g0, 0);
-        } else {
-          for (int t = 0; t < min(2, n); ++t) {
-            wait_k(g0 + t);
-            qk(g0 + t, t, 0);
-            k_done(g0 + t, t);
-          }
-        }
-        for (int t = 0; t < n; ++t) {
-          const uint32_t g = g0 + t;
-          mbar_wait(JT_BAR(kBarBFull + (g & 1)), (g >> 1) & 1, abort);
-          if (t == 0 && seq > 0) mbar_wait(JT_BAR(kBarOFree), (seq - 1) & 1, abort);
-          if (it.two) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              pv(g, s, t > 0);
-              if (s == 1) commit_warp(JT_BAR(kBarBEmpty + (g & 1)));
-              if (t + 1 < n) {
-                if (s == 0) wait_k(g + 1);
-                qk(g + 1, s, s);
-                if (s == 1) k_done(g + 1, t + 1);
-              }
+        // Step u is stream u & 1's product with key tile u (one query tile) or u >> 1 (two).
+        const int steps = n << two;
+#pragma unroll 1
+        for (int u = -2; u < steps; ++u) {
+          const int s = u & 1;
+          const uint32_t d_s = tmem + col_s(s), d_o = tmem + col_o(s);
+          if (u >= 0) {
+            const uint32_t g = g0 + (u >> two);
+            if (!two || s == 0) mbar_wait(JT_BAR(kBarBFull + (g & 1)), (g >> 1) & 1, abort);
+            if (u == 0 && seq > 0) mbar_wait(JT_BAR(kBarOFree), (seq - 1) & 1, abort);
+            mbar_wait(JT_BAR(kBarPFull + s), (p_phase >> s) & 1, abort);
+            p_phase ^= 1u << s;
+            tc_fence_after();
+            const uint64_t vd = v_desc + (g & 1) * (kTile16 >> 4);
+#pragma unroll 1
+            for (int kk = 0; kk < kN / 16; ++kk) {
+              mma_ts_warp(d_o, d_s + col_p(kk), vd + kk * (2048 / 16), kIdescPV,
+                          u > 1 || kk > 0 ? 1u : 0u);
+              if constexpr (kWide)
+                mma_ts_warp(d_o, d_s + col_p(kk) + 32, vd + kk * (2048 / 16), kIdescPV, 1u);
             }
-          } else {
-            const int s = t & 1;
-            pv(g, s, t > 1);
-            commit_warp(JT_BAR(kBarBEmpty + (g & 1)));
-            if (t + 2 < n) {
-              wait_k(g + 2);
-              qk(g + 2, s, 0);
-              k_done(g + 2, t + 2);
+            if (!two || s == 1) commit_warp(JT_BAR(kBarBEmpty + (g & 1)));
+          }
+          if (u + 2 < steps) {
+            const int t = (u + 2) >> two;
+            const uint32_t g = g0 + t;
+            if (!two || s == 0) {
+              mbar_wait(JT_BAR(kBarKFull + g % kKRing), (g / kKRing) & 1, abort);
+              tc_fence_after();
+            }
+            const uint64_t qd = q_desc + (two & s) * (kTerms * kTile8 / 16);
+            const uint64_t kd = k_desc + (g % kKRing) * (kTile8 >> 4);
+#pragma unroll 1
+            for (int i = 0; i < kTerms * 4; ++i)  // (term, 32 dims)
+              mma_f8_warp(d_s, qd + (i >> 2) * (kTile8 / 16) + (i & 3) * 2, kd + (i & 3) * 2,
+                          kIdescQK, i != 0 ? 1u : 0u);
+            commit_warp(JT_BAR(kBarSFull + s));
+            if (!two || s == 1) {
+              commit_warp(JT_BAR(kBarKEmpty + g % kKRing));
+              if (t == n - 1) commit_warp(JT_BAR(kBarQEmpty));
             }
           }
         }
@@ -770,7 +804,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool more = has_part;
       int meta_valid[2] = {0, 0};
       if (lane == 0 && more) {
-        load_request(p, r, P, T, false);
+        const int2 q = load_request(p, r, false);
+        P = q.x;
+        T = q.y;
         const int64_t ch = head_cost(ge, P, T);
         h = static_cast<int>((x0 - s_item) / ch);
         s_item += ch * h;
@@ -819,7 +855,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 h = 0;
                 do {
                   ++r;
-                  if (r < R) load_request(p, r, P, T, false);
+                  if (r < R) {
+                    const int2 q = load_request(p, r, false);
+                    P = q.x;
+                    T = q.y;
+                  }
                 } while (r < R && T == 0);
                 if (r >= R) more = false;
               }
@@ -859,6 +899,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (*abort) return;
           const uint32_t dst = base + (is_v ? L::kV8 : L::kK) + slot * kTile8;
           mbar_arrive_tx(full, is_v ? kTile8 : kTile8 + 2 * kN);
+#pragma unroll 1
           for (int i = 0; i < kN; i += plan.box) {
             const int pos = kb + i, off = pos % p.block_size;
             int page = __ldg(table + pos / p.block_size);
@@ -880,12 +921,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           else { last_k[slot] = g / ring + 1; k_used |= 1u << slot; }
         };
         if (lane == 0) {
-          load(false, 0);
-          if (n > 1) load(false, 1);
-          for (int t = 0; t < n; ++t) {
-            if (t == max(0, n - 3)) publish(seq + 1);
-            load(true, t);
-            if (t + 2 < n) load(false, t + 2);
+          // K 0, K 1, then V t and K t + 2: the order in which they are used.
+#pragma unroll 1
+          for (int i = 0; i <= 2 * n; ++i) {
+            if (i == max(0, 2 * n - 6)) publish(seq + 1);
+            const bool is_v = i >= 2 && !(i & 1);
+            const int t = i < 2 ? i : is_v ? (i >> 1) - 1 : (i >> 1) + 1;
+            if (t < n) load(is_v, t);
           }
         }
         __syncwarp();
@@ -910,7 +952,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* kf = reinterpret_cast<float*>(sbase + L::kKf);
       uint2* vm = reinterpret_cast<uint2*>(sbase + L::kVm);
       volatile int* flag = reinterpret_cast<volatile int*>(sbase + L::kFlag);
-      const int64_t pool_slots = p.num_blocks * static_cast<int64_t>(p.block_size);
       const int chunks = p.head_dim / 16;
       for (uint32_t seq = 0;; ++seq) {
         Piece it;
@@ -932,24 +973,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const int pos = kb + 2 * gt + i;
-              int64_t slot = -1;
-              page[i] = -1;
-              off[i] = 0;
-              if (pos < it.key_end) {
-                if (pos < it.P) {
-                  const int col = pos / p.block_size;
-                  slot = static_cast<int64_t>(__ldg(table + col)) * p.block_size + pos % p.block_size;
-                } else {
-                  slot = __ldg(p.tree_slots + it.q_start + (pos - it.P));
-                }
-                if (slot >= 0 && slot < pool_slots) {
-                  page[i] = slot / p.block_size;
-                  off[i] = slot - page[i] * p.block_size;
-                } else {
-                  atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
-                }
-              }
+              const KeyPlace at = locate_key(p, table, kb + 2 * gt + i, it.P, it.key_end, it.q_start);
+              page[i] = at.page;
+              off[i] = at.off;
               kbyte[i] = vbyte[i] = 127;
               if (page[i] >= 0) {
                 kbyte[i] = __ldg(static_cast<const uint8_t*>(p.k_scale) + page[i] * p.ks_stride0 +
@@ -963,15 +989,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t dst = base + L::kK + (g % kKRing) * kTile8;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const int row = 2 * gt + i;
               const char* src = static_cast<const char*>(p.k_pool);
-              if (page[i] >= 0) src += page[i] * p.k_stride0 + off[i] * p.k_stride1 + it.h * p.k_stride2;
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                const bool live = page[i] >= 0 && c < chunks;
-                jt::cp_async_16(dst + row * 128 + ((c ^ (row & 7)) << 4), live ? src + 16 * c : src,
-                                live ? 16 : 0);
-              }
+              if (page[i] >= 0)
+                src += page[i] * p.k_stride0 + off[i] * p.k_stride1 + it.h * p.k_stride2;
+              gather_row(dst, 2 * gt + i, src, page[i] >= 0 ? chunks : 0);
             }
             asm volatile("cp.async.wait_all;\n" ::: "memory");
             fence_proxy_async();
@@ -997,15 +1018,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t dst = base + L::kV8 + (g % kVRing) * kTile8;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const int row = 2 * gt + i;
               const char* src = static_cast<const char*>(p.v_pool);
-              if (page[i] >= 0) src += page[i] * p.v_stride0 + off[i] * p.v_stride1 + it.h * p.v_stride2;
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                const bool live = page[i] >= 0 && c < chunks;
-                jt::cp_async_16(dst + row * 128 + ((c ^ (row & 7)) << 4), live ? src + 16 * c : src,
-                                live ? 16 : 0);
-              }
+              if (page[i] >= 0)
+                src += page[i] * p.v_stride0 + off[i] * p.v_stride1 + it.h * p.v_stride2;
+              gather_row(dst, 2 * gt + i, src, page[i] >= 0 ? chunks : 0);
             }
             asm volatile("cp.async.wait_all;\n" ::: "memory");
             warp_arrive(JT_BAR(kBarVFull + g % kVRing));
@@ -1016,7 +1032,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------------ converters
-    regs_dec<kRegsConvert>();
     const int ct = tid - 128;  // query row; V chunk index
     uint32_t g0 = 0;
     float* qfac = reinterpret_cast<float*>(sbase + L::kQfac);
@@ -1029,6 +1044,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Piece it;
       if (!next_piece(seq, it)) break;
       if (seq > 0) warp_wait(JT_BAR(kBarQEmpty), (seq - 1) & 1, abort);
+#pragma unroll 1
       for (int tile = 0; tile < (it.two ? 2 : 1); ++tile) {
         // One row per thread: its largest magnitude, then e4m3 terms of row / 2^e.
         const int local = ct / ge.groups;
@@ -1043,60 +1059,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto unpack2 = [&](uint32_t w) {
           return is_bf16 ? jt::MmaOp<__nv_bfloat16>::unpack(w) : jt::MmaOp<__half>::unpack(w);
         };
-        const int words = p.head_dim / 8;
+        const int words = ok ? p.head_dim / 8 : 0;  // 16-byte words of a row
         uint32_t top = 0;
-        if (ok) {
-#pragma unroll 4
-          for (int i = 0; i < words; ++i) {
-            const uint4 w = __ldg(src + i);
-            const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll 1
+        for (int i = 0; i < words; i += 4) {
+          uint4 w[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = unpack2(a[k]);
-              top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
-            }
+          for (int k = 0; k < 4; ++k)
+            w[k] = i + k < words ? __ldg(src + i + k) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // The operand's own bits order like the magnitude: the type is undone at the end.
+            const uint32_t a = w[k].x & 0x7fff7fffu, b = w[k].y & 0x7fff7fffu;
+            const uint32_t c = w[k].z & 0x7fff7fffu, d = w[k].w & 0x7fff7fffu;
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(a, b), __vmaxu2(c, d)));
           }
         }
+        top = max(top & 0xffffu, top >> 16);
+        top = __float_as_uint(unpack2(top).x);
         const bool finite = top < 0x7f800000u;
         int e = 0;
         if (top != 0 && finite)
           e = max(static_cast<int>(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u), -126);
+        // A row with a non-finite element enters as zeros; its factor makes its scores NaN.
         const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        const uint32_t dst = base + L::kQ + tile * kTerms * kTile8 + ct * 128;
+        unsigned char* dst = sbase + L::kQ + tile * kTerms * kTile8 + ct * 128;
 #pragma unroll 1
         for (int c = 0; c < 8; ++c) {
           uint32_t term[kTerms][4];
+          uint4 w[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+          if (2 * c < words && finite) {
+            w[0] = __ldg(src + 2 * c);
+            w[1] = __ldg(src + 2 * c + 1);
+          }
 #pragma unroll
-          for (int k = 0; k < kTerms; ++k)
+          for (int i = 0; i < 4; ++i) {
+            const uint4 u = w[i >> 1];
+            float2 x0 = unpack2(i & 1 ? u.z : u.x), x1 = unpack2(i & 1 ? u.w : u.y);
+            x0 = make_float2(x0.x * inv, x0.y * inv);
+            x1 = make_float2(x1.x * inv, x1.y * inv);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) term[k][i] = 0u;
-          if (ok && finite && 2 * c < words) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint4 w = __ldg(src + 2 * c + half);
-              const uint32_t a[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                float2 x = unpack2(a[k]);
-                x.x *= inv;
-                x.y *= inv;
-#pragma unroll
-                for (int m = 0; m < kTerms; ++m) {
-                  const uint32_t pair = pack_e4m3(x.x, x.y);
-                  term[m][2 * half + (k >> 1)] |= pair << (16 * (k & 1));
-                  const float2 y = unpack_e4m3(pair);
-                  x.x -= y.x;
-                  x.y -= y.y;
-                }
-              }
+            for (int m = 0; m < kTerms; ++m) {
+              const uint32_t a = pack_e4m3(x0.x, x0.y), b = pack_e4m3(x1.x, x1.y);
+              term[m][i] = a | (b << 16);
+              const float2 ya = unpack_e4m3(a), yb = unpack_e4m3(b);
+              x0 = make_float2(x0.x - ya.x, x0.y - ya.y);
+              x1 = make_float2(x1.x - yb.x, x1.y - yb.y);
             }
           }
 #pragma unroll
           for (int m = 0; m < kTerms; ++m)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(
-                             dst + m * kTile8 + ((c ^ (ct & 7)) << 4)),
-                         "r"(term[m][0]), "r"(term[m][1]), "r"(term[m][2]), "r"(term[m][3])
-                         : "memory");
+            *reinterpret_cast<uint4*>(dst + m * kTile8 + ((c ^ (ct & 7)) << 4)) =
+                make_uint4(term[m][0], term[m][1], term[m][2], term[m][3]);
         }
         qfac[((seq & 1) * 2 + tile) * kM + ct] =
             finite ? p.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23)
@@ -1111,43 +1125,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         warp_wait(JT_BAR(kBarFac + (g & 1)), (g >> 1) & 1, abort);
         warp_wait(JT_BAR(kBarVFull + g % kVRing), (g / kVRing) & 1, abort);
         const bool big = ((flag[(g & 1) * 2] | flag[(g & 1) * 2 + 1]) & 2) != 0;
-        const uint32_t src = base + L::kV8 + (g % kVRing) * kTile8;
-        const uint32_t dst = base + L::kV16 + (g & 1) * kTile16;
-        // 1024 chunks: each of the warp's 8 rounds covers 4 row pairs x 4 chunks.  Row pairs
-        // (r, r ^ 5) over r in {0, 1, 2, 3} (+ 8 per group of rows).
+        const unsigned char* src = sbase + L::kV8 + (g % kVRing) * kTile8;
+        unsigned char* dst = sbase + L::kV16 + (g & 1) * kTile16;
+        const uint2* mult = vm + (g & 1) * kN;
+        // 1024 chunks: each of the warp's 8 rounds covers 4 row pairs (r, r ^ 5), r in 0..3 of
+        // a group of 8 rows, x 4 chunks.
 #pragma unroll 2
         for (int i = 0; i < 8; ++i) {
           const int unit = (warp - 4) * 32 + i * 4 + quad;  // [0, 128): row group, pair, half
           const int half = unit & 1, pair = (unit >> 1) & 3, rows8 = unit >> 3;
           const int row = rows8 * 8 + ((sub & 4) ? (pair ^ 5) : pair);
           const int c = half * 4 + (sub & 3);
-          uint32_t w[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(src + row * 128 + ((c ^ (row & 7)) << 4)));
-          const uint2 m = vm[(g & 1) * kN + row];
+          const uint4 w = *reinterpret_cast<const uint4*>(src + row * 128 + ((c ^ (row & 7)) << 4));
+          const uint2 m = mult[row];
           uint32_t o[8];
+          widen(w.x, o[0], o[1]);
+          widen(w.y, o[2], o[3]);
+          widen(w.z, o[4], o[5]);
+          widen(w.w, o[6], o[7]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            widen(w[k], o[2 * k], o[2 * k + 1]);
-            o[2 * k] = mul_bf16x2(o[2 * k], m.x);
-            o[2 * k + 1] = mul_bf16x2(o[2 * k + 1], m.x);
-          }
+          for (int k = 0; k < 8; ++k) o[k] = mul_bf16x2(o[k], m.x);
           if (big) {
             // Saturating: an infinity would reach rows that do not see this key.
 #pragma unroll
             for (int k = 0; k < 8; ++k) o[k] = clamp_bf16x2(mul_bf16x2(o[k], m.y));
           }
-          const uint32_t row_dst = dst + (c >> 2) * kHalf16 + row * 128;
+          unsigned char* row_dst = dst + half * kHalf16 + row * 128;
           const int c0 = (2 * c) & 7;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(
-                           row_dst + ((c0 ^ (row & 7)) << 4)),
-                       "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
-                       : "memory");
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(
-                           row_dst + (((c0 + 1) ^ (row & 7)) << 4)),
-                       "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
-                       : "memory");
+          *reinterpret_cast<uint4*>(row_dst + ((c0 ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(row_dst + (((c0 + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
         }
         fence_proxy_async();
         warp_arrive(JT_BAR(kBarBFull + (g & 1)));
@@ -1157,7 +1163,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------------ softmax + epilogue
-    regs_inc<kRegsSoftmax>();
     const int s = (warp - 8) >> 2;           // stream
     const int row = tid - 256 - s * 128;     // query-tile row, TMEM lane
     const uint32_t lanes = static_cast<uint32_t>((row >> 5) * 32) << 16;
@@ -1178,12 +1183,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float* bias = p.qq_bias + __ldg(p.qq_bias_offsets + it.r);
       const int t_first = it.two ? 0 : s, t_step = it.two ? 1 : 2;
       // Words of the next tile that needs a mask, built ahead of it.
-      uint32_t mw[4] = {0u, 0u, 0u, 0u};
+      uint4 mw = make_uint4(0u, 0u, 0u, 0u);
       // First masked tile of this stream: tiles below floor(P / 128) need none.
       int t_mask = max(0, it.P / kN - it.t0);
       if (!it.two && ((t_mask ^ s) & 1)) ++t_mask;
       if (live && t_mask < n)
-        mask_words(bias, (it.t0 + t_mask) * kN, it.P, it.T, it.key_end, j, ok, mw);
+        mw = mask_words(bias, (it.t0 + t_mask) * kN, it.P, it.T, it.key_end, j, ok);
       float m_run = -INFINITY, l_run = 0.f, c_row = 0.f;
       for (int t = t_first; t < n; t += t_step) {
         const uint32_t g = g0 + t;
@@ -1198,12 +1203,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (live) {
           const bool masked = t >= t_mask;
           const bool nan_row = ((flag[(g & 1) * 2] | flag[(g & 1) * 2 + 1]) & 1) != 0;
-          float alpha;
-          if (!masked && nan_row) mw[0] = mw[1] = mw[2] = mw[3] = 0xffffffffu;
-          if (masked || nan_row)
-            softmax_row<kWide, true>(s_addr, kf + (g & 1) * kN, c_row, mw, m_run, l_run, alpha);
-          else
-            softmax_row<kWide, false>(s_addr, kf + (g & 1) * kN, c_row, mw, m_run, l_run, alpha);
+          if (!masked && nan_row) mw = make_uint4(~0u, ~0u, ~0u, ~0u);
+          const RowState st =
+              masked || nan_row
+                  ? softmax_masked<kWide>(s_addr, kf + (g & 1) * kN, c_row, mw, m_run, l_run)
+                  : softmax_body<kWide, false>(s_addr, kf + (g & 1) * kN, c_row, mw, m_run, l_run);
+          m_run = st.m;
+          l_run = st.l;
+          const float alpha = st.alpha;
           // The scores of this tile were issued behind the previous PV of the stream, so that
           // PV has completed: O can be rescaled at once.
           if (t != t_first && __any_sync(0xffffffffu, alpha != 1.f)) {
@@ -1223,7 +1230,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // The masks of the next masked tile, behind this tile's product.
           const int t_next = masked ? t + t_step : t_mask;
           if ((masked || nan_row) && t_next < n)
-            mask_words(bias, (it.t0 + t_next) * kN, it.P, it.T, it.key_end, j, ok, mw);
+            mw = mask_words(bias, (it.t0 + t_next) * kN, it.P, it.T, it.key_end, j, ok);
         } else {
           // No live row in this warp: its rows of P are never read out.
           tc_fence_before();
@@ -1233,77 +1240,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Epilogue, once the piece's last PV has completed.
       warp_wait(JT_BAR(kBarODone), seq & 1, abort);
       tc_fence_after();
-      const Workspace w = carve(p.workspace);
-      const int64_t out_row =
-          (static_cast<int64_t>(it.q_start) + j) * p.out_stride0 +
-          (static_cast<int64_t>(it.h) * ge.groups + head_in) * p.out_stride1;
-      if (it.two) {
-        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-        if (live) {
-          if (it.slot >= 0 && ok)
-            w.ml[(it.slot * 2ll + s) * kM + row] = make_float2(m_run, l_run);
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            __syncwarp();
-            tmem_ld32(tmem + lanes + col_o(s) + 32 * c, o);
-            tmem_wait_ld();
-            if (!ok) continue;
-            if (it.slot >= 0) {
-              float4* dst = w.o + ((it.slot * 2ll + s) * 32 + 8 * c) * kM + row;
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                dst[k * kM] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
-                                          __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
-            } else if (32 * c < p.head_dim) {
-              float f[32];
-#pragma unroll
-              for (int k = 0; k < 32; ++k) f[k] = l_run == 0.f ? 0.f : __uint_as_float(o[k]) * inv;
-              store_columns(p, out_row + 32 * c, f, p.head_dim - 32 * c);
-            }
-          }
-        }
-      } else {
-        // The streams' rows meet: each warpgroup merges and writes 64 of the columns.
+      // One query tile: the streams' rows meet, and each warpgroup merges and writes 64 of the
+      // columns.  Two: each warpgroup writes all columns of its own tile.
+      const bool pair = !it.two;
+      float fa = 1.f, fb = 0.f, m = m_run, l = l_run;
+      if (pair) {
         xch[s * kM + row] = make_float2(m_run, l_run);
         warp_arrive(JT_BAR(kBarX));
         warp_wait(JT_BAR(kBarX), x_phase, abort);
         x_phase ^= 1u;
-        if (live) {
-          const float2 a = xch[row], b = n > 1 ? xch[kM + row] : make_float2(-INFINITY, 0.f);
-          const float m = fmaxf(a.x, b.x);
-          const float fa = a.x == -INFINITY ? 0.f : jt::fast_exp2(a.x - m);
-          const float fb = b.x == -INFINITY ? 0.f : jt::fast_exp2(b.x - m);
-          const float l = a.y * (a.x == -INFINITY ? 1.f : fa) + (n > 1 ? b.y * (b.x == -INFINITY ? 1.f : fb) : 0.f);
+        const float2 a = xch[row], b = n > 1 ? xch[kM + row] : make_float2(-INFINITY, 0.f);
+        m = fmaxf(a.x, b.x);
+        fa = a.x == -INFINITY ? 0.f : jt::fast_exp2(a.x - m);
+        fb = b.x == -INFINITY ? 0.f : jt::fast_exp2(b.x - m);
+        // A stream without a maximum has a zero sum, or a NaN that has to stay.
+        l = a.y * (a.x == -INFINITY ? 1.f : fa) + b.y * (b.x == -INFINITY ? 1.f : fb);
+      }
+      if (live) {
+        const Workspace w = carve(p.workspace);
+        const int tile = pair ? 0 : s;
+        if (it.slot >= 0) {
+          if (ok && (!pair || s == 0)) w.ml[(it.slot * 2ll + tile) * kM + row] = make_float2(m, l);
+        } else {
           const float inv = l == 0.f ? 0.f : 1.f / l;
-          if (it.slot >= 0 && ok && s == 0) w.ml[it.slot * 2ll * kM + row] = make_float2(m, l);
+          fa *= inv;
+          fb *= inv;
+        }
+        const int64_t out_row = (static_cast<int64_t>(it.q_start) + j) * p.out_stride0 +
+                                (static_cast<int64_t>(it.h) * ge.groups + head_in) * p.out_stride1;
+        const int c_end = pair ? 4 * s + 4 : 8;
 #pragma unroll 1
-          for (int c = 2 * s; c < 2 * s + 2; ++c) {
-            uint32_t o0[32], o1[32];
-            __syncwarp();
-            tmem_ld32(tmem + lanes + col_o(0) + 32 * c, o0);
-            if (n > 1) {
-              tmem_ld32(tmem + lanes + col_o(1) + 32 * c, o1);
-            } else {
+        for (int c = pair ? 4 * s : 0; c < c_end; ++c) {  // 16 columns
+          uint32_t o0[16], o1[16];
+          __syncwarp();
+          tmem_ld16(tmem + lanes + col_o(tile) + 16 * c, o0);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o1[k] = 0u;
+          for (int k = 0; k < 16; ++k) o1[k] = 0u;
+          if (pair && n > 1) tmem_ld16(tmem + lanes + col_o(1) + 16 * c, o1);
+          tmem_wait_ld();
+          float f[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            f[k] = __uint_as_float(o0[k]) * fa + __uint_as_float(o1[k]) * fb;
+          if (ok && it.slot >= 0) {
+            float4* dst = w.o + ((it.slot * 2ll + tile) * 32 + 4 * c) * kM + row;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              dst[k * kM] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+          } else if (ok && 16 * c < p.head_dim) {
+            if (l == 0.f) {  // the row sees no key
+#pragma unroll
+              for (int k = 0; k < 16; ++k) f[k] = 0.f;
             }
-            tmem_wait_ld();
-            if (!ok) continue;
-            float f[32];
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              f[k] = __uint_as_float(o0[k]) * fa + __uint_as_float(o1[k]) * fb;
-            if (it.slot >= 0) {
-              float4* dst = w.o + (it.slot * 2ll * 32 + 8 * c) * kM + row;
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                dst[k * kM] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
-            } else if (32 * c < p.head_dim) {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) f[k] = l == 0.f ? 0.f : f[k] * inv;
-              store_columns(p, out_row + 32 * c, f, p.head_dim - 32 * c);
-            }
+            store_columns<kWide>(p, out_row + 16 * c, f);
           }
         }
       }
@@ -1367,10 +1356,10 @@ __global__ void __launch_bounds__(kM) tree_attn_fp8_merge_kernel(
   const int h = first.h * p.groups + (row - local * p.groups);
   const int64_t at = (static_cast<int64_t>(p.cu_seqlens_q[first.r]) + j) * p.out_stride0 +
                      h * p.out_stride1 + 4 * cg0;
-  float f[32];
+  float f[16];
 #pragma unroll
-  for (int k = 0; k < 32; ++k) f[k] = k < 16 && l != 0.f ? acc[k & 15] * inv : 0.f;
-  store_columns(p, at, f, 16);
+  for (int k = 0; k < 16; ++k) f[k] = l != 0.f ? acc[k] * inv : 0.f;
+  store_columns<kWide>(p, at, f);
 }
 
 bool al16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
