@@ -30,9 +30,8 @@
 //
 //   warp 0       MMA issuer, TMEM owner (S0, S1, O0, O1: 128 columns each)
 //   warp 1       work pieces; TMA loads of K, V and scale bytes for prefix tiles
-//   warps 2-3    scale factors of every tile; cp.async gathers of tiles that touch tree nodes
-//                or pages TMA cannot box
-//   warps 4-7    queries -> e4m3 terms; V codes -> bf16 tile
+//   warps 2-3    cp.async gathers of tiles that touch tree nodes or pages TMA cannot box
+//   warps 4-7    queries -> e4m3 terms; scale bytes -> key factors; V codes -> bf16 tile
 //   warps 8-15   softmax + epilogue, one warpgroup per stream, one thread per row
 //
 // Every mbarrier wait is bounded; one that runs out sets JT_DEVERR_TIMEOUT and the CTA's
@@ -52,7 +51,10 @@ constexpr int kN = 128;               // keys per tile
 constexpr int kM = 128;               // rows per query tile
 constexpr int kD = 128;               // head dim in shared memory (shorter heads: zeros)
 constexpr int kThreads = 512;
-constexpr int kKRing = 3, kVRing = 2, kScaleRing = 4;
+constexpr int kKRing = 3, kVRing = 2;
+// The scale bytes' ring: a slot is refilled with tile g + 8 once QK g + 5 has been issued, hence
+// after PV g + 3, hence after the converters read tile g's.
+constexpr int kScaleRing = 8;
 constexpr int kTile8 = kN * kD;       // bytes of a code tile
 constexpr int kTile16 = 2 * kTile8;   // bytes of a bf16 tile: two 64-dim halves
 constexpr int kHalf16 = kTile8;
@@ -76,14 +78,13 @@ struct Smem {
   static constexpr int kV16 = kV8 + kVRing * kTile8;
   static constexpr int kScale = kV16 + 2 * kTile16;          // [kScaleRing][K, V][128] bytes
   static constexpr int kKf = kScale + kScaleRing * 256;       // [2][128] float
-  static constexpr int kVm = kKf + 2 * kN * 4;                // [2][128] uint2
-  static constexpr int kQfac = kVm + 2 * kN * 8;              // [2][2][128] float
+  static constexpr int kQfac = kKf + 2 * kN * 4;              // [2][2][128] float
   static constexpr int kX = kQfac + 4 * kM * 4;               // [2][128] float2: max, sum
   static constexpr int kItem = kX + 2 * kM * 8;               // [2][16] int
-  static constexpr int kFlag = kItem + 2 * 64;                // [2][2] int
-  static constexpr int kMisc = kFlag + 32;                    // TMEM base, abort
+  static constexpr int kFlag = kItem + 2 * 64;                // [2][4] int
+  static constexpr int kMisc = kFlag + 32;                    // TMEM base, abort, free slots
   static constexpr int kBar = kMisc + 32;
-  static constexpr int kBytes = kBar + 8 * 32 + 1024;         // + alignment slack
+  static constexpr int kBytes = kBar + 8 * 48 + 1024;         // + alignment slack
   static_assert(kBytes <= 227 * 1024, "shared memory per CTA");
 };
 
@@ -92,38 +93,38 @@ constexpr int kBarKFull = 0;     // [3] TMA (arrive_tx + arrive) or two gather w
 constexpr int kBarKEmpty = 3;    // [3] commit after the tile's last QK
 constexpr int kBarVFull = 6;     // [2] TMA or two gather warps
 constexpr int kBarVEmpty = 8;    // [2] 4 converter warps
-constexpr int kBarFac = 10;      // [2] 2 gather warps: the tile's factors are written
+constexpr int kBarFac = 10;      // [2] 4 converter warps: the tile's factors are written
 constexpr int kBarBFull = 12;    // [2] 4 converter warps: the tile's bf16 V is written
 constexpr int kBarBEmpty = 14;   // [2] commit after the tile's last PV
 constexpr int kBarQFull = 16;    // [2] 4 converter warps, by piece parity
 constexpr int kBarQEmpty = 18;   // commit after a piece's last QK
 constexpr int kBarSFull = 19;    // [2] commit per QK, by stream
-constexpr int kBarPFull = 21;    // [2] 4 softmax warps, by stream
-constexpr int kBarODone = 23;    // commit after a piece's last PV
-constexpr int kBarOFree = 24;    // 8 softmax warps: the epilogue has read O
-constexpr int kBarX = 25;        // 8 softmax warps: (max, sum) exchanged
-constexpr int kBarItemFull = 26;   // [2] publisher
-constexpr int kBarItemEmpty = 28;  // [2] every warp
-constexpr int kBarDrain = 30;
-constexpr int kNumBars = 31;
-static_assert(kNumBars <= 32, "barrier area");
+constexpr int kBarPFull = 21;    // [2 streams][2 half tiles] 4 softmax warps
+constexpr int kBarPvHalf = 25;   // [2] commit after the first half tile's PV, by stream
+constexpr int kBarODone = 27;    // commit after a piece's last PV
+constexpr int kBarOFree = 28;    // 8 softmax warps: the epilogue has read O
+constexpr int kBarX = 29;        // 8 softmax warps: (max, sum) exchanged
+constexpr int kBarItemFull = 30;   // [2] publisher
+constexpr int kBarItemEmpty = 32;  // [2] every warp
+constexpr int kBarDrain = 34;
+constexpr int kBarScale = 35;      // [8] as KFull, for the tile's scale bytes
+constexpr int kNumBars = 43;
+static_assert(kNumBars <= 48, "barrier area");
 
 __device__ __forceinline__ uint32_t bar_count(int i) {
   if (i < kBarKEmpty) return 2;
   if (i < kBarVFull) return 1;
   if (i < kBarVEmpty) return 2;
-  if (i < kBarFac) return 4;
-  if (i < kBarBFull) return 2;
-  if (i < kBarBEmpty) return 4;
+  if (i < kBarBEmpty) return 4;  // VEmpty, Fac, BFull
   if (i < kBarQFull) return 1;
   if (i < kBarQEmpty) return 4;
   if (i < kBarPFull) return 1;   // QEmpty, SFull
-  if (i < kBarODone) return 4;
-  if (i == kBarODone) return 1;
+  if (i < kBarPvHalf) return 4;
+  if (i < kBarOFree) return 1;   // PvHalf, ODone
   if (i < kBarItemFull) return 8;
   if (i < kBarItemEmpty) return 1;
   if (i < kBarDrain) return kThreads / 32;
-  return 1;
+  return i < kBarScale ? 1 : 2;
 }
 
 // TMEM columns.
@@ -177,6 +178,30 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Release store / bounded acquire wait on a counter in shared memory that only grows (a
+// difference below 2^31 counts as reached).
+__device__ __forceinline__ void st_release_shared(uint32_t addr, uint32_t v) {
+  asm volatile("st.release.cta.shared::cta.u32 [%0], %1;\n" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __noinline__ void wait_shared_at_least(uint32_t addr, uint32_t target,
+                                                  volatile int* abort) {
+  const long long start = clock64();
+  for (;;) {
+    uint32_t v;
+    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];\n" : "=r"(v) : "r"(addr) : "memory");
+    if (static_cast<int>(v - target) >= 0 || *abort) return;
+    if (clock64() - start > kWaitLimit) {
+      *abort = 1;
+      atomicOr(&g_attn_fp8_errors, JT_DEVERR_TIMEOUT);
+      return;
+    }
+  }
+}
 __device__ __forceinline__ void fence_proxy_async() {
   asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
 }
@@ -187,22 +212,22 @@ __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 }
 // Warp-wide forms: elect.sync picks the one issuing lane (always the same for a full warp).
-__device__ __forceinline__ void commit_warp(uint32_t bar) {
+__device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile(
       "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
       " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
           bar)
       : "memory");
 }
-__device__ __forceinline__ void mma_f8_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                            uint32_t acc) {
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
       " @e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
-__device__ __forceinline__ void mma_ts_warp(uint32_t d, uint32_t a_tmem, uint64_t b,
-                                            uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc,
+                                       uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
       " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
@@ -270,6 +295,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
+                 "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(taddr),
+               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 }
@@ -309,13 +345,17 @@ __device__ __forceinline__ uint2 v_multipliers(uint32_t b) {
   return make_uint2(m1 | (m1 << 16), m2 | (m2 << 16));
 }
 // Four e4m3 codes as bf16 pairs of value * 2^-120: the code's exponent and mantissa fields
-// dropped into bf16's (subnormal codes become bf16 subnormals of the same value).  The code
-// 0x7f (NaN), which no row of this cache holds, reads as 480: finite, so bytes of keys no row
-// sees never reach the product.
-__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  const uint32_t a = __byte_perm(w, 0u, 0x1404), b = __byte_perm(w, 0u, 0x3424);
-  lo = ((a >> 4) & 0x07f007f0u) | (a & 0x80008000u);
-  hi = ((b >> 4) & 0x07f007f0u) | (b & 0x80008000u);
+// dropped into bf16's (subnormal codes become bf16 subnormals of the same value).  The pairs
+// are codes (0, 2) and (1, 3), which saves the byte permutes: the V tile's columns, and so O's,
+// hold the head dims in the order 0, 2, 1, 3 of every four, undone where O is written out.  The
+// code 0x7f (NaN), which no row of this cache holds, reads as 480: finite, so bytes of keys
+// no row sees never reach the product.
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& even, uint32_t& odd) {
+  even = (w & 0x007f007fu) * 16u + (w & 0x00800080u) * 256u;
+  odd = ((w >> 4) & 0x07f007f0u) | (w & 0x80008000u);
+}
+__device__ __forceinline__ constexpr int o_column(int d) {  // column of head dim d in O
+  return (d & ~3) | ((d & 1) << 1) | ((d >> 1) & 1);
 }
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -475,10 +515,10 @@ __device__ __noinline__ uint4 mask_words(const float* bias, int kb, int P, int T
   const int lo = __reduce_min_sync(0xffffffffu, ok ? j : 0x7fffffff);
   const int hi = __reduce_max_sync(0xffffffffu, ok ? j : -1);
 #pragma unroll 1
-  for (int base = lo; base <= hi; base += 4) {
-    float b[4][4];
+  for (int base = lo; base <= hi; base += 2) {
+    float b[2][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int node = base + i, key = kb + 32 * w + lane - P;
@@ -491,7 +531,7 @@ __device__ __noinline__ uint4 mask_words(const float* bias, int kb, int P, int T
         }
       }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const uint32_t bits = __ballot_sync(0xffffffffu, b[i][w] == 0.f);
@@ -507,10 +547,8 @@ __device__ __forceinline__ constexpr uint32_t col_p(int kk) {
   return kk < 4 ? 8u * kk : 64u + 8u * (kk - 4);
 }
 
-// 64 scores of a row from TMEM, times the keys' factors (and -inf where masked).
-template <bool kCareful>
-__device__ __forceinline__ void load_scores(uint32_t s_addr, const float* kf, uint32_t m0,
-                                            uint32_t m1, uint32_t (&v)[64]) {
+// 64 scores of a row from TMEM, times the keys' factors.
+__device__ __forceinline__ void load_scores(uint32_t s_addr, const float* kf, uint32_t (&v)[64]) {
   tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(v));
   tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
   tmem_wait_ld();
@@ -527,44 +565,32 @@ __device__ __forceinline__ void load_scores(uint32_t s_addr, const float* kf, ui
     v[4 * k + 2] = __float_as_uint(b.x);
     v[4 * k + 3] = __float_as_uint(b.y);
   }
-  if constexpr (kCareful) {
-#pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      if (!((m0 >> k) & 1u)) v[k] = 0xff800000u;
-      if (!((m1 >> k) & 1u)) v[32 + k] = 0xff800000u;
-    }
-  }
 }
 
-// Softmax of one row of a 128-key tile, in two passes over half tiles (the scores are read
-// from TMEM twice rather than held: 128 live scores would leave too few registers for the
-// 16 warps, and the loops keep the code small enough for the instruction cache).  The running
-// maximum is lazy: it moves only when a tile exceeds it by 2^8, so P stays below 2^8 and O
-// is rarely rescaled.  kCareful (masked tiles, tiles with a NaN row): masked scores are -inf
-// and every exponential is exp2, which keeps a NaN.
+// Softmax of one row of half a tile (64 keys): the lazy running maximum (it moves only when
+// the scores exceed it by 2^8, so P stays below 2^8 and O is rarely rescaled), P to the S
+// columns the scores came from.  Half tiles keep the live scores at 64 registers and the code
+// small enough for the instruction cache (a CTA runs seven roles at once; at 200 KB of code
+// the warps waited for instructions 42 % of their time), and the first half's PV runs while
+// the second half is in here.
 struct RowState {
   float m, l, alpha;  // running maximum (log2 units) and sum; the factor older sums and O take
 };
-template <bool kWide, bool kCareful>
-__device__ __forceinline__ RowState softmax_body(uint32_t s_addr, const float* kf, float c_row,
-                                                 uint4 mw, float m_run, float l_run) {
-  float mx = -INFINITY;
-#pragma unroll 1
-  for (int h = 0; h < 2; ++h) {
-    uint32_t v[64];
-    load_scores<kCareful>(s_addr + 64 * h, kf + 64 * h, h ? mw.z : mw.x, h ? mw.w : mw.y, v);
-    float m8[8];
+template <bool kWide>
+__device__ __forceinline__ RowState softmax_half(uint32_t s_addr, const float* kf, float c_row,
+                                                 float m_run, float l_run) {
+  uint32_t v[64];
+  load_scores(s_addr, kf, v);
+  float m8[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m8[k] = fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 8]));
+  for (int k = 0; k < 8; ++k) m8[k] = fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 8]));
 #pragma unroll
-    for (int q = 16; q < 64; q += 16)
+  for (int q = 16; q < 64; q += 16)
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        m8[k] = fmaxf(m8[k], fmaxf(__uint_as_float(v[q + k]), __uint_as_float(v[q + k + 8])));
-    mx = fmaxf(mx, fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
-                         fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))));
-  }
-  mx *= c_row;
+    for (int k = 0; k < 8; ++k)
+      m8[k] = max3f(m8[k], __uint_as_float(v[q + k]), __uint_as_float(v[q + k + 8]));
+  const float mx = max3f(max3f(m8[0], m8[1], m8[2]), max3f(m8[3], m8[4], m8[5]),
+                         fmaxf(m8[6], m8[7])) * c_row;
   float alpha = 1.f;
   if (mx > m_run + 8.f) {
     if (m_run != -INFINITY) alpha = jt::fast_exp2(m_run - mx);
@@ -573,41 +599,101 @@ __device__ __forceinline__ RowState softmax_body(uint32_t s_addr, const float* k
   const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
   const float2 c2 = make_float2(c_row, c_row), n2 = make_float2(neg_m, neg_m);
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-  for (int h = 0; h < 2; ++h) {
-    uint32_t v[64];
-    load_scores<kCareful>(s_addr + 64 * h, kf + 64 * h, h ? mw.z : mw.x, h ? mw.w : mw.y, v);
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      uint32_t ph[16], pl[kWide ? 16 : 1];
+  for (int q = 0; q < 2; ++q) {
+    uint32_t ph[16], pl[kWide ? 16 : 1];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[32 * q + 2 * k]),
-                                                __uint_as_float(v[32 * q + 2 * k + 1])), c2, n2);
-        float2 e;
-        if (!kCareful && !kWide && (k & 3) == 3)
-          e = exp2_poly2(x);
-        else
-          e = make_float2(jt::fast_exp2(x.x), jt::fast_exp2(x.y));
-        sum[k & 1] = __fadd2_rn(sum[k & 1], e);
-        ph[k] = pack_bf16(e.x, e.y);
-        if constexpr (kWide) {
-          const float2 f = jt::MmaOp<__nv_bfloat16>::unpack(ph[k]);
-          pl[k] = pack_bf16(e.x - f.x, e.y - f.y);
-        }
+    for (int k = 0; k < 16; ++k) {
+      const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[32 * q + 2 * k]),
+                                              __uint_as_float(v[32 * q + 2 * k + 1])), c2, n2);
+      float2 e;
+      if (!kWide && (k & 3) == 3)
+        e = exp2_poly2(x);
+      else
+        e = make_float2(jt::fast_exp2(x.x), jt::fast_exp2(x.y));
+      sum[k & 1] = __fadd2_rn(sum[k & 1], e);
+      ph[k] = pack_bf16(e.x, e.y);
+      if constexpr (kWide) {
+        const float2 f = jt::MmaOp<__nv_bfloat16>::unpack(ph[k]);
+        pl[k] = pack_bf16(e.x - f.x, e.y - f.y);
       }
-      tmem_st16(s_addr + 64 * h + 16 * q, ph);
-      if constexpr (kWide) tmem_st16(s_addr + 64 * h + 32 + 16 * q, pl);
     }
+    tmem_st16(s_addr + 16 * q, ph);
+    if constexpr (kWide) tmem_st16(s_addr + 32 + 16 * q, pl);
   }
   return RowState{m_run, l_run * alpha + ((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)), alpha};
 }
 
-// Masked tiles (the last one or two of an item) run a copy of their own, out of line.
+// The same for tiles with masked keys or a NaN row (the last one or two of an item): masked
+// scores are -inf, every exponential is exp2, which keeps a NaN.  Two rolled passes of 8
+// columns: a few hundred instructions that run seldom cost more to fetch than to execute.
 template <bool kWide>
 __device__ __noinline__ RowState softmax_masked(uint32_t s_addr, const float* kf, float c_row,
-                                                uint4 mw, float m_run, float l_run) {
-  return softmax_body<kWide, true>(s_addr, kf, c_row, mw, m_run, l_run);
+                                                uint32_t m0, uint32_t m1, float m_run,
+                                                float l_run) {
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 8; ++c) {
+    uint32_t v[8];
+    tmem_ld8(s_addr + 8 * c, v);
+    tmem_wait_ld();
+    const uint32_t bits = (c < 4 ? m0 : m1) >> (8 * (c & 3));
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      mx = fmaxf(mx, (bits >> k) & 1u ? __uint_as_float(v[k]) * kf[8 * c + k] : -INFINITY);
+  }
+  mx *= c_row;
+  float alpha = 1.f;
+  if (mx > m_run + 8.f) {
+    if (m_run != -INFINITY) alpha = jt::fast_exp2(m_run - mx);
+    m_run = mx;
+  }
+  const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+  float sum = 0.f;
+  if constexpr (kWide) {
+    // The low parts go where scores of later columns still are: all are read first.
+    uint32_t v[64], pl[32];
+    load_scores(s_addr, kf, v);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint32_t ph[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        float e[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int col = 2 * k + i;
+          const float x = ((q ? m1 : m0) >> col) & 1u ? __uint_as_float(v[32 * q + col]) : -INFINITY;
+          e[i] = jt::fast_exp2(fmaf(x, c_row, neg_m));
+          sum += e[i];
+        }
+        ph[k] = pack_bf16(e[0], e[1]);
+        const float2 f = jt::MmaOp<__nv_bfloat16>::unpack(ph[k]);
+        pl[16 * q + k] = pack_bf16(e[0] - f.x, e[1] - f.y);
+      }
+      tmem_st16(s_addr + 16 * q, ph);
+    }
+    tmem_st32(s_addr + 32, pl);
+  } else {
+#pragma unroll 1
+    for (int c = 0; c < 8; ++c) {
+      uint32_t v[8], ph[4];
+      tmem_ld8(s_addr + 8 * c, v);
+      tmem_wait_ld();
+      const uint32_t bits = (c < 4 ? m0 : m1) >> (8 * (c & 3));
+      float e[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float x = (bits >> k) & 1u ? __uint_as_float(v[k]) * kf[8 * c + k] : -INFINITY;
+        e[k] = jt::fast_exp2(fmaf(x, c_row, neg_m));
+        sum += e[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ph[k] = pack_bf16(e[2 * k], e[2 * k + 1]);
+      tmem_st4(s_addr + 4 * c, ph);  // over scores already read
+    }
+  }
+  return RowState{m_run, l_run * alpha + sum, alpha};
 }
 
 // 16 output columns of one row.  The narrow kernel's output is bf16.
@@ -621,20 +707,23 @@ __device__ __forceinline__ void store_columns(const JtTreeAttnFp8Params& p, int6
       dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
     return;
   }
-  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
+  uint32_t w[8];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      w[e] = !kWide || p.out_dtype == JT_BF16
-                 ? pack_bf16(o[8 * k + 2 * e], o[8 * k + 2 * e + 1])
-                 : jt::MmaOp<__half>::pack(o[8 * k + 2 * e], o[8 * k + 2 * e + 1]);
-    dst[k] = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int e = 0; e < 8; ++e)
+    w[e] = !kWide || p.out_dtype == JT_BF16 ? pack_bf16(o[2 * e], o[2 * e + 1])
+                                            : jt::MmaOp<__half>::pack(o[2 * e], o[2 * e + 1]);
+  uint16_t* dst = static_cast<uint16_t*>(p.out) + at;
+  if ((reinterpret_cast<uintptr_t>(dst) & 31u) == 0) {  // a whole sector per lane
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst), "r"(w[0]),
+                 "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
 }
 
-template <bool kWide>
+template <bool kWide, typename QT>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_attn_fp8_kernel(const __grid_constant__ JtTreeAttnFp8Params p,
                          const __grid_constant__ CUtensorMap kmap,
@@ -653,10 +742,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Geometry ge{p.groups, kM / p.groups, (kM / p.groups) * L::kTiles};
 
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  if (tid < kNumBars) mbar_init(JT_BAR(tid), bar_count(tid));
-  if (tid == 0) {
-    misc[1] = 0;
+  if (tid == 0) misc[1] = misc[2] = misc[3] = 0;
+  if (tid < kNumBars) {
+    mbar_init(JT_BAR(tid), bar_count(tid));
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    fence_proxy_async();
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(
@@ -758,18 +848,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t g = g0 + (u >> two);
             if (!two || s == 0) mbar_wait(JT_BAR(kBarBFull + (g & 1)), (g >> 1) & 1, abort);
             if (u == 0 && seq > 0) mbar_wait(JT_BAR(kBarOFree), (seq - 1) & 1, abort);
-            mbar_wait(JT_BAR(kBarPFull + s), (p_phase >> s) & 1, abort);
-            p_phase ^= 1u << s;
-            tc_fence_after();
             const uint64_t vd = v_desc + (g & 1) * (kTile16 >> 4);
-#pragma unroll 1
-            for (int kk = 0; kk < kN / 16; ++kk) {
-              mma_ts_warp(d_o, d_s + col_p(kk), vd + kk * (2048 / 16), kIdescPV,
-                          u > 1 || kk > 0 ? 1u : 0u);
-              if constexpr (kWide)
-                mma_ts_warp(d_o, d_s + col_p(kk) + 32, vd + kk * (2048 / 16), kIdescPV, 1u);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              mbar_wait(JT_BAR(kBarPFull + 2 * s + h), (p_phase >> s) & 1, abort);
+              tc_fence_after();
+#pragma unroll
+              for (int kk = 4 * h; kk < 4 * h + 4; ++kk) {
+                mma_ts(d_o, d_s + col_p(kk), vd + kk * (2048 / 16), kIdescPV,
+                            u > 1 || kk > 0 ? 1u : 0u);
+                if constexpr (kWide)
+                  mma_ts(d_o, d_s + col_p(kk) + 32, vd + kk * (2048 / 16), kIdescPV, 1u);
+              }
+              if (h == 0) commit(JT_BAR(kBarPvHalf + s));
             }
-            if (!two || s == 1) commit_warp(JT_BAR(kBarBEmpty + (g & 1)));
+            p_phase ^= 1u << s;
+            if (!two || s == 1) commit(JT_BAR(kBarBEmpty + (g & 1)));
           }
           if (u + 2 < steps) {
             const int t = (u + 2) >> two;
@@ -780,21 +874,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const uint64_t qd = q_desc + (two & s) * (kTerms * kTile8 / 16);
             const uint64_t kd = k_desc + (g % kKRing) * (kTile8 >> 4);
-#pragma unroll 1
+#pragma unroll
             for (int i = 0; i < kTerms * 4; ++i)  // (term, 32 dims)
-              mma_f8_warp(d_s, qd + (i >> 2) * (kTile8 / 16) + (i & 3) * 2, kd + (i & 3) * 2,
+              mma_f8(d_s, qd + (i >> 2) * (kTile8 / 16) + (i & 3) * 2, kd + (i & 3) * 2,
                           kIdescQK, i != 0 ? 1u : 0u);
-            commit_warp(JT_BAR(kBarSFull + s));
+            commit(JT_BAR(kBarSFull + s));
             if (!two || s == 1) {
-              commit_warp(JT_BAR(kBarKEmpty + g % kKRing));
-              if (t == n - 1) commit_warp(JT_BAR(kBarQEmpty));
+              commit(JT_BAR(kBarKEmpty + g % kKRing));
+              if (t == n - 1) commit(JT_BAR(kBarQEmpty));
             }
           }
         }
-        commit_warp(JT_BAR(kBarODone));
+        commit(JT_BAR(kBarODone));
         g0 += n;
       }
-      commit_warp(JT_BAR(kBarDrain));
+      commit(JT_BAR(kBarDrain));
       mbar_wait(JT_BAR(kBarDrain), 0, abort, false);
     } else if (warp == 1) {
       // ---------------------------------------------------------------- pieces and TMA
@@ -869,15 +963,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_arrive(JT_BAR(kBarItemFull + slot));
       };
-      uint32_t g0 = 0, k_used = 0, v_used = 0;
+      uint32_t g0 = 0;
+      // Full barriers whose last fill is TMA's, as bits (K 0.., V 4.., scales 8..), and the
+      // phase parity of that fill: what the drain waits for.
+      uint32_t mine = 0, parity = 0;
+      auto note = [&](int bit, bool by_tma, uint32_t phase) {
+        mine = (mine & ~(1u << bit)) | (by_tma ? 1u << bit : 0u);
+        parity = (parity & ~(1u << bit)) | ((phase & 1u) << bit);
+      };
       if (lane == 0) publish(0);
       const char* ksc = static_cast<const char*>(p.k_scale);
       const char* vsc = static_cast<const char*>(p.v_scale);
-      uint32_t last_k[kKRing], last_v[kVRing];
-#pragma unroll
-      for (int i = 0; i < kKRing; ++i) last_k[i] = 0;
-#pragma unroll
-      for (int i = 0; i < kVRing; ++i) last_v[i] = 0;
       for (uint32_t seq = 0;; ++seq) {
         Piece it;
         if (!next_piece(seq, it)) break;
@@ -888,17 +984,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t g = g0 + t;
           const int ring = is_v ? kVRing : kKRing;
           const int slot = g % ring;
-          if (!plan.tma || kb + kN > it.P) {
-            // Gathered by warps 2-3, which wait for the slot's last TMA fill to be consumed.
-            (is_v ? v_used : k_used) &= ~(1u << slot);
-            return;
-          }
-          const uint32_t full = JT_BAR((is_v ? kBarVFull : kBarKFull) + slot);
+          // This lane alone waits on the rings' empty barriers, for every tile in order: a
+          // parity wait is right only for a waiter that is at most one phase behind.
           if (g >= static_cast<uint32_t>(ring))
             mbar_wait(JT_BAR((is_v ? kBarVEmpty : kBarKEmpty) + slot), ((g / ring) & 1) ^ 1, abort);
           if (*abort) return;
+          if (!plan.tma || kb + kN > it.P) {  // gathered by warps 2-3, told that the slot is free
+            note(is_v ? 4 + slot : slot, false, 0);
+            if (!is_v) note(8 + g % kScaleRing, false, 0);
+            st_release_shared(base + L::kMisc + (is_v ? 12 : 8), g + 1);
+            return;
+          }
+          const uint32_t full = JT_BAR((is_v ? kBarVFull : kBarKFull) + slot);
           const uint32_t dst = base + (is_v ? L::kV8 : L::kK) + slot * kTile8;
-          mbar_arrive_tx(full, is_v ? kTile8 : kTile8 + 2 * kN);
+          const uint32_t sc_slot = g % kScaleRing, sc_full = JT_BAR(kBarScale + sc_slot);
+          mbar_arrive_tx(full, kTile8);
+          if (!is_v) mbar_arrive_tx(sc_full, 2 * kN);
 #pragma unroll 1
           for (int i = 0; i < kN; i += plan.box) {
             const int pos = kb + i, off = pos % p.block_size;
@@ -911,14 +1012,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_4d(dst + i * kD, is_v ? &vmap : &kmap, 0, it.h, off, page, full);
             if (!is_v) {
               const int64_t pg = max(page, 0);
-              const uint32_t sdst = base + L::kScale + (g % kScaleRing) * 256 + i;
-              bulk_load(sdst, ksc + pg * p.ks_stride0 + it.h * p.ks_stride1 + off, plan.box, full);
-              bulk_load(sdst + kN, vsc + pg * p.vs_stride0 + it.h * p.vs_stride1 + off, plan.box, full);
+              const uint32_t sdst = base + L::kScale + sc_slot * 256 + i;
+              bulk_load(sdst, ksc + pg * p.ks_stride0 + it.h * p.ks_stride1 + off, plan.box, sc_full);
+              bulk_load(sdst + kN, vsc + pg * p.vs_stride0 + it.h * p.vs_stride1 + off, plan.box, sc_full);
             }
           }
           mbar_arrive(full);
-          if (is_v) { last_v[slot] = g / ring + 1; v_used |= 1u << slot; }
-          else { last_k[slot] = g / ring + 1; k_used |= 1u << slot; }
+          note(is_v ? 4 + slot : slot, true, g / ring);
+          if (!is_v) {
+            mbar_arrive(sc_full);
+            note(8 + sc_slot, true, g / kScaleRing);
+          }
         };
         if (lane == 0) {
           // K 0, K 1, then V t and K t + 2: the order in which they are used.
@@ -935,96 +1039,63 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (lane == 0) {
         // The copies this lane started have landed before the CTA exits.
-#pragma unroll
-        for (int i = 0; i < kKRing; ++i)
-          if (k_used & (1u << i)) mbar_wait(JT_BAR(kBarKFull + i), (last_k[i] - 1) & 1, abort, false);
-#pragma unroll
-        for (int i = 0; i < kVRing; ++i)
-          if (v_used & (1u << i)) mbar_wait(JT_BAR(kBarVFull + i), (last_v[i] - 1) & 1, abort, false);
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i)
+          if (mine & (1u << i)) {
+            const int bar = i < 4 ? kBarKFull + i : i < 8 ? kBarVFull + i - 4 : kBarScale + i - 8;
+            mbar_wait(JT_BAR(bar), (parity >> i) & 1u, abort, false);
+          }
         PieceMeta* m = carve(p.workspace).meta + 2 * blockIdx.x;
         m[0].valid = meta_valid[0];
         m[1].valid = meta_valid[1];
       }
     } else {
-      // ---------------------------------------------------------------- factors and gathers
+      // ---------------------------------------------------------------- gathers
+      // Tiles that TMA does not take: rows by cp.async, scale bytes by plain loads into the
+      // same staging.
       const int gt = tid - 64;  // two keys per thread
-      uint32_t g0 = 0;
-      float* kf = reinterpret_cast<float*>(sbase + L::kKf);
-      uint2* vm = reinterpret_cast<uint2*>(sbase + L::kVm);
-      volatile int* flag = reinterpret_cast<volatile int*>(sbase + L::kFlag);
       const int chunks = p.head_dim / 16;
+      uint32_t g0 = 0;
+#pragma unroll 1
       for (uint32_t seq = 0;; ++seq) {
         Piece it;
         if (!next_piece(seq, it)) break;
         const int32_t* table = p.block_tables + static_cast<int64_t>(it.r) * p.table_stride0;
-        for (int t = 0; t < it.n; ++t) {
+#pragma unroll 1
+        for (int t = plan.tma ? max(0, it.P / kN - it.t0) : 0; t < it.n; ++t) {
           const uint32_t g = g0 + t;
-          const int kb = (it.t0 + t) * kN;
-          const bool by_tma = plan.tma && kb + kN <= it.P;
-          uint32_t kbyte[2], vbyte[2];
-          int64_t page[2], off[2];
-          if (by_tma) {
-            warp_wait(JT_BAR(kBarKFull + g % kKRing), (g / kKRing) & 1, abort);
-            const unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256;
-            const uint32_t k2 = *reinterpret_cast<const uint16_t*>(sc + 2 * gt);
-            const uint32_t v2 = *reinterpret_cast<const uint16_t*>(sc + kN + 2 * gt);
-            kbyte[0] = k2 & 0xff; kbyte[1] = k2 >> 8;
-            vbyte[0] = v2 & 0xff; vbyte[1] = v2 >> 8;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const KeyPlace at = locate_key(p, table, kb + 2 * gt + i, it.P, it.key_end, it.q_start);
-              page[i] = at.page;
-              off[i] = at.off;
-              kbyte[i] = vbyte[i] = 127;
-              if (page[i] >= 0) {
-                kbyte[i] = __ldg(static_cast<const uint8_t*>(p.k_scale) + page[i] * p.ks_stride0 +
-                                 it.h * p.ks_stride1 + off[i]);
-                vbyte[i] = __ldg(static_cast<const uint8_t*>(p.v_scale) + page[i] * p.vs_stride0 +
-                                 it.h * p.vs_stride1 + off[i]);
-              }
-            }
-            if (g >= kKRing)
-              warp_wait(JT_BAR(kBarKEmpty + g % kKRing), ((g / kKRing) & 1) ^ 1, abort);
-            const uint32_t dst = base + L::kK + (g % kKRing) * kTile8;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const char* src = static_cast<const char*>(p.k_pool);
-              if (page[i] >= 0)
-                src += page[i] * p.k_stride0 + off[i] * p.k_stride1 + it.h * p.k_stride2;
-              gather_row(dst, 2 * gt + i, src, page[i] >= 0 ? chunks : 0);
-            }
-            asm volatile("cp.async.wait_all;\n" ::: "memory");
-            fence_proxy_async();
-            warp_arrive(JT_BAR(kBarKFull + g % kKRing));
-          }
-          // The factor buffers of tile g - 2 are free once its last PV has completed.
-          if (g >= 2) warp_wait(JT_BAR(kBarBEmpty + (g & 1)), ((g >> 1) & 1) ^ 1, abort);
-          int seen = 0;
-#pragma unroll
+          const uint32_t ks = g % kKRing, vs = g % kVRing;
+          wait_shared_at_least(base + L::kMisc + 8, g + 1, abort);
+          wait_shared_at_least(base + L::kMisc + 12, g + 1, abort);
+          __syncwarp();
+#pragma unroll 1
           for (int i = 0; i < 2; ++i) {
-            const int at = (g & 1) * kN + 2 * gt + i;
-            kf[at] = vbyte[i] == 255u ? scale_value(255u) : scale_value(kbyte[i]);
-            vm[at] = v_multipliers(vbyte[i]);
-            if (kbyte[i] == 255u || vbyte[i] == 255u) seen |= 1;  // a NaN row
-            if (vbyte[i] > 134u) seen |= 2;                        // a second V multiplier
-          }
-          seen = __reduce_or_sync(0xffffffffu, seen);
-          if (lane == 0) flag[(g & 1) * 2 + (warp - 2)] = seen;
-          warp_arrive(JT_BAR(kBarFac + (g & 1)));
-          if (!by_tma) {
-            if (g >= kVRing)
-              warp_wait(JT_BAR(kBarVEmpty + g % kVRing), ((g / kVRing) & 1) ^ 1, abort);
-            const uint32_t dst = base + L::kV8 + (g % kVRing) * kTile8;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const char* src = static_cast<const char*>(p.v_pool);
-              if (page[i] >= 0)
-                src += page[i] * p.v_stride0 + off[i] * p.v_stride1 + it.h * p.v_stride2;
-              gather_row(dst, 2 * gt + i, src, page[i] >= 0 ? chunks : 0);
+            const int row = 2 * gt + i;
+            const KeyPlace at = locate_key(p, table, (it.t0 + t) * kN + row, it.P, it.key_end, it.q_start);
+            const bool ok = at.page >= 0;
+            const char* k = static_cast<const char*>(p.k_pool);
+            const char* v = static_cast<const char*>(p.v_pool);
+            uint8_t kb = 127, vb = 127;
+            if (ok) {
+              k += at.page * p.k_stride0 + at.off * p.k_stride1 + it.h * p.k_stride2;
+              v += at.page * p.v_stride0 + at.off * p.v_stride1 + it.h * p.v_stride2;
+              kb = __ldg(static_cast<const uint8_t*>(p.k_scale) + at.page * p.ks_stride0 +
+                         it.h * p.ks_stride1 + at.off);
+              vb = __ldg(static_cast<const uint8_t*>(p.v_scale) + at.page * p.vs_stride0 +
+                         it.h * p.vs_stride1 + at.off);
             }
-            asm volatile("cp.async.wait_all;\n" ::: "memory");
-            warp_arrive(JT_BAR(kBarVFull + g % kVRing));
+            gather_row(base + L::kK + ks * kTile8, row, k, ok ? chunks : 0);
+            gather_row(base + L::kV8 + vs * kTile8, row, v, ok ? chunks : 0);
+            unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256 + row;
+            sc[0] = kb;
+            sc[kN] = vb;
+          }
+          asm volatile("cp.async.wait_all;\n" ::: "memory");
+          fence_proxy_async();
+          warp_arrive(JT_BAR(kBarKFull + ks));
+          if (lane == 0) {
+            mbar_arrive(JT_BAR(kBarVFull + vs));
+            mbar_arrive(JT_BAR(kBarScale + g % kScaleRing));
           }
         }
         g0 += it.n;
@@ -1032,131 +1103,140 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------------ converters
-    const int ct = tid - 128;  // query row; V chunk index
+    const int ct = tid - 128, cw = warp - 4;  // this thread's key; this warp's 32 rows
     uint32_t g0 = 0;
+    float* kf = reinterpret_cast<float*>(sbase + L::kKf);
     float* qfac = reinterpret_cast<float*>(sbase + L::kQfac);
-    const uint2* vm = reinterpret_cast<const uint2*>(sbase + L::kVm);
-    const volatile int* flag = reinterpret_cast<const volatile int*>(sbase + L::kFlag);
+    volatile int* flag = reinterpret_cast<volatile int*>(sbase + L::kFlag);
     // V: eight lanes of a warp take four 16-byte chunks of rows r and r ^ 5, so that both the
     // swizzled loads and the swizzled stores of the eight touch different banks.
     const int quad = lane >> 3, sub = lane & 7;
+    const int v_half = quad & 1, v_chunk = v_half * 4 + (sub & 3);
+#pragma unroll 1
     for (uint32_t seq = 0;; ++seq) {
       Piece it;
       if (!next_piece(seq, it)) break;
       if (seq > 0) warp_wait(JT_BAR(kBarQEmpty), (seq - 1) & 1, abort);
+      // Queries: half a warp per row (16 bytes per lane), its largest magnitude by shuffles,
+      // then e4m3 terms of row / 2^e.  Rows without a query keep whatever is there: their
+      // scores are never used.  Four rows' loads are in flight.
+      const int first = it.mb * ge.npi, nodes = min(it.T, first + ge.npi) - first;
+      const int tiles = it.two ? 2 : 1;
+      const int hl = lane & 15, hw = lane >> 4;
 #pragma unroll 1
-      for (int tile = 0; tile < (it.two ? 2 : 1); ++tile) {
-        // One row per thread: its largest magnitude, then e4m3 terms of row / 2^e.
-        const int local = ct / ge.groups;
-        const int j = it.mb * ge.npi + tile * ge.npt + local;
-        const bool ok = local < ge.npt && j < it.T;
-        const uint4* src = nullptr;
-        if (ok)
-          src = reinterpret_cast<const uint4*>(
-              static_cast<const uint16_t*>(p.q) + (static_cast<int64_t>(it.q_start) + j) * p.q_stride0 +
-              (static_cast<int64_t>(it.h) * ge.groups + (ct - local * ge.groups)) * p.q_stride1);
-        const bool is_bf16 = p.dtype == JT_BF16;
-        auto unpack2 = [&](uint32_t w) {
-          return is_bf16 ? jt::MmaOp<__nv_bfloat16>::unpack(w) : jt::MmaOp<__half>::unpack(w);
-        };
-        const int words = ok ? p.head_dim / 8 : 0;  // 16-byte words of a row
-        uint32_t top = 0;
-#pragma unroll 1
-        for (int i = 0; i < words; i += 4) {
-          uint4 w[4];
+      for (int i0 = 0; i0 < 16 * tiles; i0 += 4) {
+        uint4 w[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[k] = i + k < words ? __ldg(src + i + k) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < 4; ++i) {
+          const int tile = (i0 + i) >> 4, row = cw * 32 + ((i0 + i) & 15) * 2 + hw;
+          const int local = row / ge.groups, j = tile * ge.npt + local;
+          w[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (local < ge.npt && j < nodes && 8 * hl < p.head_dim)
+            w[i] = __ldg(reinterpret_cast<const uint4*>(
+                static_cast<const QT*>(p.q) + (static_cast<int64_t>(it.q_start) + first + j) * p.q_stride0 +
+                (static_cast<int64_t>(it.h) * ge.groups + (row - local * ge.groups)) * p.q_stride1 + 8 * hl));
+        }
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          const int tile = (i0 + i) >> 4, row = cw * 32 + ((i0 + i) & 15) * 2 + hw;
+          const uint32_t a[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+          w[0] = w[1];
+          w[1] = w[2];
+          w[2] = w[3];
+          // The operands' own bits order like their magnitudes.
+          uint32_t top = __vmaxu2(__vmaxu2(a[0] & 0x7fff7fffu, a[1] & 0x7fff7fffu),
+                                  __vmaxu2(a[2] & 0x7fff7fffu, a[3] & 0x7fff7fffu));
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+          top = __float_as_uint(jt::MmaOp<QT>::unpack(max(top & 0xffffu, top >> 16)).x);
+          const bool finite = top < 0x7f800000u;
+          int e = 0;
+          if (top != 0 && finite)
+            e = max(static_cast<int>(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u), -126);
+          const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+          float2 x[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            // The operand's own bits order like the magnitude: the type is undone at the end.
-            const uint32_t a = w[k].x & 0x7fff7fffu, b = w[k].y & 0x7fff7fffu;
-            const uint32_t c = w[k].z & 0x7fff7fffu, d = w[k].w & 0x7fff7fffu;
-            top = __vmaxu2(top, __vmaxu2(__vmaxu2(a, b), __vmaxu2(c, d)));
+            x[k] = jt::MmaOp<QT>::unpack(a[k]);
+            x[k] = make_float2(x[k].x * inv, x[k].y * inv);
           }
-        }
-        top = max(top & 0xffffu, top >> 16);
-        top = __float_as_uint(unpack2(top).x);
-        const bool finite = top < 0x7f800000u;
-        int e = 0;
-        if (top != 0 && finite)
-          e = max(static_cast<int>(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u), -126);
-        // A row with a non-finite element enters as zeros; its factor makes its scores NaN.
-        const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        unsigned char* dst = sbase + L::kQ + tile * kTerms * kTile8 + ct * 128;
-#pragma unroll 1
-        for (int c = 0; c < 8; ++c) {
-          uint32_t term[kTerms][4];
-          uint4 w[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-          if (2 * c < words && finite) {
-            w[0] = __ldg(src + 2 * c);
-            w[1] = __ldg(src + 2 * c + 1);
-          }
+          unsigned char* dst = sbase + L::kQ + tile * kTerms * kTile8 + row * 128 +
+                               (((hl >> 1) ^ (row & 7)) << 4) + (hl & 1) * 8;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 u = w[i >> 1];
-            float2 x0 = unpack2(i & 1 ? u.z : u.x), x1 = unpack2(i & 1 ? u.w : u.y);
-            x0 = make_float2(x0.x * inv, x0.y * inv);
-            x1 = make_float2(x1.x * inv, x1.y * inv);
+          for (int m = 0; m < kTerms; ++m) {
+            uint32_t t[4];
 #pragma unroll
-            for (int m = 0; m < kTerms; ++m) {
-              const uint32_t a = pack_e4m3(x0.x, x0.y), b = pack_e4m3(x1.x, x1.y);
-              term[m][i] = a | (b << 16);
-              const float2 ya = unpack_e4m3(a), yb = unpack_e4m3(b);
-              x0 = make_float2(x0.x - ya.x, x0.y - ya.y);
-              x1 = make_float2(x1.x - yb.x, x1.y - yb.y);
+            for (int k = 0; k < 4; ++k) {
+              t[k] = pack_e4m3(x[k].x, x[k].y);
+              const float2 y = unpack_e4m3(t[k]);
+              x[k] = make_float2(x[k].x - y.x, x[k].y - y.y);
             }
+            *reinterpret_cast<uint2*>(dst + m * kTile8) =
+                make_uint2(t[0] | (t[1] << 16), t[2] | (t[3] << 16));
           }
-#pragma unroll
-          for (int m = 0; m < kTerms; ++m)
-            *reinterpret_cast<uint4*>(dst + m * kTile8 + ((c ^ (ct & 7)) << 4)) =
-                make_uint4(term[m][0], term[m][1], term[m][2], term[m][3]);
+          // A row with a non-finite element: its factor makes its scores NaN.
+          if (hl == 0)
+            qfac[((seq & 1) * 2 + tile) * kM + row] =
+                finite ? p.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23)
+                       : __uint_as_float(0x7fc00000u);
         }
-        qfac[((seq & 1) * 2 + tile) * kM + ct] =
-            finite ? p.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23)
-                   : __uint_as_float(0x7fc00000u);
       }
       fence_proxy_async();
       warp_arrive(JT_BAR(kBarQFull + (seq & 1)));
+#pragma unroll 1
       for (int t = 0; t < it.n; ++t) {
-        const uint32_t g = g0 + t;
-        // The factors of tile g are written after the last PV of tile g - 2, whose bf16 tile
-        // is therefore free too.
-        warp_wait(JT_BAR(kBarFac + (g & 1)), (g >> 1) & 1, abort);
+        const uint32_t g = g0 + t, buf = g & 1;
+        // Factors of this thread's key, once the tile's scale bytes are here and the buffers
+        // of tile g - 2 are free (its last PV has completed).
+        warp_wait(JT_BAR(kBarScale + g % kScaleRing), (g / kScaleRing) & 1, abort);
+        const unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256 + ct;
+        const uint32_t kb = sc[0], vb = sc[kN];
+        if (g >= 2) warp_wait(JT_BAR(kBarBEmpty + buf), ((g >> 1) & 1) ^ 1, abort);
+        kf[buf * kN + ct] = vb == 255u ? scale_value(255u) : scale_value(kb);
+        const uint2 mine = v_multipliers(vb);
+        const bool nan = __any_sync(0xffffffffu, kb == 255u || vb == 255u);
+        const bool big = __any_sync(0xffffffffu, vb > 134u);  // needs the second multiplier
+        if (lane == 0) flag[buf * 4 + cw] = nan;
+        warp_arrive(JT_BAR(kBarFac + buf));
         warp_wait(JT_BAR(kBarVFull + g % kVRing), (g / kVRing) & 1, abort);
-        const bool big = ((flag[(g & 1) * 2] | flag[(g & 1) * 2 + 1]) & 2) != 0;
-        const unsigned char* src = sbase + L::kV8 + (g % kVRing) * kTile8;
-        unsigned char* dst = sbase + L::kV16 + (g & 1) * kTile16;
-        const uint2* mult = vm + (g & 1) * kN;
-        // 1024 chunks: each of the warp's 8 rounds covers 4 row pairs (r, r ^ 5), r in 0..3 of
-        // a group of 8 rows, x 4 chunks.
-#pragma unroll 2
-        for (int i = 0; i < 8; ++i) {
-          const int unit = (warp - 4) * 32 + i * 4 + quad;  // [0, 128): row group, pair, half
-          const int half = unit & 1, pair = (unit >> 1) & 3, rows8 = unit >> 3;
-          const int row = rows8 * 8 + ((sub & 4) ? (pair ^ 5) : pair);
-          const int c = half * 4 + (sub & 3);
-          const uint4 w = *reinterpret_cast<const uint4*>(src + row * 128 + ((c ^ (row & 7)) << 4));
-          const uint2 m = mult[row];
-          uint32_t o[8];
-          widen(w.x, o[0], o[1]);
-          widen(w.y, o[2], o[3]);
-          widen(w.z, o[4], o[5]);
-          widen(w.w, o[6], o[7]);
+        // This warp's 32 rows x 8 chunks in 8 rounds, four rounds' loads in flight at a time.
+        const unsigned char* src = sbase + L::kV8 + (g % kVRing) * kTile8 + cw * (32 * 128);
+        unsigned char* dst = sbase + L::kV16 + buf * kTile16 + v_half * kHalf16 + cw * (32 * 128);
+#pragma unroll 1
+        for (int i0 = 0; i0 < 8; i0 += 4) {
+          uint4 w[4];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] = mul_bf16x2(o[k], m.x);
-          if (big) {
-            // Saturating: an infinity would reach rows that do not see this key.
-#pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = clamp_bf16x2(mul_bf16x2(o[k], m.y));
+          for (int i = 0; i < 4; ++i) {
+            const int pr = (quad >> 1) + 2 * (i & 1);
+            const int row = ((i0 + i) >> 1) * 8 + ((sub & 4) ? (pr ^ 5) : pr);
+            w[i] = *reinterpret_cast<const uint4*>(src + row * 128 + ((v_chunk ^ (row & 7)) << 4));
           }
-          unsigned char* row_dst = dst + half * kHalf16 + row * 128;
-          const int c0 = (2 * c) & 7;
-          *reinterpret_cast<uint4*>(row_dst + ((c0 ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(row_dst + (((c0 + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int pr = (quad >> 1) + 2 * (i & 1);
+            const int row = ((i0 + i) >> 1) * 8 + ((sub & 4) ? (pr ^ 5) : pr);
+            const uint32_t m = __shfl_sync(0xffffffffu, mine.x, row);
+            uint32_t o[8];
+            widen(w[i].x, o[0], o[1]);
+            widen(w[i].y, o[2], o[3]);
+            widen(w[i].z, o[4], o[5]);
+            widen(w[i].w, o[6], o[7]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = mul_bf16x2(o[k], m);
+            if (big) {
+              // Saturating: an infinity would reach rows that do not see this key.
+              const uint32_t m2 = __shfl_sync(0xffffffffu, mine.y, row);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) o[k] = clamp_bf16x2(mul_bf16x2(o[k], m2));
+            }
+            unsigned char* row_dst = dst + row * 128;
+            const int c0 = 2 * (sub & 3);
+            *reinterpret_cast<uint4*>(row_dst + ((c0 ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(row_dst + (((c0 + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
         }
         fence_proxy_async();
-        warp_arrive(JT_BAR(kBarBFull + (g & 1)));
+        warp_arrive(JT_BAR(kBarBFull + buf));
         if (lane == 0) mbar_arrive(JT_BAR(kBarVEmpty + g % kVRing));
       }
       g0 += it.n;
@@ -1183,12 +1263,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float* bias = p.qq_bias + __ldg(p.qq_bias_offsets + it.r);
       const int t_first = it.two ? 0 : s, t_step = it.two ? 1 : 2;
       // Words of the next tile that needs a mask, built ahead of it.
-      uint4 mw = make_uint4(0u, 0u, 0u, 0u);
+      uint4 mw = make_uint4(0u, 0u, 0u, 0u), mw_first = mw;
       // First masked tile of this stream: tiles below floor(P / 128) need none.
       int t_mask = max(0, it.P / kN - it.t0);
       if (!it.two && ((t_mask ^ s) & 1)) ++t_mask;
       if (live && t_mask < n)
-        mw = mask_words(bias, (it.t0 + t_mask) * kN, it.P, it.T, it.key_end, j, ok);
+        mw_first = mask_words(bias, (it.t0 + t_mask) * kN, it.P, it.T, it.key_end, j, ok);
       float m_run = -INFINITY, l_run = 0.f, c_row = 0.f;
       for (int t = t_first; t < n; t += t_step) {
         const uint32_t g = g0 + t;
@@ -1200,42 +1280,47 @@ __global__ void __launch_bounds__(kThreads, 1)
         warp_wait(JT_BAR(kBarSFull + s), step & 1, abort);
         ++step;
         tc_fence_after();
-        if (live) {
-          const bool masked = t >= t_mask;
-          const bool nan_row = ((flag[(g & 1) * 2] | flag[(g & 1) * 2 + 1]) & 1) != 0;
-          if (!masked && nan_row) mw = make_uint4(~0u, ~0u, ~0u, ~0u);
-          const RowState st =
-              masked || nan_row
-                  ? softmax_masked<kWide>(s_addr, kf + (g & 1) * kN, c_row, mw, m_run, l_run)
-                  : softmax_body<kWide, false>(s_addr, kf + (g & 1) * kN, c_row, mw, m_run, l_run);
-          m_run = st.m;
-          l_run = st.l;
-          const float alpha = st.alpha;
-          // The scores of this tile were issued behind the previous PV of the stream, so that
-          // PV has completed: O can be rescaled at once.
-          if (t != t_first && __any_sync(0xffffffffu, alpha != 1.f)) {
+        const bool masked = t >= t_mask;
+        const bool careful =
+            masked || (flag[(g & 1) * 4] | flag[(g & 1) * 4 + 1] | flag[(g & 1) * 4 + 2] |
+                       flag[(g & 1) * 4 + 3]) != 0;
+        if (!masked) mw = make_uint4(~0u, ~0u, ~0u, ~0u);
+        else if (t == t_mask) mw = mw_first;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t o[32];
-              tmem_ld32(tmem + lanes + col_o(s) + 32 * c, o);
-              tmem_wait_ld();
+        for (int h = 0; h < 2; ++h) {
+          if (live) {
+            const float* f = kf + (g & 1) * kN + 64 * h;
+            const RowState st =
+                careful ? softmax_masked<kWide>(s_addr + 64 * h, f, c_row, h ? mw.z : mw.x,
+                                                h ? mw.w : mw.y, m_run, l_run)
+                        : softmax_half<kWide>(s_addr + 64 * h, f, c_row, m_run, l_run);
+            m_run = st.m;
+            l_run = st.l;
+            // O can be rescaled once the stream's last PV has completed: for a tile's first
+            // half the scores themselves were issued behind it, for the second half it is
+            // the first half's.
+            if ((t != t_first || h) && __any_sync(0xffffffffu, st.alpha != 1.f)) {
+              if (h) warp_wait(JT_BAR(kBarPvHalf + s), (step - 1) & 1, abort);
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                uint32_t o[32];
+                tmem_ld32(tmem + lanes + col_o(s) + 32 * c, o);
+                tmem_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-              tmem_st32(tmem + lanes + col_o(s) + 32 * c, o);
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * st.alpha);
+                tmem_st32(tmem + lanes + col_o(s) + 32 * c, o);
+              }
             }
+            tmem_wait_st();
           }
-          tmem_wait_st();
+          // A warp without a live row arrives too; its rows of P are never read out.
           tc_fence_before();
-          warp_arrive(JT_BAR(kBarPFull + s));
-          // The masks of the next masked tile, behind this tile's product.
-          const int t_next = masked ? t + t_step : t_mask;
-          if ((masked || nan_row) && t_next < n)
-            mw = mask_words(bias, (it.t0 + t_next) * kN, it.P, it.T, it.key_end, j, ok);
-        } else {
-          // No live row in this warp: its rows of P are never read out.
-          tc_fence_before();
-          warp_arrive(JT_BAR(kBarPFull + s));
+          warp_arrive(JT_BAR(kBarPFull + 2 * s + h));
         }
+        // The masks of the next masked tile, behind this tile's product.
+        if (live && masked && t + t_step < n)
+          mw = mask_words(bias, (it.t0 + t + t_step) * kN, it.P, it.T, it.key_end, j, ok);
       }
       // Epilogue, once the piece's last PV has completed.
       warp_wait(JT_BAR(kBarODone), seq & 1, abort);
@@ -1281,7 +1366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float f[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k)
-            f[k] = __uint_as_float(o0[k]) * fa + __uint_as_float(o1[k]) * fb;
+            f[k] = __uint_as_float(o0[o_column(k)]) * fa + __uint_as_float(o1[o_column(k)]) * fb;
           if (ok && it.slot >= 0) {
             float4* dst = w.o + ((it.slot * 2ll + tile) * 32 + 4 * c) * kM + row;
 #pragma unroll
@@ -1397,7 +1482,7 @@ bool encode_pool(CUtensorMap* map, const JtTreeAttnFp8Params& p, const void* poo
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool kWide>
+template <bool kWide, typename QT>
 int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
   LoadPlan plan{};
   // TMA where a tile is whole boxes of whole pages: pages of whole tiles, or powers of two
@@ -1411,7 +1496,7 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
       (!encode_pool(&kmap, p, p.k_pool, p.k_stride0, p.k_stride1, p.k_stride2, plan.box) ||
        !encode_pool(&vmap, p, p.v_pool, p.v_stride0, p.v_stride1, p.v_stride2, plan.box)))
     plan.tma = 0;  // a layout the encoder refuses: gathered like any other page size
-  auto kernel = tree_attn_fp8_kernel<kWide>;
+  auto kernel = tree_attn_fp8_kernel<kWide, QT>;
   int rc = jt_cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                               Smem<kWide>::kBytes),
                          "tree_attn_fp8 smem attribute");
@@ -1486,6 +1571,7 @@ extern "C" int jt_tree_attn_fp8_launch(const JtTreeAttnFp8Params* p, cudaStream_
   if (rc != JT_OK) return rc;
   rc = jt_cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "SM count");
   if (rc != JT_OK) return rc;
-  return p->dtype == JT_BF16 && p->out_dtype == JT_BF16 ? launch<false>(*p, sms, stream)
-                                                        : launch<true>(*p, sms, stream);
+  if (p->dtype == JT_F16) return launch<true, __half>(*p, sms, stream);
+  return p->out_dtype == JT_BF16 ? launch<false, __nv_bfloat16>(*p, sms, stream)
+                                 : launch<true, __nv_bfloat16>(*p, sms, stream);
 }
