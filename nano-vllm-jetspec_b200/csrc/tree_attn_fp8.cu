@@ -32,7 +32,8 @@
 //   warp 1       work pieces; TMA loads of K, V and scale bytes for prefix tiles
 //   warps 2-3    cp.async gathers of tiles that touch tree nodes or pages TMA cannot box
 //   warps 4-7    queries -> e4m3 terms; scale bytes -> key factors; V codes -> bf16 tile
-//   warps 8-15   softmax + epilogue, one warpgroup per stream, one thread per row
+//   warps 8-23   softmax + epilogue: two warpgroups per stream, each with 64 of a tile's keys
+//                and one thread per row
 //
 // Every mbarrier wait is bounded; one that runs out sets JT_DEVERR_TIMEOUT and the CTA's
 // abort flag, all roles leave their loops, drain what they started and free the TMEM.
@@ -50,7 +51,7 @@ __device__ uint32_t g_attn_fp8_errors;
 constexpr int kN = 128;               // keys per tile
 constexpr int kM = 128;               // rows per query tile
 constexpr int kD = 128;               // head dim in shared memory (shorter heads: zeros)
-constexpr int kThreads = 512;
+constexpr int kThreads = 768;
 constexpr int kKRing = 3, kVRing = 2;
 // The scale bytes' ring: a slot is refilled with tile g + 8 once QK g + 5 has been issued, hence
 // after PV g + 3, hence after the converters read tile g's.
@@ -79,12 +80,13 @@ struct Smem {
   static constexpr int kScale = kV16 + 2 * kTile16;          // [kScaleRing][K, V][128] bytes
   static constexpr int kKf = kScale + kScaleRing * 256;       // [2][128] float
   static constexpr int kQfac = kKf + 2 * kN * 4;              // [2][2][128] float
-  static constexpr int kX = kQfac + 4 * kM * 4;               // [2][128] float2: max, sum
-  static constexpr int kItem = kX + 2 * kM * 8;               // [2][16] int
+  static constexpr int kX = kQfac + 4 * kM * 4;               // [stream][half][128] float2: max, sum
+  static constexpr int kMx = kX + 4 * kM * 8;                 // [2][stream][half][128] float
+  static constexpr int kItem = kMx + 8 * kM * 4;              // [2][16] int
   static constexpr int kFlag = kItem + 2 * 64;                // [2][4] int
   static constexpr int kMisc = kFlag + 32;                    // TMEM base, abort, free slots
   static constexpr int kBar = kMisc + 32;
-  static constexpr int kBytes = kBar + 8 * 48 + 1024;         // + alignment slack
+  static constexpr int kBytes = kBar + 8 * 64 + 1024;         // + alignment slack
   static_assert(kBytes <= 227 * 1024, "shared memory per CTA");
 };
 
@@ -99,17 +101,17 @@ constexpr int kBarBEmpty = 14;   // [2] commit after the tile's last PV
 constexpr int kBarQFull = 16;    // [2] 4 converter warps, by piece parity
 constexpr int kBarQEmpty = 18;   // commit after a piece's last QK
 constexpr int kBarSFull = 19;    // [2] commit per QK, by stream
-constexpr int kBarPFull = 21;    // [2 streams][2 half tiles] 4 softmax warps
-constexpr int kBarPvHalf = 25;   // [2] commit after the first half tile's PV, by stream
-constexpr int kBarODone = 27;    // commit after a piece's last PV
-constexpr int kBarOFree = 28;    // 8 softmax warps: the epilogue has read O
-constexpr int kBarX = 29;        // 8 softmax warps: (max, sum) exchanged
-constexpr int kBarItemFull = 30;   // [2] publisher
-constexpr int kBarItemEmpty = 32;  // [2] every warp
-constexpr int kBarDrain = 34;
-constexpr int kBarScale = 35;      // [8] as KFull, for the tile's scale bytes
-constexpr int kNumBars = 43;
-static_assert(kNumBars <= 48, "barrier area");
+constexpr int kBarPFull = 21;    // [2] 8 softmax warps, by stream
+constexpr int kBarODone = 23;    // commit after a piece's last PV
+constexpr int kBarOFree = 24;    // 16 softmax warps: the epilogue has read O
+constexpr int kBarX = 25;        // 16 softmax warps: (max, sum) exchanged
+constexpr int kBarItemFull = 26;   // [2] publisher
+constexpr int kBarItemEmpty = 28;  // [2] every warp
+constexpr int kBarDrain = 30;
+constexpr int kBarScale = 31;      // [8] as KFull, for the tile's scale bytes
+constexpr int kBarMx = 39;         // [stream][32 rows] the two warps that share rows: half maxima
+constexpr int kNumBars = 47;
+static_assert(kNumBars <= 64, "barrier area");
 
 __device__ __forceinline__ uint32_t bar_count(int i) {
   if (i < kBarKEmpty) return 2;
@@ -119,12 +121,12 @@ __device__ __forceinline__ uint32_t bar_count(int i) {
   if (i < kBarQFull) return 1;
   if (i < kBarQEmpty) return 4;
   if (i < kBarPFull) return 1;   // QEmpty, SFull
-  if (i < kBarPvHalf) return 4;
-  if (i < kBarOFree) return 1;   // PvHalf, ODone
-  if (i < kBarItemFull) return 8;
+  if (i < kBarODone) return 8;
+  if (i == kBarODone) return 1;
+  if (i < kBarItemFull) return 16;
   if (i < kBarItemEmpty) return 1;
   if (i < kBarDrain) return kThreads / 32;
-  return i < kBarScale ? 1 : 2;
+  return i < kBarScale ? 1 : 2;  // Drain; Scale, Mx
 }
 
 // TMEM columns.
@@ -505,25 +507,25 @@ struct LoadPlan {
   int box;
 };
 
-// Visibility words of the 128 keys at kb for this lane's row: bit b of word w is key
+// Visibility words of the 64 keys at kb for this lane's row: bit b of word w is key
 // kb + 32 w + b.  Each warp builds its rows' words node by node: lane b reads the bias of its
 // key, a ballot collects the word, and the lanes of that node keep it.
-__device__ __noinline__ uint4 mask_words(const float* bias, int kb, int P, int T, int key_end,
+__device__ __noinline__ uint2 mask_words(const float* bias, int kb, int P, int T, int key_end,
                                          int j, bool ok) {
   const int lane = threadIdx.x & 31;
-  uint32_t mw[4] = {0u, 0u, 0u, 0u};
+  uint32_t mw[2] = {0u, 0u};
   const int lo = __reduce_min_sync(0xffffffffu, ok ? j : 0x7fffffff);
   const int hi = __reduce_max_sync(0xffffffffu, ok ? j : -1);
 #pragma unroll 1
-  for (int base = lo; base <= hi; base += 2) {
-    float b[2][4];
+  for (int base = lo; base <= hi; base += 4) {
+    float b[4][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < 2; ++w) {
         const int node = base + i, key = kb + 32 * w + lane - P;
         b[i][w] = -INFINITY;
-        if (node <= hi && kb + 32 * w + lane < key_end) {
+        if (node <= hi && key + P < key_end) {
           if (key < 0)
             b[i][w] = 0.f;
           else if (key <= node)
@@ -531,14 +533,14 @@ __device__ __noinline__ uint4 mask_words(const float* bias, int kb, int P, int T
         }
       }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < 2; ++w) {
         const uint32_t bits = __ballot_sync(0xffffffffu, b[i][w] == 0.f);
         if (ok && j == base + i) mw[w] = bits;
       }
   }
-  return make_uint4(mw[0], mw[1], mw[2], mw[3]);
+  return make_uint2(mw[0], mw[1]);
 }
 
 // Columns of P inside an S buffer: keys 16 kk .. 16 kk + 15 (8 columns of bf16 pairs).  Each
@@ -547,14 +549,17 @@ __device__ __forceinline__ constexpr uint32_t col_p(int kk) {
   return kk < 4 ? 8u * kk : 64u + 8u * (kk - 4);
 }
 
-// 64 scores of a row from TMEM, times the keys' factors.
-__device__ __forceinline__ void load_scores(uint32_t s_addr, const float* kf, uint32_t (&v)[64]) {
-  tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(v));
-  tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+// The largest of a row's 64 scores (times the keys' factors) of half a tile, and then, with the
+// row's running maximum known, their probabilities.  The scores are read from TMEM twice, 32 at
+// a time, rather than held: with 24 warps a thread has 80 registers, and four softmax warps per
+// scheduler hide each other's latencies, which two with the scores in registers do not (a
+// half tile took 712 cycles of a scheduler with two, 555 with four).
+__device__ __forceinline__ void load_scores(uint32_t s_addr, const float* kf, uint32_t (&v)[32]) {
+  tmem_ld32(s_addr, v);
   tmem_wait_ld();
   const float4* f4 = reinterpret_cast<const float4*>(kf);
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
+  for (int k = 0; k < 8; ++k) {
     const float4 f = f4[k];
     const float2 a = __fmul2_rn(make_float2(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1])),
                                 make_float2(f.x, f.y));
@@ -566,46 +571,41 @@ __device__ __forceinline__ void load_scores(uint32_t s_addr, const float* kf, ui
     v[4 * k + 3] = __float_as_uint(b.y);
   }
 }
-
-// Softmax of one row of half a tile (64 keys): the lazy running maximum (it moves only when
-// the scores exceed it by 2^8, so P stays below 2^8 and O is rarely rescaled), P to the S
-// columns the scores came from.  Half tiles keep the live scores at 64 registers and the code
-// small enough for the instruction cache (a CTA runs seven roles at once; at 200 KB of code
-// the warps waited for instructions 42 % of their time), and the first half's PV runs while
-// the second half is in here.
-struct RowState {
-  float m, l, alpha;  // running maximum (log2 units) and sum; the factor older sums and O take
-};
-template <bool kWide>
-__device__ __forceinline__ RowState softmax_half(uint32_t s_addr, const float* kf, float c_row,
-                                                 float m_run, float l_run) {
-  uint32_t v[64];
-  load_scores(s_addr, kf, v);
-  float m8[8];
+__device__ __forceinline__ float half_max(uint32_t s_addr, const float* kf) {
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int q = 0; q < 2; ++q) {
+    uint32_t v[32];
+    load_scores(s_addr + 32 * q, kf + 32 * q, v);
+    float m8[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) m8[k] = fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 8]));
-#pragma unroll
-  for (int q = 16; q < 64; q += 16)
+    for (int k = 0; k < 8; ++k) m8[k] = fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 8]));
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      m8[k] = max3f(m8[k], __uint_as_float(v[q + k]), __uint_as_float(v[q + k + 8]));
-  const float mx = max3f(max3f(m8[0], m8[1], m8[2]), max3f(m8[3], m8[4], m8[5]),
-                         fmaxf(m8[6], m8[7])) * c_row;
-  float alpha = 1.f;
-  if (mx > m_run + 8.f) {
-    if (m_run != -INFINITY) alpha = jt::fast_exp2(m_run - mx);
-    m_run = mx;
+      m8[k] = max3f(m8[k], __uint_as_float(v[k + 16]), __uint_as_float(v[k + 24]));
+    mx = max3f(mx, max3f(m8[0], m8[1], m8[2]), max3f(m8[3], m8[4], m8[5]));
+    mx = max3f(mx, m8[6], m8[7]);
   }
-  const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+  return mx;
+}
+// P = exp2(score * c_row - m), rounded to bf16, to the S columns the scores came from (its low
+// parts 32 columns on, for wide outputs); returns the fp32 sum.
+template <bool kWide>
+__device__ __forceinline__ float half_exp(uint32_t s_addr, const float* kf, float c_row, float neg_m) {
   const float2 c2 = make_float2(c_row, c_row), n2 = make_float2(neg_m, neg_m);
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
+  uint32_t low[kWide ? 16 : 1];
+#pragma unroll(kWide ? 2 : 1)
   for (int q = 0; q < 2; ++q) {
-    uint32_t ph[16], pl[kWide ? 16 : 1];
+    uint32_t v[32], ph[16];
+    load_scores(s_addr + 32 * q, kf + 32 * q, v);
+    // The first low parts go where the second scores were.
+    if constexpr (kWide)
+      if (q == 1) tmem_st16(s_addr + 32, low);
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
-      const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[32 * q + 2 * k]),
-                                              __uint_as_float(v[32 * q + 2 * k + 1])), c2, n2);
+      const float2 x = __ffma2_rn(
+          make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), c2, n2);
       float2 e;
       if (!kWide && (k & 3) == 3)
         e = exp2_poly2(x);
@@ -615,22 +615,20 @@ __device__ __forceinline__ RowState softmax_half(uint32_t s_addr, const float* k
       ph[k] = pack_bf16(e.x, e.y);
       if constexpr (kWide) {
         const float2 f = jt::MmaOp<__nv_bfloat16>::unpack(ph[k]);
-        pl[k] = pack_bf16(e.x - f.x, e.y - f.y);
+        low[k] = pack_bf16(e.x - f.x, e.y - f.y);
       }
     }
     tmem_st16(s_addr + 16 * q, ph);
-    if constexpr (kWide) tmem_st16(s_addr + 32 + 16 * q, pl);
   }
-  return RowState{m_run, l_run * alpha + ((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)), alpha};
+  if constexpr (kWide) tmem_st16(s_addr + 48, low);
+  return (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
 }
 
 // The same for tiles with masked keys or a NaN row (the last one or two of an item): masked
-// scores are -inf, every exponential is exp2, which keeps a NaN.  Two rolled passes of 8
-// columns: a few hundred instructions that run seldom cost more to fetch than to execute.
-template <bool kWide>
-__device__ __noinline__ RowState softmax_masked(uint32_t s_addr, const float* kf, float c_row,
-                                                uint32_t m0, uint32_t m1, float m_run,
-                                                float l_run) {
+// scores are -inf, every exponential is exp2, which keeps a NaN.  Rolled over 8 columns: a few
+// hundred instructions that run seldom cost more to fetch than to execute.
+__device__ __noinline__ float half_max_masked(uint32_t s_addr, const float* kf, uint32_t m0,
+                                              uint32_t m1) {
   float mx = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < 8; ++c) {
@@ -642,38 +640,36 @@ __device__ __noinline__ RowState softmax_masked(uint32_t s_addr, const float* kf
     for (int k = 0; k < 8; ++k)
       mx = fmaxf(mx, (bits >> k) & 1u ? __uint_as_float(v[k]) * kf[8 * c + k] : -INFINITY);
   }
-  mx *= c_row;
-  float alpha = 1.f;
-  if (mx > m_run + 8.f) {
-    if (m_run != -INFINITY) alpha = jt::fast_exp2(m_run - mx);
-    m_run = mx;
-  }
-  const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+  return mx;
+}
+template <bool kWide>
+__device__ __noinline__ float half_exp_masked(uint32_t s_addr, const float* kf, float c_row,
+                                              float neg_m, uint32_t m0, uint32_t m1) {
   float sum = 0.f;
   if constexpr (kWide) {
-    // The low parts go where scores of later columns still are: all are read first.
-    uint32_t v[64], pl[32];
-    load_scores(s_addr, kf, v);
+    uint32_t low[16];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      uint32_t ph[16];
+      uint32_t v[32], ph[16];
+      load_scores(s_addr + 32 * q, kf + 32 * q, v);
+      if (q == 1) tmem_st16(s_addr + 32, low);
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         float e[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int col = 2 * k + i;
-          const float x = ((q ? m1 : m0) >> col) & 1u ? __uint_as_float(v[32 * q + col]) : -INFINITY;
+          const float x = ((q ? m1 : m0) >> col) & 1u ? __uint_as_float(v[col]) : -INFINITY;
           e[i] = jt::fast_exp2(fmaf(x, c_row, neg_m));
           sum += e[i];
         }
         ph[k] = pack_bf16(e[0], e[1]);
         const float2 f = jt::MmaOp<__nv_bfloat16>::unpack(ph[k]);
-        pl[16 * q + k] = pack_bf16(e[0] - f.x, e[1] - f.y);
+        low[k] = pack_bf16(e[0] - f.x, e[1] - f.y);
       }
       tmem_st16(s_addr + 16 * q, ph);
     }
-    tmem_st32(s_addr + 32, pl);
+    tmem_st16(s_addr + 48, low);
   } else {
 #pragma unroll 1
     for (int c = 0; c < 8; ++c) {
@@ -693,7 +689,7 @@ __device__ __noinline__ RowState softmax_masked(uint32_t s_addr, const float* kf
       tmem_st4(s_addr + 4 * c, ph);  // over scores already read
     }
   }
-  return RowState{m_run, l_run * alpha + sum, alpha};
+  return sum;
 }
 
 // 16 output columns of one row.  The narrow kernel's output is bf16.
@@ -849,18 +845,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!two || s == 0) mbar_wait(JT_BAR(kBarBFull + (g & 1)), (g >> 1) & 1, abort);
             if (u == 0 && seq > 0) mbar_wait(JT_BAR(kBarOFree), (seq - 1) & 1, abort);
             const uint64_t vd = v_desc + (g & 1) * (kTile16 >> 4);
+            mbar_wait(JT_BAR(kBarPFull + s), (p_phase >> s) & 1, abort);
+            tc_fence_after();
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              mbar_wait(JT_BAR(kBarPFull + 2 * s + h), (p_phase >> s) & 1, abort);
-              tc_fence_after();
-#pragma unroll
-              for (int kk = 4 * h; kk < 4 * h + 4; ++kk) {
-                mma_ts(d_o, d_s + col_p(kk), vd + kk * (2048 / 16), kIdescPV,
-                            u > 1 || kk > 0 ? 1u : 0u);
-                if constexpr (kWide)
-                  mma_ts(d_o, d_s + col_p(kk) + 32, vd + kk * (2048 / 16), kIdescPV, 1u);
-              }
-              if (h == 0) commit(JT_BAR(kBarPvHalf + s));
+            for (int kk = 0; kk < kN / 16; ++kk) {
+              mma_ts(d_o, d_s + col_p(kk), vd + kk * (2048 / 16), kIdescPV, u > 1 || kk > 0 ? 1u : 0u);
+              if constexpr (kWide)
+                mma_ts(d_o, d_s + col_p(kk) + 32, vd + kk * (2048 / 16), kIdescPV, 1u);
             }
             p_phase ^= 1u << s;
             if (!two || s == 1) commit(JT_BAR(kBarBEmpty + (g & 1)));
@@ -1125,6 +1116,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int hl = lane & 15, hw = lane >> 4;
 #pragma unroll 1
       for (int i0 = 0; i0 < 16 * tiles; i0 += 4) {
+        if (cw * 32 + (i0 & 15) * 2 >= (nodes - (i0 >> 4) * ge.npt) * ge.groups) continue;
         uint4 w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1136,13 +1128,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 static_cast<const QT*>(p.q) + (static_cast<int64_t>(it.q_start) + first + j) * p.q_stride0 +
                 (static_cast<int64_t>(it.h) * ge.groups + (row - local * ge.groups)) * p.q_stride1 + 8 * hl));
         }
-#pragma unroll 1
+#pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int tile = (i0 + i) >> 4, row = cw * 32 + ((i0 + i) & 15) * 2 + hw;
-          const uint32_t a[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
-          w[0] = w[1];
-          w[1] = w[2];
-          w[2] = w[3];
+          const uint32_t a[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
           // The operands' own bits order like their magnitudes.
           uint32_t top = __vmaxu2(__vmaxu2(a[0] & 0x7fff7fffu, a[1] & 0x7fff7fffu),
                                   __vmaxu2(a[2] & 0x7fff7fffu, a[3] & 0x7fff7fffu));
@@ -1243,16 +1232,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------------ softmax + epilogue
-    const int s = (warp - 8) >> 2;           // stream
-    const int row = tid - 256 - s * 128;     // query-tile row, TMEM lane
+    const int wg = (warp - 8) >> 2, s = wg >> 1, half = wg & 1;  // stream, half tile of keys
+    const int row = (tid - 256) & 127;                          // query-tile row, TMEM lane
     const uint32_t lanes = static_cast<uint32_t>((row >> 5) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + col_s(s);
-    const float* kf = reinterpret_cast<const float*>(sbase + L::kKf);
+    const uint32_t s_addr = tmem + lanes + col_s(s) + 64 * half;
+    const uint32_t mx_bar = JT_BAR(kBarMx + 4 * s + (warp & 3));
+    const float* kf = reinterpret_cast<const float*>(sbase + L::kKf) + 64 * half;
     const float* qfac = reinterpret_cast<const float*>(sbase + L::kQfac);
     const volatile int* flag = reinterpret_cast<const volatile int*>(sbase + L::kFlag);
     float2* xch = reinterpret_cast<float2*>(sbase + L::kX);
+    float* mxs = reinterpret_cast<float*>(sbase + L::kMx);
     const int local = row / ge.groups, head_in = row - local * ge.groups;
-    uint32_t g0 = 0, step = 0, x_phase = 0;
+    uint32_t g0 = 0, step = 0, mx_step = 0;
+#pragma unroll 1
     for (uint32_t seq = 0;; ++seq) {
       Piece it;
       if (!next_piece(seq, it)) break;
@@ -1262,90 +1254,99 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool live = __any_sync(0xffffffffu, ok);
       const float* bias = p.qq_bias + __ldg(p.qq_bias_offsets + it.r);
       const int t_first = it.two ? 0 : s, t_step = it.two ? 1 : 2;
-      // Words of the next tile that needs a mask, built ahead of it.
-      uint4 mw = make_uint4(0u, 0u, 0u, 0u), mw_first = mw;
-      // First masked tile of this stream: tiles below floor(P / 128) need none.
+      // First masked tile of this stream (tiles below floor(P / 128) need no mask), and its
+      // words, built ahead of it.
       int t_mask = max(0, it.P / kN - it.t0);
       if (!it.two && ((t_mask ^ s) & 1)) ++t_mask;
+      uint2 mw = make_uint2(0u, 0u);
       if (live && t_mask < n)
-        mw_first = mask_words(bias, (it.t0 + t_mask) * kN, it.P, it.T, it.key_end, j, ok);
+        mw = mask_words(bias, (it.t0 + t_mask) * kN + 64 * half, it.P, it.T, it.key_end, j, ok);
       float m_run = -INFINITY, l_run = 0.f, c_row = 0.f;
+#pragma unroll 1
       for (int t = t_first; t < n; t += t_step) {
         const uint32_t g = g0 + t;
         if (t == t_first) {
           warp_wait(JT_BAR(kBarQFull + (seq & 1)), (seq >> 1) & 1, abort);
-          c_row = qfac[((seq & 1) * 2 + (it.two ? s : 0)) * kM + row];
+          c_row = ok ? qfac[((seq & 1) * 2 + (it.two ? s : 0)) * kM + row] : 0.f;
         }
         warp_wait(JT_BAR(kBarFac + (g & 1)), (g >> 1) & 1, abort);
         warp_wait(JT_BAR(kBarSFull + s), step & 1, abort);
         ++step;
         tc_fence_after();
-        const bool masked = t >= t_mask;
-        const bool careful =
-            masked || (flag[(g & 1) * 4] | flag[(g & 1) * 4 + 1] | flag[(g & 1) * 4 + 2] |
-                       flag[(g & 1) * 4 + 3]) != 0;
-        if (!masked) mw = make_uint4(~0u, ~0u, ~0u, ~0u);
-        else if (t == t_mask) mw = mw_first;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          if (live) {
-            const float* f = kf + (g & 1) * kN + 64 * h;
-            const RowState st =
-                careful ? softmax_masked<kWide>(s_addr + 64 * h, f, c_row, h ? mw.z : mw.x,
-                                                h ? mw.w : mw.y, m_run, l_run)
-                        : softmax_half<kWide>(s_addr + 64 * h, f, c_row, m_run, l_run);
-            m_run = st.m;
-            l_run = st.l;
-            // O can be rescaled once the stream's last PV has completed: for a tile's first
-            // half the scores themselves were issued behind it, for the second half it is
-            // the first half's.
-            if ((t != t_first || h) && __any_sync(0xffffffffu, st.alpha != 1.f)) {
-              if (h) warp_wait(JT_BAR(kBarPvHalf + s), (step - 1) & 1, abort);
-              tc_fence_after();
-#pragma unroll 1
-              for (int c = 0; c < 4; ++c) {
-                uint32_t o[32];
-                tmem_ld32(tmem + lanes + col_o(s) + 32 * c, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * st.alpha);
-                tmem_st32(tmem + lanes + col_o(s) + 32 * c, o);
-              }
-            }
-            tmem_wait_st();
+        if (live) {
+          const float* f = kf + (g & 1) * kN;
+          const bool masked = t >= t_mask;
+          const bool careful =
+              masked || (flag[(g & 1) * 4] | flag[(g & 1) * 4 + 1] | flag[(g & 1) * 4 + 2] |
+                         flag[(g & 1) * 4 + 3]) != 0;
+          const uint2 w = masked ? mw : make_uint2(~0u, ~0u);
+          const float mine = careful ? half_max_masked(s_addr, f, w.x, w.y) : half_max(s_addr, f);
+          // The two warps that share these rows meet, so that both halves use one maximum.
+          float* slot = mxs + (mx_step & 1) * 4 * kM + s * 2 * kM + row;
+          slot[half * kM] = mine;
+          warp_arrive(mx_bar);
+          warp_wait(mx_bar, mx_step & 1, abort);
+          ++mx_step;
+          // Lazy running maximum: it moves only when a tile exceeds it by 2^8, so P stays
+          // below 2^8 and O is rarely rescaled.
+          const float mx = fmaxf(mine, slot[(half ^ 1) * kM]) * c_row;
+          float alpha = 1.f;
+          if (mx > m_run + 8.f) {
+            if (m_run != -INFINITY) alpha = jt::fast_exp2(m_run - mx);
+            m_run = mx;
           }
-          // A warp without a live row arrives too; its rows of P are never read out.
-          tc_fence_before();
-          warp_arrive(JT_BAR(kBarPFull + 2 * s + h));
+          const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+          const float sum = careful ? half_exp_masked<kWide>(s_addr, f, c_row, neg_m, w.x, w.y)
+                                    : half_exp<kWide>(s_addr, f, c_row, neg_m);
+          l_run = l_run * alpha + sum;
+          // This tile's scores were issued behind the stream's last PV, which has therefore
+          // completed: O (this half of its columns) can be rescaled at once.
+          if (t != t_first && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[16];
+              tmem_ld16(tmem + lanes + col_o(s) + 64 * half + 16 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+              tmem_st16(tmem + lanes + col_o(s) + 64 * half + 16 * c, o);
+            }
+          }
+          tmem_wait_st();
         }
-        // The masks of the next masked tile, behind this tile's product.
-        if (live && masked && t + t_step < n)
-          mw = mask_words(bias, (it.t0 + t + t_step) * kN, it.P, it.T, it.key_end, j, ok);
+        // A warp without a live row arrives too; its rows of P are never read out.
+        tc_fence_before();
+        warp_arrive(JT_BAR(kBarPFull + s));
+        // The words of the next masked tile, behind this tile's product.
+        if (live && t >= t_mask && t + t_step < n)
+          mw = mask_words(bias, (it.t0 + t + t_step) * kN + 64 * half, it.P, it.T, it.key_end, j, ok);
       }
-      // Epilogue, once the piece's last PV has completed.
+      // Epilogue, once the piece's last PV has completed: the halves' sums meet, with one query
+      // tile also the streams' (max, sum).  With one tile each warpgroup merges and writes 32
+      // of the columns, with two 64 of its stream's.
       warp_wait(JT_BAR(kBarODone), seq & 1, abort);
       tc_fence_after();
-      // One query tile: the streams' rows meet, and each warpgroup merges and writes 64 of the
-      // columns.  Two: each warpgroup writes all columns of its own tile.
-      const bool pair = !it.two;
-      float fa = 1.f, fb = 0.f, m = m_run, l = l_run;
-      if (pair) {
-        xch[s * kM + row] = make_float2(m_run, l_run);
-        warp_arrive(JT_BAR(kBarX));
-        warp_wait(JT_BAR(kBarX), x_phase, abort);
-        x_phase ^= 1u;
-        const float2 a = xch[row], b = n > 1 ? xch[kM + row] : make_float2(-INFINITY, 0.f);
-        m = fmaxf(a.x, b.x);
-        fa = a.x == -INFINITY ? 0.f : jt::fast_exp2(a.x - m);
-        fb = b.x == -INFINITY ? 0.f : jt::fast_exp2(b.x - m);
-        // A stream without a maximum has a zero sum, or a NaN that has to stay.
-        l = a.y * (a.x == -INFINITY ? 1.f : fa) + b.y * (b.x == -INFINITY ? 1.f : fb);
-      }
+      xch[wg * kM + row] = make_float2(m_run, l_run);
+      warp_arrive(JT_BAR(kBarX));
+      warp_wait(JT_BAR(kBarX), seq & 1, abort);
       if (live) {
+        const bool pair = !it.two;
+        const float2 a0 = xch[(pair ? 0 : 2 * s) * kM + row], a1 = xch[(pair ? 1 : 2 * s + 1) * kM + row];
+        float fa = 1.f, fb = 0.f, m = a0.x, l = a0.y + a1.y;
+        if (pair && n > 1) {
+          const float2 b0 = xch[2 * kM + row], b1 = xch[3 * kM + row];
+          const float lb = b0.y + b1.y;
+          m = fmaxf(a0.x, b0.x);
+          fa = a0.x == -INFINITY ? 0.f : jt::fast_exp2(a0.x - m);
+          fb = b0.x == -INFINITY ? 0.f : jt::fast_exp2(b0.x - m);
+          // A stream without a maximum has a zero sum, or a NaN that has to stay.
+          l = l * (a0.x == -INFINITY ? 1.f : fa) + lb * (b0.x == -INFINITY ? 1.f : fb);
+        }
         const Workspace w = carve(p.workspace);
         const int tile = pair ? 0 : s;
         if (it.slot >= 0) {
-          if (ok && (!pair || s == 0)) w.ml[(it.slot * 2ll + tile) * kM + row] = make_float2(m, l);
+          if (ok && (pair ? wg == 0 : half == 0))
+            w.ml[(it.slot * 2ll + tile) * kM + row] = make_float2(m, l);
         } else {
           const float inv = l == 0.f ? 0.f : 1.f / l;
           fa *= inv;
@@ -1353,9 +1354,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int64_t out_row = (static_cast<int64_t>(it.q_start) + j) * p.out_stride0 +
                                 (static_cast<int64_t>(it.h) * ge.groups + head_in) * p.out_stride1;
-        const int c_end = pair ? 4 * s + 4 : 8;
+        const int c0 = pair ? 2 * wg : 4 * half, c1 = c0 + (pair ? 2 : 4);
 #pragma unroll 1
-        for (int c = pair ? 4 * s : 0; c < c_end; ++c) {  // 16 columns
+        for (int c = c0; c < c1; ++c) {  // 16 columns
           uint32_t o0[16], o1[16];
           __syncwarp();
           tmem_ld16(tmem + lanes + col_o(tile) + 16 * c, o0);
