@@ -31,7 +31,7 @@
 //   warp 0       MMA issuer, TMEM owner (S0, S1, O0, O1: 128 columns each)
 //   warp 1       work pieces; TMA loads of K, V and scale bytes for prefix tiles
 //   warps 2-3    cp.async gathers of tiles that touch tree nodes or pages TMA cannot box
-//   warps 4-7    queries -> e4m3 terms; scale bytes -> key factors; V codes -> bf16 tile
+//   warps 4-7    scale bytes -> key factors; V codes -> bf16 tile
 //   warps 8-23   softmax + epilogue: two warpgroups per stream, each with 64 of a tile's keys
 //                and one thread per row
 //
@@ -79,8 +79,7 @@ struct Smem {
   static constexpr int kV16 = kV8 + kVRing * kTile8;
   static constexpr int kScale = kV16 + 2 * kTile16;          // [kScaleRing][K, V][128] bytes
   static constexpr int kKf = kScale + kScaleRing * 256;       // [2][128] float
-  static constexpr int kQfac = kKf + 2 * kN * 4;              // [2][2][128] float
-  static constexpr int kX = kQfac + 4 * kM * 4;               // [stream][half][128] float2: max, sum
+  static constexpr int kX = kKf + 2 * kN * 4;                 // [stream][half][128] float2: max, sum
   static constexpr int kMx = kX + 4 * kM * 8;                 // [2][stream][half][128] float
   static constexpr int kItem = kMx + 8 * kM * 4;              // [2][16] int
   static constexpr int kFlag = kItem + 2 * 64;                // [2][4] int
@@ -98,7 +97,7 @@ constexpr int kBarVEmpty = 8;    // [2] 4 converter warps
 constexpr int kBarFac = 10;      // [2] 4 converter warps: the tile's factors are written
 constexpr int kBarBFull = 12;    // [2] 4 converter warps: the tile's bf16 V is written
 constexpr int kBarBEmpty = 14;   // [2] commit after the tile's last PV
-constexpr int kBarQFull = 16;    // [2] 4 converter warps, by piece parity
+constexpr int kBarQFull = 16;    // TMA (arrive_tx + arrive); 17 is unused
 constexpr int kBarQEmpty = 18;   // commit after a piece's last QK
 constexpr int kBarSFull = 19;    // [2] commit per QK, by stream
 constexpr int kBarPFull = 21;    // [2] 8 softmax warps, by stream
@@ -119,7 +118,7 @@ __device__ __forceinline__ uint32_t bar_count(int i) {
   if (i < kBarVEmpty) return 2;
   if (i < kBarBEmpty) return 4;  // VEmpty, Fac, BFull
   if (i < kBarQFull) return 1;
-  if (i < kBarQEmpty) return 4;
+  if (i < kBarQEmpty) return 2;
   if (i < kBarPFull) return 1;   // QEmpty, SFull
   if (i < kBarODone) return 8;
   if (i == kBarODone) return 1;
@@ -322,6 +321,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1,
+                                            int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
                                           uint32_t bar) {
   asm volatile(
@@ -458,15 +465,23 @@ struct Workspace {
   PieceMeta* meta;   // [2 * kMaxCtas]
   float2* ml;        // [slot][tile][128] max (log2 units), sum
   float4* o;         // [slot][tile][32 groups of 4 columns][128]
+  float* q_factor;   // [kv head][packed query row] scale * log2(e) * 2^e
+  uint8_t* q_terms;  // [kv head][term][packed query row][128] e4m3
 };
 constexpr int64_t kMetaBytes = 2 * kMaxCtas * sizeof(PieceMeta);
 constexpr int64_t kMlBytes = 2ll * kMaxCtas * 2 * kM * sizeof(float2);
 constexpr int64_t kPartBytes = 2ll * kMaxCtas * 2 * kM * kD * sizeof(float);
 static_assert(kMetaBytes % 256 == 0 && kMlBytes % 256 == 0, "workspace alignment");
-__host__ __device__ __forceinline__ Workspace carve(void* base) {
+// Query terms of one KV head and term: a packed row is (node, query head of the group).
+__host__ __device__ __forceinline__ int64_t factor_bytes(int64_t rows, int heads) {
+  return (rows * heads * 4 + 255) / 256 * 256;
+}
+__host__ __device__ __forceinline__ Workspace carve(void* base, int64_t rows = 0, int heads = 0) {
   char* b = static_cast<char*>(base);
+  char* q = b + kMetaBytes + kMlBytes + kPartBytes;
   return Workspace{reinterpret_cast<PieceMeta*>(b), reinterpret_cast<float2*>(b + kMetaBytes),
-                   reinterpret_cast<float4*>(b + kMetaBytes + kMlBytes)};
+                   reinterpret_cast<float4*>(b + kMetaBytes + kMlBytes), reinterpret_cast<float*>(q),
+                   reinterpret_cast<uint8_t*>(q + factor_bytes(rows, heads))};
 }
 
 // Page and offset of key position `pos` of a piece, page -1 past its keys or out of the pool.
@@ -719,11 +734,72 @@ __device__ __forceinline__ void store_columns(const JtTreeAttnFp8Params& p, int6
   }
 }
 
+// Queries as e4m3 terms of row / 2^e and the rows' factors, for the attention kernel's TMA: half
+// a warp per row (16 bytes per lane), its largest magnitude by shuffles.  A kernel of its own
+// (the attention starts beside it as a programmatic dependent): inside, the split of a
+// piece's 256 rows by one warpgroup took 25 thousand cycles, a third of a short piece.
 template <bool kWide, typename QT>
+__global__ void __launch_bounds__(256) tree_attn_fp8_split_kernel(
+    const __grid_constant__ JtTreeAttnFp8Params p) {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  constexpr int kTerms = Smem<kWide>::kTerms;
+  const int64_t rows = static_cast<int64_t>(p.total_queries) * p.groups;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const int hl = threadIdx.x & 15;
+  const bool ok = id < rows * p.num_kv_heads;
+  const int64_t node = (ok ? id : 0) / (p.num_kv_heads * p.groups);
+  const int hq = static_cast<int>((ok ? id : 0) - node * (p.num_kv_heads * p.groups));
+  const int h = hq / p.groups;
+  const int64_t row = node * p.groups + (hq - h * p.groups);
+  uint4 w = make_uint4(0u, 0u, 0u, 0u);
+  if (ok && 8 * hl < p.head_dim)
+    w = __ldg(reinterpret_cast<const uint4*>(static_cast<const QT*>(p.q) + node * p.q_stride0 +
+                                             hq * p.q_stride1 + 8 * hl));
+  const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+  // The operands' own bits order like their magnitudes.
+  uint32_t top = __vmaxu2(__vmaxu2(a[0] & 0x7fff7fffu, a[1] & 0x7fff7fffu),
+                          __vmaxu2(a[2] & 0x7fff7fffu, a[3] & 0x7fff7fffu));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (!ok) return;
+  top = __float_as_uint(jt::MmaOp<QT>::unpack(max(top & 0xffffu, top >> 16)).x);
+  const bool finite = top < 0x7f800000u;
+  int e = 0;
+  if (top != 0 && finite)
+    e = max(static_cast<int>(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u), -126);
+  const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  float2 x[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    x[k] = jt::MmaOp<QT>::unpack(a[k]);
+    x[k] = make_float2(x[k].x * inv, x[k].y * inv);
+  }
+  const Workspace ws = carve(p.workspace, rows, p.num_kv_heads);
+  uint8_t* dst = ws.q_terms + (static_cast<int64_t>(h) * kTerms * rows + row) * kD + 8 * hl;
+#pragma unroll
+  for (int m = 0; m < kTerms; ++m) {
+    uint32_t t[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      t[k] = pack_e4m3(x[k].x, x[k].y);
+      const float2 y = unpack_e4m3(t[k]);
+      x[k] = make_float2(x[k].x - y.x, x[k].y - y.y);
+    }
+    *reinterpret_cast<uint2*>(dst + m * rows * kD) = make_uint2(t[0] | (t[1] << 16), t[2] | (t[3] << 16));
+  }
+  // A row with a non-finite element: its factor makes its scores NaN.
+  if (hl == 0)
+    ws.q_factor[h * rows + row] =
+        finite ? p.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23)
+               : __uint_as_float(0x7fc00000u);
+}
+
+template <bool kWide>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_attn_fp8_kernel(const __grid_constant__ JtTreeAttnFp8Params p,
                          const __grid_constant__ CUtensorMap kmap,
-                         const __grid_constant__ CUtensorMap vmap, const LoadPlan plan) {
+                         const __grid_constant__ CUtensorMap vmap,
+                         const __grid_constant__ CUtensorMap qmap, const LoadPlan plan) {
   using L = Smem<kWide>;
   constexpr int kTerms = L::kTerms;
   extern __shared__ unsigned char smem_raw[];
@@ -800,6 +876,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int r_start = has_part ? static_cast<int>(scan[32]) : R;
   const int64_t s_start = has_part ? scan[33] : 0;
   __syncthreads();  // the scan area is free
+  // From here on the query terms are complete, and so is every earlier use of the workspace.
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
 
   // Pieces: a two-entry ring in shared memory, filled one piece ahead by warp 1's first lane.
   volatile int* item_ring = reinterpret_cast<volatile int*>(sbase + L::kItem);
@@ -832,7 +910,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         Piece it;
         if (!next_piece(seq, it)) break;
         const int n = it.n, two = it.two;
-        mbar_wait(JT_BAR(kBarQFull + (seq & 1)), (seq >> 1) & 1, abort);
+        mbar_wait(JT_BAR(kBarQFull), seq & 1, abort);
         tc_fence_after();
         // Step u is stream u & 1's product with key tile u (one query tile) or u >> 1 (two).
         const int steps = n << two;
@@ -954,7 +1032,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_arrive(JT_BAR(kBarItemFull + slot));
       };
-      uint32_t g0 = 0;
+      uint32_t g0 = 0, q_fills = 0;
       // Full barriers whose last fill is TMA's, as bits (K 0.., V 4.., scales 8..), and the
       // phase parity of that fill: what the drain waits for.
       uint32_t mine = 0, parity = 0;
@@ -1020,6 +1098,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int i = 0; i <= 2 * n; ++i) {
             if (i == max(0, 2 * n - 6)) publish(seq + 1);
+            if (i == 2) {
+              // The query tiles, once the previous piece's last QK has read them.  Rows past
+              // the item's are other nodes' (or zeros): their scores are never used.
+              if (seq > 0) mbar_wait(JT_BAR(kBarQEmpty), (seq - 1) & 1, abort);
+              const int tiles = 1 + it.two;
+              mbar_arrive_tx(JT_BAR(kBarQFull), tiles * kTerms * kTile8);
+              const int row = (it.q_start + it.mb * ge.npi) * ge.groups;
+#pragma unroll 1
+              for (int k = 0; k < tiles * kTerms; ++k)
+                tma_load_3d(base + L::kQ + k * kTile8, &qmap, 0,
+                            row + (k >= kTerms ? ge.npt * ge.groups : 0),
+                            it.h * kTerms + (k >= kTerms ? k - kTerms : k), JT_BAR(kBarQFull));
+              mbar_arrive(JT_BAR(kBarQFull));
+              q_fills = seq + 1;
+            }
             const bool is_v = i >= 2 && !(i & 1);
             const int t = i < 2 ? i : is_v ? (i >> 1) - 1 : (i >> 1) + 1;
             if (t < n) load(is_v, t);
@@ -1036,6 +1129,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int bar = i < 4 ? kBarKFull + i : i < 8 ? kBarVFull + i - 4 : kBarScale + i - 8;
             mbar_wait(JT_BAR(bar), (parity >> i) & 1u, abort, false);
           }
+        if (q_fills > 0) mbar_wait(JT_BAR(kBarQFull), (q_fills - 1) & 1, abort, false);
         PieceMeta* m = carve(p.workspace).meta + 2 * blockIdx.x;
         m[0].valid = meta_valid[0];
         m[1].valid = meta_valid[1];
@@ -1097,7 +1191,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int ct = tid - 128, cw = warp - 4;  // this thread's key; this warp's 32 rows
     uint32_t g0 = 0;
     float* kf = reinterpret_cast<float*>(sbase + L::kKf);
-    float* qfac = reinterpret_cast<float*>(sbase + L::kQfac);
     volatile int* flag = reinterpret_cast<volatile int*>(sbase + L::kFlag);
     // V: eight lanes of a warp take four 16-byte chunks of rows r and r ^ 5, so that both the
     // swizzled loads and the swizzled stores of the eight touch different banks.
@@ -1107,71 +1200,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t seq = 0;; ++seq) {
       Piece it;
       if (!next_piece(seq, it)) break;
-      if (seq > 0) warp_wait(JT_BAR(kBarQEmpty), (seq - 1) & 1, abort);
-      // Queries: half a warp per row (16 bytes per lane), its largest magnitude by shuffles,
-      // then e4m3 terms of row / 2^e.  Rows without a query keep whatever is there: their
-      // scores are never used.  Four rows' loads are in flight.
-      const int first = it.mb * ge.npi, nodes = min(it.T, first + ge.npi) - first;
-      const int tiles = it.two ? 2 : 1;
-      const int hl = lane & 15, hw = lane >> 4;
-#pragma unroll 1
-      for (int i0 = 0; i0 < 16 * tiles; i0 += 4) {
-        if (cw * 32 + (i0 & 15) * 2 >= (nodes - (i0 >> 4) * ge.npt) * ge.groups) continue;
-        uint4 w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tile = (i0 + i) >> 4, row = cw * 32 + ((i0 + i) & 15) * 2 + hw;
-          const int local = row / ge.groups, j = tile * ge.npt + local;
-          w[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (local < ge.npt && j < nodes && 8 * hl < p.head_dim)
-            w[i] = __ldg(reinterpret_cast<const uint4*>(
-                static_cast<const QT*>(p.q) + (static_cast<int64_t>(it.q_start) + first + j) * p.q_stride0 +
-                (static_cast<int64_t>(it.h) * ge.groups + (row - local * ge.groups)) * p.q_stride1 + 8 * hl));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tile = (i0 + i) >> 4, row = cw * 32 + ((i0 + i) & 15) * 2 + hw;
-          const uint32_t a[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-          // The operands' own bits order like their magnitudes.
-          uint32_t top = __vmaxu2(__vmaxu2(a[0] & 0x7fff7fffu, a[1] & 0x7fff7fffu),
-                                  __vmaxu2(a[2] & 0x7fff7fffu, a[3] & 0x7fff7fffu));
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-          top = __float_as_uint(jt::MmaOp<QT>::unpack(max(top & 0xffffu, top >> 16)).x);
-          const bool finite = top < 0x7f800000u;
-          int e = 0;
-          if (top != 0 && finite)
-            e = max(static_cast<int>(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u), -126);
-          const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-          float2 x[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[k] = jt::MmaOp<QT>::unpack(a[k]);
-            x[k] = make_float2(x[k].x * inv, x[k].y * inv);
-          }
-          unsigned char* dst = sbase + L::kQ + tile * kTerms * kTile8 + row * 128 +
-                               (((hl >> 1) ^ (row & 7)) << 4) + (hl & 1) * 8;
-#pragma unroll
-          for (int m = 0; m < kTerms; ++m) {
-            uint32_t t[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              t[k] = pack_e4m3(x[k].x, x[k].y);
-              const float2 y = unpack_e4m3(t[k]);
-              x[k] = make_float2(x[k].x - y.x, x[k].y - y.y);
-            }
-            *reinterpret_cast<uint2*>(dst + m * kTile8) =
-                make_uint2(t[0] | (t[1] << 16), t[2] | (t[3] << 16));
-          }
-          // A row with a non-finite element: its factor makes its scores NaN.
-          if (hl == 0)
-            qfac[((seq & 1) * 2 + tile) * kM + row] =
-                finite ? p.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23)
-                       : __uint_as_float(0x7fc00000u);
-        }
-      }
-      fence_proxy_async();
-      warp_arrive(JT_BAR(kBarQFull + (seq & 1)));
 #pragma unroll 1
       for (int t = 0; t < it.n; ++t) {
         const uint32_t g = g0 + t, buf = g & 1;
@@ -1238,7 +1266,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = tmem + lanes + col_s(s) + 64 * half;
     const uint32_t mx_bar = JT_BAR(kBarMx + 4 * s + (warp & 3));
     const float* kf = reinterpret_cast<const float*>(sbase + L::kKf) + 64 * half;
-    const float* qfac = reinterpret_cast<const float*>(sbase + L::kQfac);
+    const float* q_factor = carve(p.workspace, static_cast<int64_t>(p.total_queries) * ge.groups,
+                                  p.num_kv_heads).q_factor;
     const volatile int* flag = reinterpret_cast<const volatile int*>(sbase + L::kFlag);
     float2* xch = reinterpret_cast<float2*>(sbase + L::kX);
     float* mxs = reinterpret_cast<float*>(sbase + L::kMx);
@@ -1261,14 +1290,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint2 mw = make_uint2(0u, 0u);
       if (live && t_mask < n)
         mw = mask_words(bias, (it.t0 + t_mask) * kN + 64 * half, it.P, it.T, it.key_end, j, ok);
-      float m_run = -INFINITY, l_run = 0.f, c_row = 0.f;
+      float m_run = -INFINITY, l_run = 0.f;
+      const float c_row =
+          ok ? __ldg(q_factor + (static_cast<int64_t>(it.h) * p.total_queries + it.q_start + j) * ge.groups + head_in)
+             : 0.f;
 #pragma unroll 1
       for (int t = t_first; t < n; t += t_step) {
         const uint32_t g = g0 + t;
-        if (t == t_first) {
-          warp_wait(JT_BAR(kBarQFull + (seq & 1)), (seq >> 1) & 1, abort);
-          c_row = ok ? qfac[((seq & 1) * 2 + (it.two ? s : 0)) * kM + row] : 0.f;
-        }
         warp_wait(JT_BAR(kBarFac + (g & 1)), (g >> 1) & 1, abort);
         warp_wait(JT_BAR(kBarSFull + s), step & 1, abort);
         ++step;
@@ -1448,6 +1476,10 @@ __global__ void __launch_bounds__(kM) tree_attn_fp8_merge_kernel(
   store_columns<kWide>(p, at, f);
 }
 
+int64_t workspace_bytes(int64_t rows, int heads) {  // for either kernel's number of terms
+  return kMetaBytes + kMlBytes + kPartBytes + factor_bytes(rows, heads) + rows * heads * 3 * kD;
+}
+
 bool al16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
@@ -1483,6 +1515,37 @@ bool encode_pool(CUtensorMap* map, const JtTreeAttnFp8Params& p, const void* poo
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// [kv heads x terms][packed query rows][128] e4m3, a box of 128 rows.
+bool encode_queries(CUtensorMap* map, const void* terms, int64_t rows, int planes) {
+  auto encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[3] = {kD, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+  const cuuint64_t strides[2] = {kD, static_cast<cuuint64_t>(rows) * kD};
+  const cuuint32_t box[3] = {kD, kM, 1};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(terms), dims, strides, box,
+                elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Programmatic dependent launch: the grid may start beside its predecessor and waits for it
+// (griddepcontrol.wait) before it touches what that one writes.
+template <typename... Params, typename... Args>
+int launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
+                     cudaStream_t stream, const char* what, const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return jt_cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
+
 template <bool kWide, typename QT>
 int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
   LoadPlan plan{};
@@ -1497,26 +1560,28 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
       (!encode_pool(&kmap, p, p.k_pool, p.k_stride0, p.k_stride1, p.k_stride2, plan.box) ||
        !encode_pool(&vmap, p, p.v_pool, p.v_stride0, p.v_stride1, p.v_stride2, plan.box)))
     plan.tma = 0;  // a layout the encoder refuses: gathered like any other page size
-  auto kernel = tree_attn_fp8_kernel<kWide, QT>;
-  int rc = jt_cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  const int64_t rows = static_cast<int64_t>(p.total_queries) * p.groups;
+  CUtensorMap qmap{};
+  if (!encode_queries(&qmap, carve(p.workspace, rows, p.num_kv_heads).q_terms, rows,
+                      p.num_kv_heads * Smem<kWide>::kTerms))
+    return jt_fail(JT_ERR_CUDA, "tree_attn_fp8: cuTensorMapEncodeTiled rejected the query terms");
+  int rc = jt_cuda_check(cudaFuncSetAttribute(tree_attn_fp8_kernel<kWide>,
+                                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                                               Smem<kWide>::kBytes),
                          "tree_attn_fp8 smem attribute");
   if (rc != JT_OK) return rc;
-  const int grid = std::min(sms, kMaxCtas);
-  kernel<<<grid, kThreads, Smem<kWide>::kBytes, stream>>>(p, kmap, vmap, plan);
-  rc = jt_cuda_check(cudaGetLastError(), "tree_attn_fp8 launch");
+  const int64_t split = (rows * p.num_kv_heads + 15) / 16;
+  if (split > 0x7fffffff || rows > 0x7fffffff)
+    return jt_fail(JT_ERR_INVALID, "tree_attn_fp8: too many query rows");
+  tree_attn_fp8_split_kernel<kWide, QT><<<static_cast<unsigned>(split), 256, 0, stream>>>(p);
+  rc = jt_cuda_check(cudaGetLastError(), "tree_attn_fp8 query split launch");
   if (rc != JT_OK) return rc;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, 8 * Smem<kWide>::kTiles);
-  cfg.blockDim = dim3(kM);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return jt_cuda_check(cudaLaunchKernelEx(&cfg, tree_attn_fp8_merge_kernel<kWide>, p, grid),
-                       "tree_attn_fp8 merge launch");
+  const int grid = std::min(sms, kMaxCtas);
+  rc = launch_dependent(tree_attn_fp8_kernel<kWide>, dim3(grid), kThreads, Smem<kWide>::kBytes, stream,
+                        "tree_attn_fp8 launch", p, kmap, vmap, qmap, plan);
+  if (rc != JT_OK) return rc;
+  return launch_dependent(tree_attn_fp8_merge_kernel<kWide>, dim3(grid, 8 * Smem<kWide>::kTiles), kM,
+                          0, stream, "tree_attn_fp8 merge launch", p, grid);
 }
 
 }  // namespace
@@ -1535,7 +1600,7 @@ extern "C" int64_t jt_tree_attn_fp8_workspace_size(int32_t num_requests, int32_t
                                                    int32_t head_dim) {
   if (num_requests < 1 || total_queries < 1 || num_kv_heads < 1 || groups < 1 || head_dim < 1)
     return -1;
-  return kMetaBytes + kMlBytes + kPartBytes;
+  return workspace_bytes(static_cast<int64_t>(total_queries) * groups, num_kv_heads);
 }
 
 extern "C" int jt_tree_attn_fp8_launch(const JtTreeAttnFp8Params* p, cudaStream_t stream) {
@@ -1562,7 +1627,7 @@ extern "C" int jt_tree_attn_fp8_launch(const JtTreeAttnFp8Params* p, cudaStream_
       (p->k_stride0 | p->k_stride1 | p->k_stride2 | p->v_stride0 | p->v_stride1 | p->v_stride2) % 16 != 0)
     return jt_fail(JT_ERR_INVALID,
                    "tree_attn_fp8: queries, output and pool rows must start on 16 bytes");
-  const int64_t need = kMetaBytes + kMlBytes + kPartBytes;
+  const int64_t need = workspace_bytes(static_cast<int64_t>(p->total_queries) * p->groups, p->num_kv_heads);
   if (p->workspace == nullptr || p->workspace_bytes < need ||
       (reinterpret_cast<uintptr_t>(p->workspace) & 255u) != 0)
     return jt_fail(JT_ERR_WORKSPACE, "tree_attn_fp8: workspace of %lld bytes required (got %lld)",
