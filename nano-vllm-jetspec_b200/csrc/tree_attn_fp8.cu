@@ -28,9 +28,9 @@
 // tile; with one, the streams take alternate key tiles of the same rows and their (max, sum,
 // O) are merged at the end.
 //
-//   warp 0       MMA issuer, TMEM owner (S0, S1, O0, O1: 128 columns each)
+//   warps 0, 2   MMA issuers, one per stream; TMEM (S0, S1, O0, O1: 128 columns each)
 //   warp 1       work pieces; TMA loads of K, V and scale bytes for prefix tiles
-//   warps 2-3    cp.async gathers of tiles that touch tree nodes or pages TMA cannot box
+//   warp 3       cp.async gathers of tiles that touch tree nodes or pages TMA cannot box
 //   warps 4-7    scale bytes -> key factors; V codes -> bf16 tile
 //   warps 8-23   softmax + epilogue: two warpgroups per stream, each with 64 of a tile's keys
 //                and one thread per row
@@ -49,6 +49,7 @@ namespace {
 __device__ uint32_t g_attn_fp8_errors;
 
 constexpr int kN = 128;               // keys per tile
+constexpr int kHalf = 64;             // keys per score buffer (a granule)
 constexpr int kM = 128;               // rows per query tile
 constexpr int kD = 128;               // head dim in shared memory (shorter heads: zeros)
 constexpr int kThreads = 768;
@@ -61,6 +62,7 @@ constexpr int kTile16 = 2 * kTile8;   // bytes of a bf16 tile: two 64-dim halves
 constexpr int kHalf16 = kTile8;
 constexpr int kMaxCtas = 160;         // workspace slots are sized for this many SMs
 constexpr int kMaxNodes = 1024;
+constexpr int kMaskWords = kMaxNodes / 32;
 // Costs in units of one 128-row, 128-key tile: an item's fixed cost (query load, pipeline
 // fill, epilogue), and the least part worth a CTA of its own.
 constexpr int kItemCost = 3;
@@ -80,8 +82,8 @@ struct Smem {
   static constexpr int kScale = kV16 + 2 * kTile16;          // [kScaleRing][K, V][128] bytes
   static constexpr int kKf = kScale + kScaleRing * 256;       // [2][128] float
   static constexpr int kX = kKf + 2 * kN * 4;                 // [stream][half][128] float2: max, sum
-  static constexpr int kMx = kX + 4 * kM * 8;                 // [2][stream][half][128] float
-  static constexpr int kItem = kMx + 8 * kM * 4;              // [2][16] int
+  static constexpr int kMx = kX + 4 * kM * 8;                 // [stream][128] float: maxima
+  static constexpr int kItem = kMx + 2 * kM * 4;              // [2][16] int
   static constexpr int kFlag = kItem + 2 * 64;                // [2][4] int
   static constexpr int kMisc = kFlag + 32;                    // TMEM base, abort, free slots
   static constexpr int kBar = kMisc + 32;
@@ -90,46 +92,44 @@ struct Smem {
 };
 
 // ---- barriers -------------------------------------------------------------------------
-constexpr int kBarKFull = 0;     // [3] TMA (arrive_tx + arrive) or two gather warps
-constexpr int kBarKEmpty = 3;    // [3] commit after the tile's last QK
-constexpr int kBarVFull = 6;     // [2] TMA or two gather warps
+constexpr int kBarKFull = 0;     // [3] TMA (arrive_tx) or the gather warp
+constexpr int kBarKEmpty = 3;    // [3] commit after each stream's last QK of the tile
+constexpr int kBarVFull = 6;     // [2] TMA or the gather warp
 constexpr int kBarVEmpty = 8;    // [2] 4 converter warps
 constexpr int kBarFac = 10;      // [2] 4 converter warps: the tile's factors are written
 constexpr int kBarBFull = 12;    // [2] 4 converter warps: the tile's bf16 V is written
-constexpr int kBarBEmpty = 14;   // [2] commit after the tile's last PV
-constexpr int kBarQFull = 16;    // TMA (arrive_tx + arrive); 17 is unused
-constexpr int kBarQEmpty = 18;   // commit after a piece's last QK
-constexpr int kBarSFull = 19;    // [2] commit per QK, by stream
-constexpr int kBarPFull = 21;    // [2] 8 softmax warps, by stream
-constexpr int kBarODone = 23;    // commit after a piece's last PV
-constexpr int kBarOFree = 24;    // 16 softmax warps: the epilogue has read O
-constexpr int kBarX = 25;        // 16 softmax warps: (max, sum) exchanged
-constexpr int kBarItemFull = 26;   // [2] publisher
-constexpr int kBarItemEmpty = 28;  // [2] every warp
-constexpr int kBarDrain = 30;
-constexpr int kBarScale = 31;      // [8] as KFull, for the tile's scale bytes
-constexpr int kBarMx = 39;         // [stream][32 rows] the two warps that share rows: half maxima
-constexpr int kNumBars = 47;
+constexpr int kBarBEmpty = 14;   // [2] commit after each stream's last PV of the tile
+constexpr int kBarQEmpty = 16;   // commit after each stream's last QK of a piece
+constexpr int kBarODone = 17;    // commit after each stream's last PV of a piece
+constexpr int kBarQFull = 18;    // TMA
+constexpr int kBarSFull = 19;    // [2 streams][2 buffers] commit per QK
+constexpr int kBarPFull = 23;    // [2 streams][2 buffers] 4 softmax warps
+constexpr int kBarPv = 27;       // [2] commit per PV, by stream
+constexpr int kBarOFree = 29;    // 16 softmax warps: the epilogue has read O
+constexpr int kBarX = 30;        // 16 softmax warps: (max, sum) exchanged
+constexpr int kBarItemEmpty = 31;  // [2] every warp
+constexpr int kBarItemFull = 33;   // [2] publisher
+constexpr int kBarDrain = 35;      // [2] commit after a stream's last MMA
+constexpr int kBarMx = 37;         // [stream][buffer][32 rows] the warp has set the rows' maxima
+constexpr int kBarScale = 53;      // [8] as KFull, for the tile's scale bytes
+constexpr int kNumBars = 61;
 static_assert(kNumBars <= 64, "barrier area");
 
 __device__ __forceinline__ uint32_t bar_count(int i) {
-  if (i < kBarKEmpty) return 2;
-  if (i < kBarVFull) return 1;
-  if (i < kBarVEmpty) return 2;
+  if (i < kBarKEmpty) return 1;
+  if (i < kBarVFull) return 2;   // KEmpty
+  if (i < kBarVEmpty) return 1;
   if (i < kBarBEmpty) return 4;  // VEmpty, Fac, BFull
-  if (i < kBarQFull) return 1;
-  if (i < kBarQEmpty) return 2;
-  if (i < kBarPFull) return 1;   // QEmpty, SFull
-  if (i < kBarODone) return 8;
-  if (i == kBarODone) return 1;
-  if (i < kBarItemFull) return 16;
-  if (i < kBarItemEmpty) return 1;
-  if (i < kBarDrain) return kThreads / 32;
-  return i < kBarScale ? 1 : 2;  // Drain; Scale, Mx
+  if (i < kBarQFull) return 2;   // BEmpty, QEmpty, ODone
+  if (i < kBarPFull) return 1;   // QFull, SFull
+  if (i < kBarPv) return 4;
+  if (i < kBarOFree) return 1;   // Pv
+  if (i < kBarItemEmpty) return 16;
+  return i < kBarItemFull ? kThreads / 32 : 1;
 }
 
 // TMEM columns.
-__device__ __forceinline__ constexpr uint32_t col_s(int s) { return 128u * s; }
+__device__ __forceinline__ constexpr uint32_t col_s(int s, int b) { return 128u * s + 64u * b; }
 __device__ __forceinline__ constexpr uint32_t col_o(int s) { return 256u + 128u * s; }
 
 // ---- PTX ------------------------------------------------------------------------------
@@ -212,26 +212,29 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 }
-// Warp-wide forms: elect.sync picks the one issuing lane (always the same for a full warp).
+// One lane of a full warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}\n" : "=r"(e));
+  return e != 0;
+}
 __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile(
-      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
-      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
-          bar)
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar)
       : "memory");
 }
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                        uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc,
                                        uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
 }
 // Shared-memory matrix descriptor, 128-byte swizzle (sm_100 descriptor version 1).
@@ -243,9 +246,9 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint3
   d |= 2ull << 61;
   return d;
 }
-// Instruction descriptors, M128 N128, fp32 accumulator: e4m3 x e4m3 (both K-major), and
-// bf16 x bf16 with an MN-major B.
-constexpr uint32_t kIdescQK = (1u << 4) | (static_cast<uint32_t>(kN >> 3) << 17) |
+// Instruction descriptors, fp32 accumulator: M128 N64, e4m3 x e4m3 (both K-major), and M128
+// N128, bf16 x bf16 with an MN-major B.
+constexpr uint32_t kIdescQK = (1u << 4) | (static_cast<uint32_t>(kHalf >> 3) << 17) |
                               (static_cast<uint32_t>(kM >> 4) << 24);
 constexpr uint32_t kIdescPV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
                               (static_cast<uint32_t>(kD >> 3) << 17) |
@@ -455,7 +458,7 @@ __device__ __forceinline__ int cut_tile(const ItemInfo& it, int64_t start, int64
 }
 
 struct Piece {
-  int r, h, mb, P, T, q_start, t0, n, key_end, two, slot, last;
+  int r, h, mb, P, T, q_start, t0, n, key_end, two, slot;
 };
 // A piece's partial slot in the workspace, or -1 for a whole item.
 struct PieceMeta {
@@ -466,22 +469,28 @@ struct Workspace {
   float2* ml;        // [slot][tile][128] max (log2 units), sum
   float4* o;         // [slot][tile][32 groups of 4 columns][128]
   float* q_factor;   // [kv head][packed query row] scale * log2(e) * 2^e
+  uint32_t* mask;    // [node][kMaskWords] bit n: the node sees tree node n
   uint8_t* q_terms;  // [kv head][term][packed query row][128] e4m3
 };
 constexpr int64_t kMetaBytes = 2 * kMaxCtas * sizeof(PieceMeta);
 constexpr int64_t kMlBytes = 2ll * kMaxCtas * 2 * kM * sizeof(float2);
 constexpr int64_t kPartBytes = 2ll * kMaxCtas * 2 * kM * kD * sizeof(float);
 static_assert(kMetaBytes % 256 == 0 && kMlBytes % 256 == 0, "workspace alignment");
-// Query terms of one KV head and term: a packed row is (node, query head of the group).
+// A packed query row is (node, query head of the group).
 __host__ __device__ __forceinline__ int64_t factor_bytes(int64_t rows, int heads) {
   return (rows * heads * 4 + 255) / 256 * 256;
 }
-__host__ __device__ __forceinline__ Workspace carve(void* base, int64_t rows = 0, int heads = 0) {
+__host__ __device__ __forceinline__ int64_t mask_bytes(int64_t nodes) {
+  return (nodes * kMaskWords * 4 + 255) / 256 * 256;
+}
+__host__ __device__ __forceinline__ Workspace carve(void* base, int64_t nodes = 0, int groups = 0,
+                                                    int heads = 0) {
   char* b = static_cast<char*>(base);
   char* q = b + kMetaBytes + kMlBytes + kPartBytes;
   return Workspace{reinterpret_cast<PieceMeta*>(b), reinterpret_cast<float2*>(b + kMetaBytes),
                    reinterpret_cast<float4*>(b + kMetaBytes + kMlBytes), reinterpret_cast<float*>(q),
-                   reinterpret_cast<uint8_t*>(q + factor_bytes(rows, heads))};
+                   reinterpret_cast<uint32_t*>(q + factor_bytes(nodes * groups, heads)),
+                   reinterpret_cast<uint8_t*>(q + factor_bytes(nodes * groups, heads) + mask_bytes(nodes))};
 }
 
 // Page and offset of key position `pos` of a piece, page -1 past its keys or out of the pool.
@@ -522,46 +531,17 @@ struct LoadPlan {
   int box;
 };
 
-// Visibility words of the 64 keys at kb for this lane's row: bit b of word w is key
-// kb + 32 w + b.  Each warp builds its rows' words node by node: lane b reads the bias of its
-// key, a ballot collects the word, and the lanes of that node keep it.
-__device__ __noinline__ uint2 mask_words(const float* bias, int kb, int P, int T, int key_end,
-                                         int j, bool ok) {
-  const int lane = threadIdx.x & 31;
-  uint32_t mw[2] = {0u, 0u};
-  const int lo = __reduce_min_sync(0xffffffffu, ok ? j : 0x7fffffff);
-  const int hi = __reduce_max_sync(0xffffffffu, ok ? j : -1);
-#pragma unroll 1
-  for (int base = lo; base <= hi; base += 4) {
-    float b[4][2];
+// Visibility words of 64 keys for a row, from its node's bits: bit b of the first word is the key
+// `off` + b past the prefix.  Prefix keys are visible.
+__device__ __noinline__ uint2 mask_words(const uint32_t* bits, int off) {
+  uint32_t w[3], out[2];
+  const int first = off >> 5;  // -1 and below: prefix
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 3; ++i)
+    w[i] = first + i < 0 ? ~0u : first + i < kMaskWords ? __ldg(bits + first + i) : 0u;
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int node = base + i, key = kb + 32 * w + lane - P;
-        b[i][w] = -INFINITY;
-        if (node <= hi && key + P < key_end) {
-          if (key < 0)
-            b[i][w] = 0.f;
-          else if (key <= node)
-            b[i][w] = __ldg(bias + static_cast<int64_t>(node) * T + key);
-        }
-      }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const uint32_t bits = __ballot_sync(0xffffffffu, b[i][w] == 0.f);
-        if (ok && j == base + i) mw[w] = bits;
-      }
-  }
-  return make_uint2(mw[0], mw[1]);
-}
-
-// Columns of P inside an S buffer: keys 16 kk .. 16 kk + 15 (8 columns of bf16 pairs).  Each
-// half tile's P lies in the columns of the scores it came from, the low parts 32 columns on.
-__device__ __forceinline__ constexpr uint32_t col_p(int kk) {
-  return kk < 4 ? 8u * kk : 64u + 8u * (kk - 4);
+  for (int i = 0; i < 2; ++i) out[i] = __funnelshift_r(w[i], w[i + 1], off & 31);
+  return make_uint2(out[0], out[1]);
 }
 
 // The largest of a row's 64 scores (times the keys' factors) of half a tile, and then, with the
@@ -737,11 +717,35 @@ __device__ __forceinline__ void store_columns(const JtTreeAttnFp8Params& p, int6
 // Queries as e4m3 terms of row / 2^e and the rows' factors, for the attention kernel's TMA: half
 // a warp per row (16 bytes per lane), its largest magnitude by shuffles.  A kernel of its own
 // (the attention starts beside it as a programmatic dependent): inside, the split of a
-// piece's 256 rows by one warpgroup took 25 thousand cycles, a third of a short piece.
+// piece's 256 rows by one warpgroup took 25 thousand cycles, a third of a short piece.  The
+// blocks from `first_mask` on turn the nodes' bias rows into visibility bits, a warp per node:
+// built at the start of a piece by its softmax warps, from the fp32 biases, they held up its
+// first tile by 7 thousand cycles.
 template <bool kWide, typename QT>
 __global__ void __launch_bounds__(256) tree_attn_fp8_split_kernel(
-    const __grid_constant__ JtTreeAttnFp8Params p) {
+    const __grid_constant__ JtTreeAttnFp8Params p, const unsigned first_mask) {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  if (blockIdx.x >= first_mask) {
+    const int64_t q = static_cast<int64_t>(blockIdx.x - first_mask) * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (q >= p.total_queries) return;
+    const int r = __ldg(p.query_to_request + q), j = __ldg(p.query_local_row + q);
+    uint32_t mine = 0;  // word `lane`
+    if (r >= 0 && r < p.num_requests && j >= 0) {
+      const int T = __ldg(p.node_counts + r);
+      if (j < T && T <= kMaxNodes) {
+        const float* bias = p.qq_bias + __ldg(p.qq_bias_offsets + r) + static_cast<int64_t>(j) * T;
+#pragma unroll 4
+        for (int w = 0; 32 * w <= j; ++w) {
+          const int n = 32 * w + lane;
+          const uint32_t word = __ballot_sync(0xffffffffu, n <= j && __ldg(bias + min(n, j)) == 0.f);
+          if (lane == w) mine = word;
+        }
+      }
+    }
+    carve(p.workspace, p.total_queries, p.groups, p.num_kv_heads).mask[q * kMaskWords + lane] = mine;
+    return;
+  }
   constexpr int kTerms = Smem<kWide>::kTerms;
   const int64_t rows = static_cast<int64_t>(p.total_queries) * p.groups;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
@@ -774,7 +778,7 @@ __global__ void __launch_bounds__(256) tree_attn_fp8_split_kernel(
     x[k] = jt::MmaOp<QT>::unpack(a[k]);
     x[k] = make_float2(x[k].x * inv, x[k].y * inv);
   }
-  const Workspace ws = carve(p.workspace, rows, p.num_kv_heads);
+  const Workspace ws = carve(p.workspace, p.total_queries, p.groups, p.num_kv_heads);
   uint8_t* dst = ws.q_terms + (static_cast<int64_t>(h) * kTerms * rows + row) * kD + 8 * hl;
 #pragma unroll
   for (int m = 0; m < kTerms; ++m) {
@@ -810,7 +814,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #define JT_BAR(i) (bar0 + 8u * static_cast<uint32_t>(i))
   volatile int* misc = reinterpret_cast<volatile int*>(sbase + L::kMisc);
   volatile int* abort = misc + 1;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform for the compiler too
   const Geometry ge{p.groups, kM / p.groups, (kM / p.groups) * L::kTiles};
 
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
@@ -872,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = static_cast<uint32_t>(misc[0]);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, static_cast<uint32_t>(misc[0]), 0);
   const int r_start = has_part ? static_cast<int>(scan[32]) : R;
   const int64_t s_start = has_part ? scan[33] : 0;
   __syncthreads();  // the scan area is free
@@ -888,8 +893,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       volatile int* e = item_ring + 16 * slot;
       it.r = e[0]; it.h = e[1]; it.mb = e[2]; it.P = e[3]; it.T = e[4]; it.q_start = e[5];
       it.t0 = e[6]; it.n = e[7]; it.key_end = e[8]; it.two = e[9]; it.slot = e[10];
-      it.last = e[11];
-      ok = e[12];
+      ok = e[11];
     }
     ok = __all_sync(0xffffffffu, ok != 0);
     if (lane == 0) mbar_arrive(JT_BAR(kBarItemEmpty + slot));
@@ -897,68 +901,82 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   if (warp < 4) {
-    if (warp == 0) {
-      // ---------------------------------------------------------------- MMA issuer
-      // QK of a stream's next tile is issued right behind the PV that reads P out of the same
-      // S buffer: MMAs of one thread execute in order.
+    if (warp == 0 || warp == 2) {
+      // ---------------------------------------------------------------- MMA issuers
+      // One per stream: a step's waits, 12 MMAs and commits take a lone issuer, between warps
+      // that keep every scheduler busy, longer than the softmax takes for the granule.
+      const int s = warp >> 1;
       uint32_t g0 = 0, seq = 0;
-      uint32_t p_phase = 0;  // bit s: stream s
+      uint32_t p_phase = 0;  // bit b: score buffer b
       const uint64_t q_desc = smem_desc(base + L::kQ, 16, 1024);
       const uint64_t k_desc = smem_desc(base + L::kK, 16, 1024);
       const uint64_t v_desc = smem_desc(base + L::kV16, kHalf16, 1024);
+      const uint32_t d_o = tmem + col_o(s);
       for (;; ++seq) {
         Piece it;
         if (!next_piece(seq, it)) break;
-        const int n = it.n, two = it.two;
+        const int n = __shfl_sync(0xffffffffu, it.n, 0), two = __shfl_sync(0xffffffffu, it.two, 0);
         mbar_wait(JT_BAR(kBarQFull), seq & 1, abort);
         tc_fence_after();
-        // Step u is stream u & 1's product with key tile u (one query tile) or u >> 1 (two).
-        const int steps = n << two;
+        // A stream takes its keys 64 at a time, in granules that alternate between its two
+        // score buffers: with two query tiles granule k is half k & 1 of key tile k >> 1, with
+        // one it is stream s's half of key tile k.  QK of granule k + 2 follows PV of granule
+        // k, which read P out of the same buffer (MMAs of one thread execute in order);
+        // granule k + 1 is in the softmax meanwhile.
+        const int granules = two ? 2 * n : n;
+        const uint64_t qd = q_desc + (two & s) * (kTerms * kTile8 / 16);
 #pragma unroll 1
-        for (int u = -2; u < steps; ++u) {
-          const int s = u & 1;
-          const uint32_t d_s = tmem + col_s(s), d_o = tmem + col_o(s);
-          if (u >= 0) {
-            const uint32_t g = g0 + (u >> two);
-            if (!two || s == 0) mbar_wait(JT_BAR(kBarBFull + (g & 1)), (g >> 1) & 1, abort);
-            if (u == 0 && seq > 0) mbar_wait(JT_BAR(kBarOFree), (seq - 1) & 1, abort);
-            const uint64_t vd = v_desc + (g & 1) * (kTile16 >> 4);
-            mbar_wait(JT_BAR(kBarPFull + s), (p_phase >> s) & 1, abort);
+        for (int k = -2; k < granules; ++k) {
+          const int b = k & 1, h = two ? b : s;
+          const bool first = !two || b == 0, last = !two || b == 1;  // granule of its tile
+          const uint32_t d_s = tmem + col_s(s, b);
+          if (k >= 0) {
+            const uint32_t g = g0 + (two ? k >> 1 : k);
+            if (first) mbar_wait(JT_BAR(kBarBFull + (g & 1)), (g >> 1) & 1, abort);
+            if (k == 0 && seq > 0) mbar_wait(JT_BAR(kBarOFree), (seq - 1) & 1, abort);
+            mbar_wait(JT_BAR(kBarPFull + 2 * s + b), (p_phase >> b) & 1, abort);
+            p_phase ^= 1u << b;
             tc_fence_after();
+            const uint64_t vd = v_desc + ((g & 1) * kTile16 + h * (kHalf * 128)) / 16;
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kN / 16; ++kk) {
-              mma_ts(d_o, d_s + col_p(kk), vd + kk * (2048 / 16), kIdescPV, u > 1 || kk > 0 ? 1u : 0u);
-              if constexpr (kWide)
-                mma_ts(d_o, d_s + col_p(kk) + 32, vd + kk * (2048 / 16), kIdescPV, 1u);
+              for (int kk = 0; kk < kHalf / 16; ++kk) {
+                mma_ts(d_o, d_s + 8 * kk, vd + kk * (2048 / 16), kIdescPV, k > 0 || kk > 0 ? 1u : 0u);
+                if constexpr (kWide)
+                  mma_ts(d_o, d_s + 8 * kk + 32, vd + kk * (2048 / 16), kIdescPV, 1u);
+              }
+              commit(JT_BAR(kBarPv + s));
+              if (last) commit(JT_BAR(kBarBEmpty + (g & 1)));
             }
-            p_phase ^= 1u << s;
-            if (!two || s == 1) commit(JT_BAR(kBarBEmpty + (g & 1)));
+            __syncwarp();
           }
-          if (u + 2 < steps) {
-            const int t = (u + 2) >> two;
+          if (k + 2 < granules) {
+            const int t = two ? (k + 2) >> 1 : k + 2;
             const uint32_t g = g0 + t;
-            if (!two || s == 0) {
+            if (first) {
               mbar_wait(JT_BAR(kBarKFull + g % kKRing), (g / kKRing) & 1, abort);
               tc_fence_after();
             }
-            const uint64_t qd = q_desc + (two & s) * (kTerms * kTile8 / 16);
-            const uint64_t kd = k_desc + (g % kKRing) * (kTile8 >> 4);
+            const uint64_t kd = k_desc + ((g % kKRing) * kTile8 + h * (kHalf * 128)) / 16;
+            if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < kTerms * 4; ++i)  // (term, 32 dims)
-              mma_f8(d_s, qd + (i >> 2) * (kTile8 / 16) + (i & 3) * 2, kd + (i & 3) * 2,
-                          kIdescQK, i != 0 ? 1u : 0u);
-            commit(JT_BAR(kBarSFull + s));
-            if (!two || s == 1) {
-              commit(JT_BAR(kBarKEmpty + g % kKRing));
-              if (t == n - 1) commit(JT_BAR(kBarQEmpty));
+              for (int m = 0; m < kTerms * 4; ++m)  // (term, 32 dims)
+                mma_f8(d_s, qd + (m >> 2) * (kTile8 / 16) + (m & 3) * 2, kd + (m & 3) * 2, kIdescQK,
+                       m != 0 ? 1u : 0u);
+              commit(JT_BAR(kBarSFull + 2 * s + b));
+              if (last) commit(JT_BAR(kBarKEmpty + g % kKRing));
+              if (last && t == n - 1) commit(JT_BAR(kBarQEmpty));
             }
+            __syncwarp();
           }
         }
-        commit(JT_BAR(kBarODone));
+        if (elect_one()) commit(JT_BAR(kBarODone));
+        __syncwarp();
         g0 += n;
       }
-      commit(JT_BAR(kBarDrain));
-      mbar_wait(JT_BAR(kBarDrain), 0, abort, false);
+      if (elect_one()) commit(JT_BAR(kBarDrain + s));
+      __syncwarp();
+      mbar_wait(JT_BAR(kBarDrain + s), 0, abort, false);
     } else if (warp == 1) {
       // ---------------------------------------------------------------- pieces and TMA
       // The whole warp follows the pieces; its first lane does the work.
@@ -984,7 +1002,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int slot = seq & 1;
         if (seq >= 2) mbar_wait(JT_BAR(kBarItemEmpty + slot), ((seq >> 1) - 1) & 1, abort);
         volatile int* e = item_ring + 16 * slot;
-        e[12] = 0;
+        e[11] = 0;
         while (more && !*abort) {
           const ItemInfo it = item_info(ge, P, T, mb);
           const int tb = cut_tile(it, s_item, x0), te = cut_tile(it, s_item, x1);
@@ -996,7 +1014,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             e[0] = r; e[1] = h; e[2] = mb; e[3] = P; e[4] = T;
             e[5] = __ldg(p.cu_seqlens_q + r);
             e[6] = tb; e[7] = te - tb; e[8] = it.key_end; e[9] = it.weight == 2 ? 1 : 0;
-            e[10] = part; e[11] = te == it.n; e[12] = 1;
+            e[10] = part; e[11] = 1;
             if (!whole) {
               PieceMeta* m = carve(p.workspace).meta + part;
               m->finishes = te == it.n;
@@ -1058,7 +1076,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (g >= static_cast<uint32_t>(ring))
             mbar_wait(JT_BAR((is_v ? kBarVEmpty : kBarKEmpty) + slot), ((g / ring) & 1) ^ 1, abort);
           if (*abort) return;
-          if (!plan.tma || kb + kN > it.P) {  // gathered by warps 2-3, told that the slot is free
+          if (!plan.tma || kb + kN > it.P) {  // gathered by warp 3, told that the slot is free
             note(is_v ? 4 + slot : slot, false, 0);
             if (!is_v) note(8 + g % kScaleRing, false, 0);
             st_release_shared(base + L::kMisc + (is_v ? 12 : 8), g + 1);
@@ -1086,12 +1104,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               bulk_load(sdst + kN, vsc + pg * p.vs_stride0 + it.h * p.vs_stride1 + off, plan.box, sc_full);
             }
           }
-          mbar_arrive(full);
           note(is_v ? 4 + slot : slot, true, g / ring);
-          if (!is_v) {
-            mbar_arrive(sc_full);
-            note(8 + sc_slot, true, g / kScaleRing);
-          }
+          if (!is_v) note(8 + sc_slot, true, g / kScaleRing);
         };
         if (lane == 0) {
           // K 0, K 1, then V t and K t + 2: the order in which they are used.
@@ -1110,7 +1124,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tma_load_3d(base + L::kQ + k * kTile8, &qmap, 0,
                             row + (k >= kTerms ? ge.npt * ge.groups : 0),
                             it.h * kTerms + (k >= kTerms ? k - kTerms : k), JT_BAR(kBarQFull));
-              mbar_arrive(JT_BAR(kBarQFull));
               q_fills = seq + 1;
             }
             const bool is_v = i >= 2 && !(i & 1);
@@ -1138,7 +1151,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---------------------------------------------------------------- gathers
       // Tiles that TMA does not take: rows by cp.async, scale bytes by plain loads into the
       // same staging.
-      const int gt = tid - 64;  // two keys per thread
       const int chunks = p.head_dim / 16;
       uint32_t g0 = 0;
 #pragma unroll 1
@@ -1150,35 +1162,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = plan.tma ? max(0, it.P / kN - it.t0) : 0; t < it.n; ++t) {
           const uint32_t g = g0 + t;
           const uint32_t ks = g % kKRing, vs = g % kVRing;
+          // Four keys per lane; their slots and scales are loaded together, before the slot is
+          // free.
+          const char* k_src[4];
+          const char* v_src[4];
+          uint32_t kb[4], vb[4];
+          bool ok[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const KeyPlace at = locate_key(p, table, (it.t0 + t) * kN + 32 * i + lane, it.P, it.key_end, it.q_start);
+            ok[i] = at.page >= 0;
+            const int64_t page = ok[i] ? at.page : 0;
+            k_src[i] = static_cast<const char*>(p.k_pool) + page * p.k_stride0 + at.off * p.k_stride1 + it.h * p.k_stride2;
+            v_src[i] = static_cast<const char*>(p.v_pool) + page * p.v_stride0 + at.off * p.v_stride1 + it.h * p.v_stride2;
+            kb[i] = vb[i] = 127;
+            if (ok[i]) {
+              kb[i] = __ldg(static_cast<const uint8_t*>(p.k_scale) + page * p.ks_stride0 +
+                            it.h * p.ks_stride1 + at.off);
+              vb[i] = __ldg(static_cast<const uint8_t*>(p.v_scale) + page * p.vs_stride0 +
+                            it.h * p.vs_stride1 + at.off);
+            }
+          }
           wait_shared_at_least(base + L::kMisc + 8, g + 1, abort);
           wait_shared_at_least(base + L::kMisc + 12, g + 1, abort);
           __syncwarp();
-#pragma unroll 1
-          for (int i = 0; i < 2; ++i) {
-            const int row = 2 * gt + i;
-            const KeyPlace at = locate_key(p, table, (it.t0 + t) * kN + row, it.P, it.key_end, it.q_start);
-            const bool ok = at.page >= 0;
-            const char* k = static_cast<const char*>(p.k_pool);
-            const char* v = static_cast<const char*>(p.v_pool);
-            uint8_t kb = 127, vb = 127;
-            if (ok) {
-              k += at.page * p.k_stride0 + at.off * p.k_stride1 + it.h * p.k_stride2;
-              v += at.page * p.v_stride0 + at.off * p.v_stride1 + it.h * p.v_stride2;
-              kb = __ldg(static_cast<const uint8_t*>(p.k_scale) + at.page * p.ks_stride0 +
-                         it.h * p.ks_stride1 + at.off);
-              vb = __ldg(static_cast<const uint8_t*>(p.v_scale) + at.page * p.vs_stride0 +
-                         it.h * p.vs_stride1 + at.off);
-            }
-            gather_row(base + L::kK + ks * kTile8, row, k, ok ? chunks : 0);
-            gather_row(base + L::kV8 + vs * kTile8, row, v, ok ? chunks : 0);
-            unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256 + row;
-            sc[0] = kb;
-            sc[kN] = vb;
+          unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256 + lane;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            gather_row(base + L::kK + ks * kTile8, 32 * i + lane, k_src[i], ok[i] ? chunks : 0);
+            gather_row(base + L::kV8 + vs * kTile8, 32 * i + lane, v_src[i], ok[i] ? chunks : 0);
+            sc[32 * i] = static_cast<unsigned char>(kb[i]);
+            sc[kN + 32 * i] = static_cast<unsigned char>(vb[i]);
           }
           asm volatile("cp.async.wait_all;\n" ::: "memory");
           fence_proxy_async();
-          warp_arrive(JT_BAR(kBarKFull + ks));
+          __syncwarp();
           if (lane == 0) {
+            mbar_arrive(JT_BAR(kBarKFull + ks));
             mbar_arrive(JT_BAR(kBarVFull + vs));
             mbar_arrive(JT_BAR(kBarScale + g % kScaleRing));
           }
@@ -1260,19 +1280,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------------ softmax + epilogue
-    const int wg = (warp - 8) >> 2, s = wg >> 1, half = wg & 1;  // stream, half tile of keys
+    const int wg = (warp - 8) >> 2, s = wg >> 1, buf = wg & 1;  // stream, score buffer
     const int row = (tid - 256) & 127;                          // query-tile row, TMEM lane
     const uint32_t lanes = static_cast<uint32_t>((row >> 5) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + col_s(s) + 64 * half;
-    const uint32_t mx_bar = JT_BAR(kBarMx + 4 * s + (warp & 3));
-    const float* kf = reinterpret_cast<const float*>(sbase + L::kKf) + 64 * half;
-    const float* q_factor = carve(p.workspace, static_cast<int64_t>(p.total_queries) * ge.groups,
-                                  p.num_kv_heads).q_factor;
+    const uint32_t s_addr = tmem + lanes + col_s(s, buf);
+    const uint32_t my_bar = JT_BAR(kBarMx + (2 * s + buf) * 4 + (warp & 3));
+    const uint32_t other_bar = JT_BAR(kBarMx + (2 * s + (buf ^ 1)) * 4 + (warp & 3));
+    const float* kf = reinterpret_cast<const float*>(sbase + L::kKf);
+    const Workspace ws = carve(p.workspace, p.total_queries, ge.groups, p.num_kv_heads);
     const volatile int* flag = reinterpret_cast<const volatile int*>(sbase + L::kFlag);
     float2* xch = reinterpret_cast<float2*>(sbase + L::kX);
-    float* mxs = reinterpret_cast<float*>(sbase + L::kMx);
+    float* m_row = reinterpret_cast<float*>(sbase + L::kMx) + s * kM + row;
     const int local = row / ge.groups, head_in = row - local * ge.groups;
-    uint32_t g0 = 0, step = 0, mx_step = 0;
+    uint32_t g0 = 0, own = 0, other = 0;  // tiles; granules of this buffer, of the other one
 #pragma unroll 1
     for (uint32_t seq = 0;; ++seq) {
       Piece it;
@@ -1281,73 +1301,74 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int j = it.mb * ge.npi + (it.two ? s * ge.npt : 0) + local;
       const bool ok = local < ge.npt && j < it.T;
       const bool live = __any_sync(0xffffffffu, ok);
-      const float* bias = p.qq_bias + __ldg(p.qq_bias_offsets + it.r);
-      const int t_first = it.two ? 0 : s, t_step = it.two ? 1 : 2;
-      // First masked tile of this stream (tiles below floor(P / 128) need no mask), and its
-      // words, built ahead of it.
-      int t_mask = max(0, it.P / kN - it.t0);
-      if (!it.two && ((t_mask ^ s) & 1)) ++t_mask;
-      uint2 mw = make_uint2(0u, 0u);
-      if (live && t_mask < n)
-        mw = mask_words(bias, (it.t0 + t_mask) * kN + 64 * half, it.P, it.T, it.key_end, j, ok);
+      const int granules = it.two ? 2 * n : n, half = it.two ? buf : s;
+      // Tiles below floor(P / 128) need no mask.
+      const int t_mask = max(0, it.P / kN - it.t0);
       float m_run = -INFINITY, l_run = 0.f;
       const float c_row =
-          ok ? __ldg(q_factor + (static_cast<int64_t>(it.h) * p.total_queries + it.q_start + j) * ge.groups + head_in)
+          ok ? __ldg(ws.q_factor + (static_cast<int64_t>(it.h) * p.total_queries + it.q_start + j) * ge.groups + head_in)
              : 0.f;
 #pragma unroll 1
-      for (int t = t_first; t < n; t += t_step) {
-        const uint32_t g = g0 + t;
+      for (int k = buf; k < granules; k += 2) {
+        const int t = it.two ? k >> 1 : k;
+        const uint32_t g = g0 + t, step = own + (k >> 1);
+        bool careful = t >= t_mask;
+        uint2 w = make_uint2(~0u, ~0u);
+        if (careful && live) {
+          w = mask_words(ws.mask + (static_cast<int64_t>(it.q_start) + (ok ? j : 0)) * kMaskWords,
+                         (it.t0 + t) * kN + kHalf * half - it.P);
+          if (!ok) w = make_uint2(0u, 0u);
+        }
         warp_wait(JT_BAR(kBarFac + (g & 1)), (g >> 1) & 1, abort);
-        warp_wait(JT_BAR(kBarSFull + s), step & 1, abort);
-        ++step;
+        warp_wait(JT_BAR(kBarSFull + 2 * s + buf), step & 1, abort);
         tc_fence_after();
         if (live) {
-          const float* f = kf + (g & 1) * kN;
-          const bool masked = t >= t_mask;
-          const bool careful =
-              masked || (flag[(g & 1) * 4] | flag[(g & 1) * 4 + 1] | flag[(g & 1) * 4 + 2] |
-                         flag[(g & 1) * 4 + 3]) != 0;
-          const uint2 w = masked ? mw : make_uint2(~0u, ~0u);
-          const float mine = careful ? half_max_masked(s_addr, f, w.x, w.y) : half_max(s_addr, f);
-          // The two warps that share these rows meet, so that both halves use one maximum.
-          float* slot = mxs + (mx_step & 1) * 4 * kM + s * 2 * kM + row;
-          slot[half * kM] = mine;
-          warp_arrive(mx_bar);
-          warp_wait(mx_bar, mx_step & 1, abort);
-          ++mx_step;
-          // Lazy running maximum: it moves only when a tile exceeds it by 2^8, so P stays
-          // below 2^8 and O is rarely rescaled.
-          const float mx = fmaxf(mine, slot[(half ^ 1) * kM]) * c_row;
-          float alpha = 1.f;
-          if (mx > m_run + 8.f) {
-            if (m_run != -INFINITY) alpha = jt::fast_exp2(m_run - mx);
-            m_run = mx;
+          const float* f = kf + (g & 1) * kN + kHalf * half;
+          careful |= (flag[(g & 1) * 4] | flag[(g & 1) * 4 + 1] | flag[(g & 1) * 4 + 2] |
+                      flag[(g & 1) * 4 + 3]) != 0;
+          const float mx = c_row * (careful ? half_max_masked(s_addr, f, w.x, w.y) : half_max(s_addr, f));
+          // The rows' running maximum goes from granule to granule, between the two warps that
+          // share the rows.  It is lazy: it moves only when a granule exceeds it by 2^8, so P
+          // stays below 2^8 and O is rarely rescaled.
+          float m_old = -INFINITY;
+          if (k > 0) {
+            warp_wait(other_bar, (other + ((k - 1) >> 1)) & 1, abort);
+            m_old = *m_row;
           }
-          const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
-          const float sum = careful ? half_exp_masked<kWide>(s_addr, f, c_row, neg_m, w.x, w.y)
-                                    : half_exp<kWide>(s_addr, f, c_row, neg_m);
-          l_run = l_run * alpha + sum;
-          // This tile's scores were issued behind the stream's last PV, which has therefore
-          // completed: O (this half of its columns) can be rescaled at once.
-          if (t != t_first && __any_sync(0xffffffffu, alpha != 1.f)) {
+          const bool moved = mx > m_old + 8.f;
+          const float m_new = moved ? mx : m_old;
+          *m_row = m_new;
+          warp_arrive(my_bar);
+          // This warp's sum is relative to the maximum at its previous granule.
+          if (m_run != m_new && m_run != -INFINITY) l_run *= jt::fast_exp2(m_run - m_new);
+          m_run = m_new;
+          const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
+          l_run += careful ? half_exp_masked<kWide>(s_addr, f, c_row, neg_m, w.x, w.y)
+                           : half_exp<kWide>(s_addr, f, c_row, neg_m);
+          if (__any_sync(0xffffffffu, moved && m_old != -INFINITY)) {
+            // Rescale O once PV of the stream's previous granule has completed.  The wait is for
+            // exactly the latest phase: the PV before it completed ahead of this granule's
+            // scores, which were issued behind it, and the next PV needs this granule's P.
+            const float alpha = moved && m_old != -INFINITY ? jt::fast_exp2(m_old - m_new) : 1.f;
+            warp_wait(JT_BAR(kBarPv + s), (own + other + k - 1) & 1, abort);
+            tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 8; ++c) {
               uint32_t o[16];
-              tmem_ld16(tmem + lanes + col_o(s) + 64 * half + 16 * c, o);
+              tmem_ld16(tmem + lanes + col_o(s) + 16 * c, o);
               tmem_wait_ld();
 #pragma unroll
               for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-              tmem_st16(tmem + lanes + col_o(s) + 64 * half + 16 * c, o);
+              tmem_st16(tmem + lanes + col_o(s) + 16 * c, o);
             }
           }
           tmem_wait_st();
+        } else {
+          warp_arrive(my_bar);
         }
         // A warp without a live row arrives too; its rows of P are never read out.
         tc_fence_before();
-        warp_arrive(JT_BAR(kBarPFull + s));
-        // The words of the next masked tile, behind this tile's product.
-        if (live && t >= t_mask && t + t_step < n)
-          mw = mask_words(bias, (it.t0 + t + t_step) * kN + 64 * half, it.P, it.T, it.key_end, j, ok);
+        warp_arrive(JT_BAR(kBarPFull + 2 * s + buf));
       }
       // Epilogue, once the piece's last PV has completed: the halves' sums meet, with one query
       // tile also the streams' (max, sum).  With one tile each warpgroup merges and writes 32
@@ -1359,22 +1380,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       warp_wait(JT_BAR(kBarX), seq & 1, abort);
       if (live) {
         const bool pair = !it.two;
-        const float2 a0 = xch[(pair ? 0 : 2 * s) * kM + row], a1 = xch[(pair ? 1 : 2 * s + 1) * kM + row];
-        float fa = 1.f, fb = 0.f, m = a0.x, l = a0.y + a1.y;
-        if (pair && n > 1) {
-          const float2 b0 = xch[2 * kM + row], b1 = xch[3 * kM + row];
-          const float lb = b0.y + b1.y;
-          m = fmaxf(a0.x, b0.x);
-          fa = a0.x == -INFINITY ? 0.f : jt::fast_exp2(a0.x - m);
-          fb = b0.x == -INFINITY ? 0.f : jt::fast_exp2(b0.x - m);
-          // A stream without a maximum has a zero sum, or a NaN that has to stay.
-          l = l * (a0.x == -INFINITY ? 1.f : fa) + lb * (b0.x == -INFINITY ? 1.f : fb);
+        // A sum without a maximum is zero, or a NaN that has to stay.
+        auto joined = [&](float2 a, float2 b) {
+          const float m = fmaxf(a.x, b.x);
+          return make_float2(m, a.y * (a.x == -INFINITY ? 1.f : jt::fast_exp2(a.x - m)) +
+                                    b.y * (b.x == -INFINITY ? 1.f : jt::fast_exp2(b.x - m)));
+        };
+        const int s0 = pair ? 0 : 2 * s;
+        const float2 a = joined(xch[s0 * kM + row], xch[(s0 + 1) * kM + row]);
+        float fa = 1.f, fb = 0.f, m = a.x, l = a.y;
+        if (pair) {
+          const float2 b = joined(xch[2 * kM + row], xch[3 * kM + row]);
+          const float2 both = joined(a, b);
+          m = both.x;
+          l = both.y;
+          fa = a.x == -INFINITY ? 0.f : jt::fast_exp2(a.x - m);
+          fb = b.x == -INFINITY ? 0.f : jt::fast_exp2(b.x - m);
         }
-        const Workspace w = carve(p.workspace);
         const int tile = pair ? 0 : s;
         if (it.slot >= 0) {
-          if (ok && (pair ? wg == 0 : half == 0))
-            w.ml[(it.slot * 2ll + tile) * kM + row] = make_float2(m, l);
+          if (ok && (pair ? wg == 0 : buf == 0))
+            ws.ml[(it.slot * 2ll + tile) * kM + row] = make_float2(m, l);
         } else {
           const float inv = l == 0.f ? 0.f : 1.f / l;
           fa *= inv;
@@ -1382,7 +1408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int64_t out_row = (static_cast<int64_t>(it.q_start) + j) * p.out_stride0 +
                                 (static_cast<int64_t>(it.h) * ge.groups + head_in) * p.out_stride1;
-        const int c0 = pair ? 2 * wg : 4 * half, c1 = c0 + (pair ? 2 : 4);
+        const int c0 = pair ? 2 * wg : 4 * buf, c1 = c0 + (pair ? 2 : 4);
 #pragma unroll 1
         for (int c = c0; c < c1; ++c) {  // 16 columns
           uint32_t o0[16], o1[16];
@@ -1390,14 +1416,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld16(tmem + lanes + col_o(tile) + 16 * c, o0);
 #pragma unroll
           for (int k = 0; k < 16; ++k) o1[k] = 0u;
-          if (pair && n > 1) tmem_ld16(tmem + lanes + col_o(1) + 16 * c, o1);
+          if (pair) tmem_ld16(tmem + lanes + col_o(1) + 16 * c, o1);
           tmem_wait_ld();
           float f[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k)
             f[k] = __uint_as_float(o0[o_column(k)]) * fa + __uint_as_float(o1[o_column(k)]) * fb;
           if (ok && it.slot >= 0) {
-            float4* dst = w.o + ((it.slot * 2ll + tile) * 32 + 4 * c) * kM + row;
+            float4* dst = ws.o + ((it.slot * 2ll + tile) * 32 + 4 * c) * kM + row;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               dst[k * kM] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
@@ -1414,6 +1440,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       warp_arrive(JT_BAR(kBarOFree));
       g0 += n;
+      own += (granules + 1 - buf) >> 1;
+      other += (granules + buf) >> 1;
     }
   }
 #undef JT_BAR
@@ -1476,8 +1504,9 @@ __global__ void __launch_bounds__(kM) tree_attn_fp8_merge_kernel(
   store_columns<kWide>(p, at, f);
 }
 
-int64_t workspace_bytes(int64_t rows, int heads) {  // for either kernel's number of terms
-  return kMetaBytes + kMlBytes + kPartBytes + factor_bytes(rows, heads) + rows * heads * 3 * kD;
+int64_t workspace_bytes(int64_t nodes, int groups, int heads) {  // for either kernel's terms
+  return kMetaBytes + kMlBytes + kPartBytes + factor_bytes(nodes * groups, heads) +
+         mask_bytes(nodes) + nodes * groups * heads * 3 * kD;
 }
 
 bool al16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
@@ -1562,7 +1591,7 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
     plan.tma = 0;  // a layout the encoder refuses: gathered like any other page size
   const int64_t rows = static_cast<int64_t>(p.total_queries) * p.groups;
   CUtensorMap qmap{};
-  if (!encode_queries(&qmap, carve(p.workspace, rows, p.num_kv_heads).q_terms, rows,
+  if (!encode_queries(&qmap, carve(p.workspace, p.total_queries, p.groups, p.num_kv_heads).q_terms, rows,
                       p.num_kv_heads * Smem<kWide>::kTerms))
     return jt_fail(JT_ERR_CUDA, "tree_attn_fp8: cuTensorMapEncodeTiled rejected the query terms");
   int rc = jt_cuda_check(cudaFuncSetAttribute(tree_attn_fp8_kernel<kWide>,
@@ -1570,10 +1599,11 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
                                               Smem<kWide>::kBytes),
                          "tree_attn_fp8 smem attribute");
   if (rc != JT_OK) return rc;
-  const int64_t split = (rows * p.num_kv_heads + 15) / 16;
-  if (split > 0x7fffffff || rows > 0x7fffffff)
+  const int64_t split = (rows * p.num_kv_heads + 15) / 16, mask = (p.total_queries + 7ll) / 8;
+  if (split + mask > 0x7fffffff || rows > 0x7fffffff)
     return jt_fail(JT_ERR_INVALID, "tree_attn_fp8: too many query rows");
-  tree_attn_fp8_split_kernel<kWide, QT><<<static_cast<unsigned>(split), 256, 0, stream>>>(p);
+  tree_attn_fp8_split_kernel<kWide, QT><<<static_cast<unsigned>(split + mask), 256, 0, stream>>>(
+      p, static_cast<unsigned>(split));
   rc = jt_cuda_check(cudaGetLastError(), "tree_attn_fp8 query split launch");
   if (rc != JT_OK) return rc;
   const int grid = std::min(sms, kMaxCtas);
@@ -1600,7 +1630,7 @@ extern "C" int64_t jt_tree_attn_fp8_workspace_size(int32_t num_requests, int32_t
                                                    int32_t head_dim) {
   if (num_requests < 1 || total_queries < 1 || num_kv_heads < 1 || groups < 1 || head_dim < 1)
     return -1;
-  return workspace_bytes(static_cast<int64_t>(total_queries) * groups, num_kv_heads);
+  return workspace_bytes(total_queries, groups, num_kv_heads);
 }
 
 extern "C" int jt_tree_attn_fp8_launch(const JtTreeAttnFp8Params* p, cudaStream_t stream) {
@@ -1627,7 +1657,7 @@ extern "C" int jt_tree_attn_fp8_launch(const JtTreeAttnFp8Params* p, cudaStream_
       (p->k_stride0 | p->k_stride1 | p->k_stride2 | p->v_stride0 | p->v_stride1 | p->v_stride2) % 16 != 0)
     return jt_fail(JT_ERR_INVALID,
                    "tree_attn_fp8: queries, output and pool rows must start on 16 bytes");
-  const int64_t need = workspace_bytes(static_cast<int64_t>(p->total_queries) * p->groups, p->num_kv_heads);
+  const int64_t need = workspace_bytes(p->total_queries, p->groups, p->num_kv_heads);
   if (p->workspace == nullptr || p->workspace_bytes < need ||
       (reinterpret_cast<uintptr_t>(p->workspace) & 255u) != 0)
     return jt_fail(JT_ERR_WORKSPACE, "tree_attn_fp8: workspace of %lld bytes required (got %lld)",
