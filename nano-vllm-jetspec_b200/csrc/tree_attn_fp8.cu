@@ -63,10 +63,12 @@ constexpr int kHalf16 = kTile8;
 constexpr int kMaxCtas = 160;         // workspace slots are sized for this many SMs
 constexpr int kMaxNodes = 1024;
 constexpr int kMaskWords = kMaxNodes / 32;
-// Costs in units of one 128-row, 128-key tile: an item's fixed cost (query load, pipeline
-// fill, epilogue), and the least part worth a CTA of its own.
-constexpr int kItemCost = 3;
-constexpr int kMinPart = 6;
+// Costs of the work line: a key tile against one and against two query tiles, an item's fixed
+// cost (pipeline fill, first maxima, epilogue), and the least part worth a CTA of its own.  From
+// the CTAs' cycles over a mix of items: 4.2 thousand, 6.0 thousand and 13 to 17 thousand.
+constexpr int kTileCost = 2, kPairCost = 3;
+constexpr int kItemCost = 8;
+constexpr int kMinPart = 24;
 constexpr int kMinTiles = 2;          // cuts closer than this to an item's end move to it
 constexpr long long kWaitLimit = 4000000000ll;  // cycles (~2 s) per wait
 
@@ -416,14 +418,15 @@ struct Geometry {
   int groups, npt, npi;  // nodes per query tile, per item
 };
 struct ItemInfo {
-  int key_end, n, weight, cost;
+  int key_end, n, two, weight, cost;
 };
 __device__ __forceinline__ ItemInfo item_info(const Geometry& ge, int P, int T, int mb) {
   const int first = mb * ge.npi, last = min(T, first + ge.npi);
   ItemInfo it;
   it.key_end = P + last;
   it.n = (it.key_end + kN - 1) >> 7;
-  it.weight = last - first > ge.npt ? 2 : 1;
+  it.two = last - first > ge.npt;
+  it.weight = it.two ? kPairCost : kTileCost;
   it.cost = it.n * it.weight + kItemCost;
   return it;
 }
@@ -451,7 +454,7 @@ __device__ __noinline__ int64_t head_cost(const Geometry ge, int P, int T) {
 __device__ __forceinline__ int cut_tile(const ItemInfo& it, int64_t start, int64_t x) {
   if (x <= start) return 0;
   if (x >= start + it.cost) return it.n;
-  const int t = static_cast<int>(x - start) >> (it.weight - 1);
+  const int t = static_cast<int>(x - start) / it.weight;
   if (t < kMinTiles) return 0;
   if (it.n - t < kMinTiles) return it.n;
   return t;
@@ -1013,7 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int part = whole ? -1 : 2 * static_cast<int>(blockIdx.x) + which;
             e[0] = r; e[1] = h; e[2] = mb; e[3] = P; e[4] = T;
             e[5] = __ldg(p.cu_seqlens_q + r);
-            e[6] = tb; e[7] = te - tb; e[8] = it.key_end; e[9] = it.weight == 2 ? 1 : 0;
+            e[6] = tb; e[7] = te - tb; e[8] = it.key_end; e[9] = it.two;
             e[10] = part; e[11] = 1;
             if (!whole) {
               PieceMeta* m = carve(p.workspace).meta + part;
