@@ -205,7 +205,7 @@ class JtTreeAttnFp8Params(ctypes.Structure):
                          "v_stride1 v_stride2 ks_stride0 ks_stride1 vs_stride0 vs_stride1")
         + _fields(ctypes.c_float, "scale")
         + _fields(c_i32, "num_requests total_queries num_kv_heads groups head_dim block_size "
-                         "table_width dtype out_dtype"))
+                         "table_width dtype out_dtype min_nodes max_nodes"))
 
 
 _lock = threading.Lock()

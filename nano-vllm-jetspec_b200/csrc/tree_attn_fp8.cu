@@ -62,6 +62,7 @@ constexpr int kTile16 = 2 * kTile8;   // bytes of a bf16 tile: two 64-dim halves
 constexpr int kHalf16 = kTile8;
 constexpr int kMaxCtas = 160;         // workspace slots are sized for this many SMs
 constexpr int kMaxNodes = 1024;
+constexpr int kFewRows = 16;          // requests with up to this many rows: tree_attn_fp8_few.cuh
 constexpr int kMaskWords = kMaxNodes / 32;
 // Costs of the work line: a key tile against one and against two query tiles, an item's fixed
 // cost (pipeline fill, first maxima, epilogue), and the least part worth a CTA of its own.  From
@@ -430,7 +431,7 @@ __device__ __forceinline__ ItemInfo item_info(const Geometry& ge, int P, int T, 
   it.cost = it.n * it.weight + kItemCost;
   return it;
 }
-// A request as the kernel takes it: no nodes when it has none or is refused.
+// A request as the kernels take it: no nodes when it has none or is refused.
 __device__ __noinline__ int2 load_request(const JtTreeAttnFp8Params& p, int r, bool flag) {
   int P = __ldg(p.prefix_lens + r), T = __ldg(p.node_counts + r);
   const int64_t capacity = static_cast<int64_t>(p.table_width) * p.block_size;
@@ -443,6 +444,11 @@ __device__ __noinline__ int2 load_request(const JtTreeAttnFp8Params& p, int r, b
     P = P < 0 ? 0 : static_cast<int>(capacity);
   }
   return make_int2(P, max(T, 0));
+}
+__device__ __forceinline__ int2 tree_request(const JtTreeAttnFp8Params& p, int r, bool flag) {
+  int2 q = load_request(p, r, flag);
+  if (q.y * p.groups <= kFewRows) q.y = 0;  // the other kernel's
+  return q;
 }
 __device__ __noinline__ int64_t head_cost(const Geometry ge, int P, int T) {
   int64_t c = 0;
@@ -717,6 +723,26 @@ __device__ __forceinline__ void store_columns(const JtTreeAttnFp8Params& p, int6
   }
 }
 
+// Four output columns of one row from its unnormalised sums.
+template <bool kWide>
+__device__ __forceinline__ void store_row4(const JtTreeAttnFp8Params& p, int q_start, int h, int row,
+                                           int d, float4 o, float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (l == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);  // the row sees no key
+  o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  const int node = row / p.groups;
+  const int64_t at = (static_cast<int64_t>(q_start) + node) * p.out_stride0 +
+                     (static_cast<int64_t>(h) * p.groups + row - node * p.groups) * p.out_stride1 + d;
+  if (kWide && p.out_dtype == JT_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = o;
+  } else {
+    const bool bf = !kWide || p.out_dtype == JT_BF16;
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+        bf ? make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w))
+           : make_uint2(jt::MmaOp<__half>::pack(o.x, o.y), jt::MmaOp<__half>::pack(o.z, o.w));
+  }
+}
+
 // Queries as e4m3 terms of row / 2^e and the rows' factors, for the attention kernel's TMA: half
 // a warp per row (16 bytes per lane), its largest magnitude by shuffles.  A kernel of its own
 // (the attention starts beside it as a programmatic dependent): inside, the split of a
@@ -842,7 +868,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int r_lo = min(tid * per, R), r_hi = min(r_lo + per, R);
   int64_t mine = 0;
   for (int r = r_lo; r < r_hi; ++r) {
-    const int2 q = load_request(p, r, blockIdx.x == 0);
+    const int2 q = tree_request(p, r, blockIdx.x == 0);
     mine += head_cost(ge, q.x, q.y) * p.num_kv_heads;
   }
   int64_t incl = mine;
@@ -867,7 +893,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (has_part && mine > 0 && my_start <= x0 && x0 < my_start + mine) {
     int64_t s = my_start;
     for (int r = r_lo; r < r_hi; ++r) {
-      const int2 q = load_request(p, r, false);
+      const int2 q = tree_request(p, r, false);
       const int64_t c = head_cost(ge, q.x, q.y) * p.num_kv_heads;
       if (x0 < s + c) {
         scan[32] = r;
@@ -988,7 +1014,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool more = has_part;
       int meta_valid[2] = {0, 0};
       if (lane == 0 && more) {
-        const int2 q = load_request(p, r, false);
+        const int2 q = tree_request(p, r, false);
         P = q.x;
         T = q.y;
         const int64_t ch = head_cost(ge, P, T);
@@ -1040,7 +1066,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 do {
                   ++r;
                   if (r < R) {
-                    const int2 q = load_request(p, r, false);
+                    const int2 q = tree_request(p, r, false);
                     P = q.x;
                     T = q.y;
                   }
@@ -1578,6 +1604,8 @@ int launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, size_t s
   return jt_cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), what);
 }
 
+#include "tree_attn_fp8_few.cuh"
+
 template <bool kWide, typename QT>
 int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
   LoadPlan plan{};
@@ -1592,6 +1620,15 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
       (!encode_pool(&kmap, p, p.k_pool, p.k_stride0, p.k_stride1, p.k_stride2, plan.box) ||
        !encode_pool(&vmap, p, p.v_pool, p.v_stride0, p.v_stride1, p.v_stride2, plan.box)))
     plan.tma = 0;  // a layout the encoder refuses: gathered like any other page size
+  // Requests of up to 16 rows and larger trees take kernels of their own; each skips the other's
+  // requests, and the host leaves out a kernel that it knows to be without any.
+  const int grid = std::min(sms, kMaxCtas);
+  const int64_t most = p.max_nodes > 0 ? static_cast<int64_t>(p.max_nodes) * p.groups : kFewRows + 1;
+  if (std::max(p.min_nodes, 1) * static_cast<int64_t>(p.groups) <= kFewRows) {
+    const int rc = most <= 8 ? launch_few<1, kWide, QT>(p, plan, kmap, vmap, grid, stream)
+                             : launch_few<2, kWide, QT>(p, plan, kmap, vmap, grid, stream);
+    if (rc != JT_OK || most <= kFewRows) return rc;
+  }
   const int64_t rows = static_cast<int64_t>(p.total_queries) * p.groups;
   CUtensorMap qmap{};
   if (!encode_queries(&qmap, carve(p.workspace, p.total_queries, p.groups, p.num_kv_heads).q_terms, rows,
@@ -1609,7 +1646,6 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
       p, static_cast<unsigned>(split));
   rc = jt_cuda_check(cudaGetLastError(), "tree_attn_fp8 query split launch");
   if (rc != JT_OK) return rc;
-  const int grid = std::min(sms, kMaxCtas);
   rc = launch_dependent(tree_attn_fp8_kernel<kWide>, dim3(grid), kThreads, Smem<kWide>::kBytes, stream,
                         "tree_attn_fp8 launch", p, kmap, vmap, qmap, plan);
   if (rc != JT_OK) return rc;

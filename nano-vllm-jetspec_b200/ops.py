@@ -172,13 +172,15 @@ def tree_attention_fp8_(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor
                         node_counts: torch.Tensor, block_tables: torch.Tensor,
                         tree_slots: torch.Tensor, qq_bias: torch.Tensor,
                         qq_bias_offsets: torch.Tensor, scale: float, groups: int) -> None:
+    # Without the host's node counts (which would be guards of the graph): the launch covers
+    # small and large trees.
     from .tree_fp8 import _launch_attention
 
     metadata = SimpleNamespace(
         cu_seqlens_q=cu_seqlens_q, query_to_request=query_to_request,
         query_local_row=query_local_row, prefix_lens=prefix_lens, node_counts=node_counts,
         block_tables=block_tables, tree_slots=tree_slots, qq_bias=qq_bias,
-        qq_bias_offsets=qq_bias_offsets)
+        qq_bias_offsets=qq_bias_offsets, node_counts_host=None)
     _launch_attention(out, q, k_pool, v_pool, k_scale, v_scale, metadata, scale, groups)
 
 

@@ -72,6 +72,15 @@ def packed_tree_attention_fp8(q, k_pool, v_pool, k_scale, v_scale, metadata, sca
     return out
 
 
+def _node_range(metadata) -> tuple[int, int]:
+    """Least (above zero) and largest node count, (0, 0) when the host does not know them."""
+    counts = getattr(metadata, "node_counts_host", None)
+    if not counts:
+        return 0, 0
+    low, high = min(counts), max(counts)
+    return low or min((c for c in counts if c), default=0), high
+
+
 def _launch_attention(out, q, k_pool, v_pool, k_scale, v_scale, m, scale, groups) -> None:
     """jt_tree_attn_fp8_launch on the current stream (validated arguments)."""
     lib = _lib.load_library()
@@ -99,5 +108,6 @@ def _launch_attention(out, q, k_pool, v_pool, k_scale, v_scale, m, scale, groups
         m.qq_bias_offsets.data_ptr(), scratch.data_ptr(), nbytes,
         blocks, qs[0], qs[1], os_[0], os_[1], m.block_tables.stride(0), ks[0], ks[1], ks[2],
         vs[0], vs[1], vs[2], kss[0], kss[1], vss[0], vss[1], scale, requests, total, kv_heads,
-        groups, dim, block_size, m.block_tables.shape[1], codes[q.dtype], codes[out.dtype])
+        groups, dim, block_size, m.block_tables.shape[1], codes[q.dtype], codes[out.dtype],
+        *_node_range(m))
     _lib.check(lib.jt_tree_attn_fp8_launch(ctypes.byref(p), stream))
