@@ -12,10 +12,11 @@
 // as NaN.
 //
 // Bound: HBM for long inputs (each byte read once, written once), a launch and two dependent
-// loads (position, cos / sin) for a decode round.  A head row is held by D / 8 lanes, each
-// with 4 elements of the first half and their rotation partners of the second, so the
+// loads (position, cos / sin) for a decode round.  A head row is held by D / 16 lanes, each
+// with 8 elements of the first half and their rotation partners of the second, so the
 // rotation needs no exchange and the norm (and the 8-bit maximum) is a few shuffles; a lane
-// group loads kRows rows before it computes any, to keep enough bytes in flight.
+// group takes four heads of a token, which keeps enough bytes in flight and reads the
+// position, cos / sin and weights once for the four.
 #include <algorithm>
 
 #include "common.cuh"
@@ -57,36 +58,59 @@ __device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
   return __half2float(__ldg(static_cast<const __half*>(p) + i));
 }
 
-// Four consecutive elements as loaded (8 or 16 bytes).
+// Eight consecutive elements as loaded (16 or 32 bytes), 16-byte aligned.
 template <typename T>
-struct Quad {
+struct Oct {
   static_assert(sizeof(T) == 2, "16-bit operands");
-  uint2 raw;
-  __device__ __forceinline__ void load(const T* p) { raw = __ldcs(reinterpret_cast<const uint2*>(p)); }
-  __device__ __forceinline__ void unpack(float (&f)[4]) const {
+  uint4 raw;
+  __device__ __forceinline__ void load(const T* p) { raw = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void unpack(float (&f)[8]) const {
     const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = to_f<T>(e[i]);
+    for (int i = 0; i < 8; ++i) f[i] = to_f<T>(e[i]);
   }
-  __device__ __forceinline__ static void store(T* p, const float (&f)[4]) {
-    uint2 v;
+  __device__ __forceinline__ static void store(T* p, const float (&f)[8]) {
+    uint4 v;
     T* e = reinterpret_cast<T*>(&v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = from_f<T>(f[i]);
-    *reinterpret_cast<uint2*>(p) = v;
+    for (int i = 0; i < 8; ++i) e[i] = from_f<T>(f[i]);
+    *reinterpret_cast<uint4*>(p) = v;
   }
 };
 template <>
-struct Quad<float> {
-  float4 raw;
-  __device__ __forceinline__ void load(const float* p) { raw = __ldcs(reinterpret_cast<const float4*>(p)); }
-  __device__ __forceinline__ void unpack(float (&f)[4]) const {
-    f[0] = raw.x; f[1] = raw.y; f[2] = raw.z; f[3] = raw.w;
+struct Oct<float> {
+  float4 lo, hi;
+  __device__ __forceinline__ void load(const float* p) {
+    lo = __ldcs(reinterpret_cast<const float4*>(p));
+    hi = __ldcs(reinterpret_cast<const float4*>(p) + 1);
   }
-  __device__ __forceinline__ static void store(float* p, const float (&f)[4]) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  __device__ __forceinline__ void unpack(float (&f)[8]) const {
+    f[0] = lo.x; f[1] = lo.y; f[2] = lo.z; f[3] = lo.w;
+    f[4] = hi.x; f[5] = hi.y; f[6] = hi.z; f[7] = hi.w;
+  }
+  __device__ __forceinline__ static void store(float* p, const float (&f)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
   }
 };
+// Eight weights or cosines of any type.
+__device__ __forceinline__ void load_any8(const void* p, int64_t i, int dtype, float (&f)[8]) {
+  if (dtype == JT_F32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 a = __ldg(q), b = __ldg(q + 1);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = dtype == JT_BF16 ? jt::MmaOp<__nv_bfloat16>::unpack(w[k]) : jt::MmaOp<__half>::unpack(w[k]);
+      f[2 * k] = x.x;
+      f[2 * k + 1] = x.y;
+    }
+  }
+}
 
 // Scale exponent of an 8-bit row from its largest magnitude (finite): the smallest e with
 // amax <= 448 * 2^e, read off the float's fields (448 = 1.75 * 2^8); 0 for a row of zeros,
@@ -106,8 +130,9 @@ __device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint32_t pack_e4m3x4(const float (&f)[4], float s) {
-  return pack_e4m3(f[0] * s, f[1] * s) | (pack_e4m3(f[2] * s, f[3] * s) << 16);
+__device__ __forceinline__ uint2 pack_e4m3x8(const float (&f)[8], float s) {
+  return make_uint2(pack_e4m3(f[0] * s, f[1] * s) | (pack_e4m3(f[2] * s, f[3] * s) << 16),
+                    pack_e4m3(f[4] * s, f[5] * s) | (pack_e4m3(f[6] * s, f[7] * s) << 16));
 }
 
 // Where one row comes from and goes to.
@@ -165,135 +190,126 @@ __device__ __forceinline__ int64_t cache_row(const JtQkNormRopeParams& p, int64_
   return position * p.cache_stride0;
 }
 
-template <typename T, int D, int MODE, int kRows>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const JtQkNormRopeParams p) {
-  constexpr int L = D / 8;                  // lanes per row
-  constexpr int kGroups = kThreads / L;     // lane groups per CTA
-  const int group = threadIdx.x / L, l = threadIdx.x % L;
-  const int heads = p.q_heads + p.kv_heads * (MODE == kStoreNone ? 1 : 2);
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * (kGroups * kRows) + group;
-  const int c1 = 4 * l, c2 = D / 2 + 4 * l;
-
-  Row row[kRows];
-  Quad<T> x1[kRows], x2[kRows];
-  float4 co[kRows], si[kRows];
+// C heads of one kind (0 query, 1 key, 2 value) of one token by a group of D / 16 lanes: all
+// their loads first, then row after row.  Position, slot, cos / sin and weights are read once
+// for the C rows.
+template <typename T, int D, int MODE, int C, int KIND>
+__device__ __forceinline__ void norm_unit(const JtQkNormRopeParams& p, int64_t token, int head0,
+                                          bool live, int l) {
+  constexpr int L = D / 16;
+  const int heads = KIND == 0 ? p.q_heads : p.kv_heads;
+  const int c1 = 8 * l, c2 = D / 2 + 8 * l;
+  const T* src = KIND == 0   ? static_cast<const T*>(p.q) + token * p.q_stride0
+                 : KIND == 1 ? static_cast<const T*>(p.k) + token * p.k_stride0
+                             : static_cast<const T*>(p.v) + token * p.v_stride0;
+  const int64_t head_stride = KIND == 0 ? p.q_stride1 : KIND == 1 ? p.k_stride1 : p.v_stride1;
+  Oct<T> x1[C], x2[C];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    row[i] = decode_row(p, base + i * kGroups, heads);
-    if (row[i].kind >= 0) {
-      const T* src = source_row<T>(p, row[i]);
-      x1[i].load(src + c1);
-      x2[i].load(src + c2);
-    }
+  for (int i = 0; i < C; ++i) {
+    const T* row = src + min(head0 + i, heads - 1) * head_stride;
+    x1[i].load(row + c1);
+    x2[i].load(row + c2);
+  }
+  int64_t page = -1, offset = 0;
+  if (MODE != kStoreNone && KIND >= 1) cache_place(p, token, page, offset);
+  float co[8], si[8], w1[8], w2[8];
+  if constexpr (KIND < 2) {
+    const int64_t cr = cache_row(p, token);
+    load_any8(p.cos_sin_cache, cr + c1, p.cache_dtype, co);
+    load_any8(p.cos_sin_cache, cr + c2, p.cache_dtype, si);
+    const void* weight = KIND == 0 ? p.q_weight : p.k_weight;
+    load_any8(weight, c1, p.weight_dtype, w1);
+    load_any8(weight, c2, p.weight_dtype, w2);
   }
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    co[i] = make_float4(1.f, 1.f, 1.f, 1.f);
-    si[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row[i].kind == 0 || row[i].kind == 1) {
-      const int64_t cr = cache_row(p, row[i].token);
-      if (p.cache_dtype == JT_F32) {
-        const float* c = static_cast<const float*>(p.cos_sin_cache) + cr;
-        co[i] = __ldg(reinterpret_cast<const float4*>(c + c1));
-        si[i] = __ldg(reinterpret_cast<const float4*>(c + c2));
-      } else {
-        co[i] = make_float4(load_any(p.cos_sin_cache, cr + c1, p.cache_dtype),
-                            load_any(p.cos_sin_cache, cr + c1 + 1, p.cache_dtype),
-                            load_any(p.cos_sin_cache, cr + c1 + 2, p.cache_dtype),
-                            load_any(p.cos_sin_cache, cr + c1 + 3, p.cache_dtype));
-        si[i] = make_float4(load_any(p.cos_sin_cache, cr + c2, p.cache_dtype),
-                            load_any(p.cos_sin_cache, cr + c2 + 1, p.cache_dtype),
-                            load_any(p.cos_sin_cache, cr + c2 + 2, p.cache_dtype),
-                            load_any(p.cos_sin_cache, cr + c2 + 3, p.cache_dtype));
-      }
-    }
-  }
-  float wq[8], wk[8];
+  for (int i = 0; i < C; ++i) {
+    const int head = head0 + i;
+    const bool ok = live && head < heads;
+    float a[8], b[8];
+    x1[i].unpack(a);
+    x2[i].unpack(b);
+    if constexpr (KIND < 2) {
+      float ss = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    wq[e] = load_any(p.q_weight, c1 + e, p.weight_dtype);
-    wq[4 + e] = load_any(p.q_weight, c2 + e, p.weight_dtype);
-    wk[e] = load_any(p.k_weight, c1 + e, p.weight_dtype);
-    wk[4 + e] = load_any(p.k_weight, c2 + e, p.weight_dtype);
-  }
+      for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + b[e] * b[e];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const Row& r = row[i];
-    float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (r.kind >= 0) {
-      x1[i].unpack(a);
-      x2[i].unpack(b);
-    }
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ss += a[e] * a[e] + b[e] * b[e];
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (r.kind == 0 || r.kind == 1) {
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       const float inv = 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
-      const float c[4] = {co[i].x, co[i].y, co[i].z, co[i].w};
-      const float s[4] = {si[i].x, si[i].y, si[i].z, si[i].w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float y1 = a[e] * inv * (r.kind == 0 ? wq[e] : wk[e]);
-        const float y2 = b[e] * inv * (r.kind == 0 ? wq[4 + e] : wk[4 + e]);
-        a[e] = y1 * c[e] - y2 * s[e];
-        b[e] = y2 * c[e] + y1 * s[e];
+      for (int e = 0; e < 8; ++e) {
+        const float y1 = a[e] * inv * w1[e];
+        const float y2 = b[e] * inv * w2[e];
+        a[e] = y1 * co[e] - y2 * si[e];
+        b[e] = y2 * co[e] + y1 * si[e];
       }
     }
-    if constexpr (MODE == kStoreFp8) {
+    if constexpr (MODE == kStoreFp8 && KIND >= 1) {
       // The largest magnitude's bits order like the value, infinities and NaN above all.
       uint32_t m = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 8; ++e)
         m = max(m, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(b[e]) & 0x7fffffffu));
 #pragma unroll
       for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (r.kind >= 1) {
-        int64_t page, offset;
-        cache_place(p, r.token, page, offset);
-        if (page >= 0) {
-          const bool is_k = r.kind == 1;
-          const bool finite = m < 0x7f800000u;
-          const int e = finite ? scale_exponent(__uint_as_float(m)) : 0;
-          const float s = exp2_neg(e);
-          uint8_t* dst = is_k ? static_cast<uint8_t*>(p.k_pool) + page * p.kp_stride0 +
-                                    offset * p.kp_stride1 + r.head * p.kp_stride2
-                              : static_cast<uint8_t*>(p.v_pool) + page * p.vp_stride0 +
-                                    offset * p.vp_stride1 + r.head * p.vp_stride2;
-          *reinterpret_cast<uint32_t*>(dst + c1) = finite ? pack_e4m3x4(a, s) : 0u;
-          *reinterpret_cast<uint32_t*>(dst + c2) = finite ? pack_e4m3x4(b, s) : 0u;
-          if (l == 0) {
-            uint8_t* sc = is_k ? static_cast<uint8_t*>(p.k_scale) + page * p.ks_stride0 +
-                                     r.head * p.ks_stride1 + offset
-                               : static_cast<uint8_t*>(p.v_scale) + page * p.vs_stride0 +
-                                     r.head * p.vs_stride1 + offset;
-            *sc = finite ? static_cast<uint8_t>(e + 127) : 255;
-          }
+      if (ok && page >= 0) {
+        const bool finite = m < 0x7f800000u;
+        const int e = finite ? scale_exponent(__uint_as_float(m)) : 0;
+        const float s = exp2_neg(e);
+        uint8_t* dst = KIND == 1 ? static_cast<uint8_t*>(p.k_pool) + page * p.kp_stride0 +
+                                       offset * p.kp_stride1 + head * p.kp_stride2
+                                 : static_cast<uint8_t*>(p.v_pool) + page * p.vp_stride0 +
+                                       offset * p.vp_stride1 + head * p.vp_stride2;
+        *reinterpret_cast<uint2*>(dst + c1) = finite ? pack_e4m3x8(a, s) : make_uint2(0u, 0u);
+        *reinterpret_cast<uint2*>(dst + c2) = finite ? pack_e4m3x8(b, s) : make_uint2(0u, 0u);
+        if (l == 0) {
+          uint8_t* sc = KIND == 1 ? static_cast<uint8_t*>(p.k_scale) + page * p.ks_stride0 +
+                                        head * p.ks_stride1 + offset
+                                  : static_cast<uint8_t*>(p.v_scale) + page * p.vs_stride0 +
+                                        head * p.vs_stride1 + offset;
+          *sc = finite ? static_cast<uint8_t>(e + 127) : 255;
         }
       }
-    }
-    if (r.kind == 0) {
-      T* dst = static_cast<T*>(p.q_out) + r.token * p.qo_stride0 + r.head * p.qo_stride1;
-      Quad<T>::store(dst + c1, a);
-      Quad<T>::store(dst + c2, b);
-    } else if (MODE == kStoreNone && r.kind == 1) {
-      T* dst = static_cast<T*>(p.k_out) + r.token * p.ko_stride0 + r.head * p.ko_stride1;
-      Quad<T>::store(dst + c1, a);
-      Quad<T>::store(dst + c2, b);
-    } else if (MODE == kStoreSame && r.kind >= 1) {
-      int64_t page, offset;
-      cache_place(p, r.token, page, offset);
-      if (page >= 0) {
-        T* dst = r.kind == 1 ? static_cast<T*>(p.k_pool) + page * p.kp_stride0 +
-                                   offset * p.kp_stride1 + r.head * p.kp_stride2
-                             : static_cast<T*>(p.v_pool) + page * p.vp_stride0 +
-                                   offset * p.vp_stride1 + r.head * p.vp_stride2;
-        Quad<T>::store(dst + c1, a);  // V: the loaded values, unchanged
-        Quad<T>::store(dst + c2, b);
+    } else {
+      T* dst = nullptr;
+      if (KIND == 0)
+        dst = static_cast<T*>(p.q_out) + token * p.qo_stride0 + head * p.qo_stride1;
+      else if (MODE == kStoreNone)
+        dst = static_cast<T*>(p.k_out) + token * p.ko_stride0 + head * p.ko_stride1;
+      else if (page >= 0)
+        dst = KIND == 1 ? static_cast<T*>(p.k_pool) + page * p.kp_stride0 + offset * p.kp_stride1 +
+                              head * p.kp_stride2
+                        : static_cast<T*>(p.v_pool) + page * p.vp_stride0 + offset * p.vp_stride1 +
+                              head * p.vp_stride2;
+      if (ok && dst != nullptr) {
+        Oct<T>::store(dst + c1, a);  // V: the loaded values, unchanged
+        Oct<T>::store(dst + c2, b);
       }
     }
   }
+}
+
+template <typename T, int D, int MODE, int C>
+__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const JtQkNormRopeParams p,
+                                                                unsigned q_blocks, unsigned k_blocks) {
+  constexpr int L = D / 16;              // lanes per row
+  constexpr int kGroups = kThreads / L;  // lane groups per CTA
+  const int group = threadIdx.x / L, l = threadIdx.x % L;
+  // A CTA's rows are of one kind.
+  const int kind = blockIdx.x < q_blocks ? 0 : blockIdx.x < q_blocks + k_blocks ? 1 : 2;
+  const unsigned block = blockIdx.x - (kind == 0 ? 0u : kind == 1 ? q_blocks : q_blocks + k_blocks);
+  const int heads = kind == 0 ? p.q_heads : p.kv_heads;
+  const unsigned chunks = (heads + C - 1) / C;
+  const uint64_t unit = static_cast<uint64_t>(block) * kGroups + group;
+  uint64_t token = unit < 0x80000000u ? static_cast<uint32_t>(unit) / chunks : unit / chunks;
+  const int head0 = static_cast<int>(unit - token * chunks) * C;
+  const bool live = token < static_cast<uint64_t>(p.rows);
+  if (!live) token = p.rows - 1;  // takes part in the shuffles, writes nothing
+  if (kind == 0)
+    norm_unit<T, D, MODE, C, 0>(p, token, head0, live, l);
+  else if (kind == 1)
+    norm_unit<T, D, MODE, C, 1>(p, token, head0, live, l);
+  else
+    norm_unit<T, D, MODE, C, 2>(p, token, head0, live, l);
 }
 
 // Any even head dim up to 512 and any alignment: one warp per row, element by element.
@@ -389,37 +405,42 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_any_kernel(const JtQkNo
 
 bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-// Four-element accesses need bases and row strides on four elements (16 bytes for the fp32
-// cos / sin cache; four bytes for 8-bit rows).
+// Eight-element accesses need 16-byte bases and row strides (8 bytes for 8-bit rows).
 bool vector_ok(const JtQkNormRopeParams& p) {
   if (p.head_dim != 64 && p.head_dim != 128 && p.head_dim != 256) return false;
-  const int quad = p.dtype == JT_F32 ? 16 : 8;
-  if (!aligned(p.q, quad) || !aligned(p.k, quad) || !aligned(p.q_out, quad) ||
-      (p.q_stride0 | p.q_stride1 | p.k_stride0 | p.k_stride1 | p.qo_stride0 | p.qo_stride1) % 4 != 0)
+  const int step = p.dtype == JT_F32 ? 4 : 8;
+  if (!aligned(p.q, 16) || !aligned(p.k, 16) || !aligned(p.q_out, 16) || !aligned(p.q_weight, 16) ||
+      !aligned(p.k_weight, 16) || !aligned(p.cos_sin_cache, 16) ||
+      p.cache_stride0 % (p.cache_dtype == JT_F32 ? 4 : 8) != 0 ||
+      (p.q_stride0 | p.q_stride1 | p.k_stride0 | p.k_stride1 | p.qo_stride0 | p.qo_stride1) % step != 0)
     return false;
-  if (p.cache_dtype == JT_F32 && (!aligned(p.cos_sin_cache, 16) || p.cache_stride0 % 4 != 0))
-    return false;
-  if (p.store == kStoreNone)
-    return aligned(p.k_out, quad) && (p.ko_stride0 | p.ko_stride1) % 4 == 0;
-  const int pool = p.store == kStoreFp8 ? 4 : quad;
-  return aligned(p.v, quad) && (p.v_stride0 | p.v_stride1) % 4 == 0 && aligned(p.k_pool, pool) &&
+  if (p.store == kStoreNone) return aligned(p.k_out, 16) && (p.ko_stride0 | p.ko_stride1) % step == 0;
+  const int pool = p.store == kStoreFp8 ? 8 : 16, pool_step = p.store == kStoreFp8 ? 8 : step;
+  return aligned(p.v, 16) && (p.v_stride0 | p.v_stride1) % step == 0 && aligned(p.k_pool, pool) &&
          aligned(p.v_pool, pool) &&
          (p.kp_stride0 | p.kp_stride1 | p.kp_stride2 | p.vp_stride0 | p.vp_stride1 |
-          p.vp_stride2) % 4 == 0;
+          p.vp_stride2) % pool_step == 0;
+}
+
+template <typename T, int D, int MODE, int C>
+void launch_chunks(const JtQkNormRopeParams& p, cudaStream_t stream) {
+  constexpr int kGroups = kThreads / (D / 16);
+  auto blocks = [&](int heads) {
+    return static_cast<unsigned>((p.rows * ((heads + C - 1) / C) + kGroups - 1) / kGroups);
+  };
+  const unsigned q = blocks(p.q_heads), k = blocks(p.kv_heads);
+  qk_norm_rope_kernel<T, D, MODE, C><<<q + k * (MODE == kStoreNone ? 1 : 2), kThreads, 0, stream>>>(p, q, k);
 }
 
 template <typename T, int D, int MODE>
 void launch_vector(const JtQkNormRopeParams& p, int64_t rows, int sms, cudaStream_t stream) {
-  constexpr int kGroups = kThreads / (D / 8);
-  // Four rows per lane group once they still give every SM two CTAs: below that a row each,
+  constexpr int kGroups = kThreads / (D / 16), C = sizeof(T) == 2 ? 4 : 2;
+  // C heads per lane group once they still give every SM two CTAs: below that a head each,
   // spread over more SMs, answers sooner.
-  if (rows >= 2LL * sms * kGroups * 4) {
-    const int64_t grid = (rows + kGroups * 4 - 1) / (kGroups * 4);
-    qk_norm_rope_kernel<T, D, MODE, 4><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
-  } else {
-    const int64_t grid = (rows + kGroups - 1) / kGroups;
-    qk_norm_rope_kernel<T, D, MODE, 1><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
-  }
+  if (rows >= 2LL * sms * kGroups * C)
+    launch_chunks<T, D, MODE, C>(p, stream);
+  else
+    launch_chunks<T, D, MODE, 1>(p, stream);
 }
 
 template <typename T, int MODE>
