@@ -4,11 +4,14 @@
 //   kv_scale [2, L, blocks, H, B] bytes:     dst <- src
 // A pure copy with every read of a plane before any write to it, so that overlapping slot
 // sets behave like a gather followed by a scatter.  A plane is one (axis, layer, head, chunk
-// of W 16-byte words of the head row) over every slot; one CTA gathers it into shared memory,
-// synchronises and scatters it.  Planes cover disjoint bytes: no CTA waits for another.
+// of W 16-byte words of the head row) over every slot; a CTA, or for many slots a cluster of
+// CTAs with a part of the slots each, gathers it into shared memory, meets at the cluster's
+// barrier and scatters it.  Planes cover disjoint bytes: no cluster waits for another.
 //
-// Bound: HBM (each 32-byte sector read and written once: W >= 2 keeps sectors whole), and for
-// small rounds the launch and two dependent loads (slot, row).
+// Bound: HBM (whole 128-byte rows read and written once), and for small rounds the launch and
+// two dependent loads (slot, row).  The rows are gathered by cp.async, a plane in flight at a
+// time, and a CTA's staging is kept below 40 KB so that several share an SM and one's gather
+// overlaps another's scatter.
 #include <algorithm>
 
 #include "common.cuh"
@@ -18,41 +21,50 @@ namespace {
 __device__ uint32_t g_fp8_commit_errors;
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;
-constexpr int kSmemCap = 200 * 1024;
-// A wider chunk is taken while the staging stays below this, so that several CTAs share an
-// SM and one's gather overlaps another's scatter.
-constexpr int kSmemShare = 72 * 1024;
+constexpr int kSmemCap = 220 * 1024;
+constexpr int kSmemShare = 40 * 1024;
+constexpr int kMaxCluster = 8;
+constexpr int kSlotBytes = 17;  // (page, offset) of source and destination, the scale byte
+constexpr int kMaxSlots = 200 * 1024 / 17;
+static_assert((kMaxSlots + kMaxCluster - 1) / kMaxCluster * (8 * 16 + kSlotBytes) <= kSmemCap,
+              "the largest cluster stages every slot");
 
 __device__ __forceinline__ int64_t load_slot(const void* base, int is64, int64_t i) {
   return is64 ? __ldg(static_cast<const int64_t*>(base) + i)
               : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(base) + i));
 }
 
-struct Place {
-  int64_t page, offset;
-  bool ok;
-};
-__device__ __forceinline__ Place place(const JtKvFp8CommitParams& p, const void* slots, int s) {
+// Page and offset of a slot, page -1 outside the pool.
+__device__ __forceinline__ int2 place(const JtKvFp8CommitParams& p, const void* slots, int s) {
   const int64_t slot = load_slot(slots, p.slot_is_int64, s);
-  Place r;
-  r.ok = slot >= 0 && slot < p.num_blocks * static_cast<int64_t>(p.block_size);
-  if (slot >= 0 && slot < 0x7fffffff) {  // 32-bit division for every pool in use
-    r.page = static_cast<uint32_t>(slot) / static_cast<uint32_t>(p.block_size);
-  } else {
-    r.page = slot / p.block_size;
+  if (slot < 0 || slot >= p.num_blocks * static_cast<int64_t>(p.block_size)) {
+    atomicOr(&g_fp8_commit_errors, JT_DEVERR_OUT_OF_RANGE);
+    return make_int2(-1, 0);
   }
-  r.offset = slot - r.page * p.block_size;
-  return r;
+  // 32-bit division for every pool in use.
+  const int64_t page = slot < 0x7fffffff
+                           ? static_cast<int64_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(p.block_size))
+                           : slot / p.block_size;
+  return make_int2(static_cast<int>(page), static_cast<int>(slot - page * p.block_size));
 }
 
 template <int W>
 __global__ void __launch_bounds__(kThreads) kv_fp8_commit_kernel(const JtKvFp8CommitParams p,
-                                                                 int planes, int chunks) {
-  extern __shared__ __align__(16) int4 staging[];
-  const int n = p.num_slots, units = n * W;
-  uint8_t* bytes = reinterpret_cast<uint8_t*>(staging + units);
-  for (int plane = blockIdx.x; plane < planes; plane += gridDim.x) {
+                                                                 int planes, int chunks, int per) {
+  extern __shared__ __align__(16) int4 staging[];  // [per][W], then [per] places, [per] bytes
+  int4* places = staging + per * W;                // source page, offset, destination page, offset
+  uint8_t* bytes = reinterpret_cast<uint8_t*>(places + per);
+  uint32_t rank, cluster;
+  asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctaid.x;\n" : "=r"(cluster));
+  const int lo = static_cast<int>(rank) * per, n = max(0, min(per, p.num_slots - lo));
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int2 s = place(p, p.source_slots, lo + i), d = place(p, p.destination_slots, lo + i);
+    const bool ok = s.x >= 0 && d.x >= 0;
+    places[i] = make_int4(ok ? s.x : -1, s.y, d.x, d.y);
+  }
+  __syncthreads();
+  for (int plane = blockIdx.x / cluster; plane < planes; plane += gridDim.x / cluster) {
     const int chunk = plane % chunks;
     int rest = plane / chunks;
     const int head = rest % p.num_kv_heads;
@@ -62,63 +74,64 @@ __global__ void __launch_bounds__(kThreads) kv_fp8_commit_kernel(const JtKvFp8Co
                  head * p.stride_head + chunk * (W * 16);
     uint8_t* scales = static_cast<uint8_t*>(p.kv_scale) + axis * p.scale_axis +
                       layer * p.scale_layer + head * p.scale_head;
-    for (int base = threadIdx.x; base < units; base += kThreads * kUnroll) {
-      int4 v[kUnroll];
-#pragma unroll
-      for (int k = 0; k < kUnroll; ++k) {
-        const int i = base + k * kThreads;
-        v[k] = make_int4(0, 0, 0, 0);
-        if (i < units) {
-          const Place s = place(p, p.source_slots, i / W);
-          if (s.ok)
-            v[k] = *reinterpret_cast<const int4*>(rows + s.page * p.stride_block +
-                                                  s.offset * p.stride_offset + (i % W) * 16);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kUnroll; ++k)
-        if (base + k * kThreads < units) staging[base + k * kThreads] = v[k];
+    for (int i = threadIdx.x; i < n * W; i += kThreads) {
+      const int4 at = places[i / W];
+      if (at.x >= 0)
+        jt::cp_async_16(jt::smem_u32(staging + i),
+                        rows + at.x * p.stride_block + at.y * p.stride_offset + (i % W) * 16, 16);
     }
     if (chunk == 0)
       for (int i = threadIdx.x; i < n; i += kThreads) {
-        const Place s = place(p, p.source_slots, i);
-        if (s.ok)
-          bytes[i] = scales[s.page * p.scale_block + s.offset];
-        else
-          atomicOr(&g_fp8_commit_errors, JT_DEVERR_OUT_OF_RANGE);
+        const int4 at = places[i];
+        if (at.x >= 0) bytes[i] = scales[at.x * p.scale_block + at.y];
       }
-    __syncthreads();  // every read of this plane precedes every write to it
-    for (int i = threadIdx.x; i < units; i += kThreads) {
-      const Place s = place(p, p.source_slots, i / W), d = place(p, p.destination_slots, i / W);
-      if (s.ok && d.ok)
-        *reinterpret_cast<int4*>(rows + d.page * p.stride_block + d.offset * p.stride_offset +
-                                 (i % W) * 16) = staging[i];
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+    // Every read of this plane precedes every write to it.
+    if (cluster > 1) {
+      asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    } else {
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < n * W; i += kThreads) {
+      const int4 at = places[i / W];
+      if (at.x >= 0)
+        *reinterpret_cast<int4*>(rows + at.z * p.stride_block + at.w * p.stride_offset + (i % W) * 16) = staging[i];
     }
     if (chunk == 0)
       for (int i = threadIdx.x; i < n; i += kThreads) {
-        const Place s = place(p, p.source_slots, i), d = place(p, p.destination_slots, i);
-        if (s.ok && d.ok)
-          scales[d.page * p.scale_block + d.offset] = bytes[i];
-        else if (!d.ok)
-          atomicOr(&g_fp8_commit_errors, JT_DEVERR_OUT_OF_RANGE);
+        const int4 at = places[i];
+        if (at.x >= 0) scales[at.z * p.scale_block + at.w] = bytes[i];
       }
     __syncthreads();  // the staging is free for the next plane
   }
 }
 
+int staging_bytes(int per, int w) { return per * (w * 16 + kSlotBytes); }
+
 template <int W>
-int launch(const JtKvFp8CommitParams& p, int sms, cudaStream_t stream) {
+int launch(const JtKvFp8CommitParams& p, int cluster, int sms, cudaStream_t stream) {
   const int chunks = p.head_dim / (16 * W);
   const int64_t planes = 2LL * p.num_layers * p.num_kv_heads * chunks;
   if (planes > 0x7fffffff) return jt_fail(JT_ERR_INVALID, "kv_fp8_commit: too many planes");
-  const int smem = p.num_slots * (W * 16 + 1);
+  const int per = (p.num_slots + cluster - 1) / cluster;
   int rc = jt_cuda_check(cudaFuncSetAttribute(kv_fp8_commit_kernel<W>,
                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemCap),
                          "kv_fp8_commit smem attribute");
   if (rc != JT_OK) return rc;
-  const int grid = static_cast<int>(std::min<int64_t>(planes, 16LL * sms));
-  kv_fp8_commit_kernel<W><<<grid, kThreads, smem, stream>>>(p, static_cast<int>(planes), chunks);
-  return jt_cuda_check(cudaGetLastError(), "kv_fp8_commit launch");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(planes, 16LL * sms) * cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = staging_bytes(per, W);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return jt_cuda_check(cudaLaunchKernelEx(&cfg, kv_fp8_commit_kernel<W>, p, static_cast<int>(planes),
+                                          chunks, per),
+                       "kv_fp8_commit launch");
 }
 
 }  // namespace
@@ -132,12 +145,14 @@ int jt_read_errors_fp8_commit(uint32_t* bits) {
                        "clear fp8 commit error word");
 }
 
-extern "C" int32_t jt_kv_fp8_commit_max_slots(void) { return kSmemCap / 17; }
+extern "C" int32_t jt_kv_fp8_commit_max_slots(void) {
+  return kMaxSlots;
+}
 
 extern "C" int jt_kv_fp8_commit_launch(const JtKvFp8CommitParams* p, cudaStream_t stream) {
   if (p == nullptr) return jt_fail(JT_ERR_INVALID, "kv_fp8_commit: null params");
   if (p->num_slots < 0 || p->num_layers < 1 || p->num_kv_heads < 1 || p->head_dim < 16 ||
-      p->head_dim % 16 != 0 || p->block_size < 1 || p->num_blocks < 1)
+      p->head_dim % 16 != 0 || p->block_size < 1 || p->num_blocks < 1 || p->num_blocks > 0x7fffffff)
     return jt_fail(JT_ERR_INVALID, "kv_fp8_commit: invalid geometry");
   if (p->num_slots == 0) return JT_OK;
   if (p->num_slots > jt_kv_fp8_commit_max_slots())
@@ -154,11 +169,17 @@ extern "C" int jt_kv_fp8_commit_launch(const JtKvFp8CommitParams* p, cudaStream_
   rc = jt_cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev),
                      "SM count");
   if (rc != JT_OK) return rc;
+  // Whole 128-byte chunks (the widest that divide the row), by the smallest cluster whose CTAs
+  // stage little enough to share an SM; the largest cluster may fill it.
   const int words = p->head_dim / 16;
-  const int64_t n = p->num_slots;
-  for (int w : {8, 4, 2})
-    if (words % w == 0 && n * (w * 16 + 1) <= kSmemShare)
-      return w == 8 ? launch<8>(*p, sms, stream)
-                    : w == 4 ? launch<4>(*p, sms, stream) : launch<2>(*p, sms, stream);
-  return launch<1>(*p, sms, stream);
+  const int w = words % 8 == 0 ? 8 : words % 4 == 0 ? 4 : words % 2 == 0 ? 2 : 1;
+  int cluster = 1;
+  while (cluster < kMaxCluster && staging_bytes((p->num_slots + cluster - 1) / cluster, w) > kSmemShare)
+    cluster *= 2;
+  switch (w) {
+    case 8: return launch<8>(*p, cluster, sms, stream);
+    case 4: return launch<4>(*p, cluster, sms, stream);
+    case 2: return launch<2>(*p, cluster, sms, stream);
+    default: return launch<1>(*p, cluster, sms, stream);
+  }
 }
