@@ -41,11 +41,12 @@ def check_layer(k_pool, v_pool, k_scale, v_scale) -> None:
     if k_scale.dtype != SCALE_DTYPE or v_scale.dtype != SCALE_DTYPE:
         raise ValueError("scales must be float8_e8m0fnu")
     blocks, block_size, heads, _ = k_pool.shape
-    if k_scale.shape != (blocks, heads, block_size) or v_scale.shape != k_scale.shape:
+    shape, device = (blocks, heads, block_size), k_pool.device
+    if k_scale.shape != shape or v_scale.shape != shape:
         raise ValueError("scales must be [pages, kv_heads, page_size]")
     if k_scale.stride(2) != 1 or v_scale.stride(2) != 1:
         raise ValueError("scales need a contiguous last dimension")
-    if k_scale.device != k_pool.device or v_scale.device != k_pool.device:
+    if k_scale.device != device or v_scale.device != device:
         raise ValueError("pools and scales must share one device")
 
 
@@ -84,15 +85,16 @@ def copy_accepted_kv_fp8(kv_pool: torch.Tensor, kv_scale: torch.Tensor,
     if n == 0:
         return 0
     device = kv_pool.device
-    if not kv_pool.is_cuda or any(t.device != device
-                                  for t in (kv_scale, source_slots, destination_slots)):
+    if (not kv_pool.is_cuda or kv_scale.device != device or source_slots.device != device
+            or destination_slots.device != device):
         raise ValueError("KV commit requires the pool, scales and slot maps on one CUDA device")
     if source_slots.dtype not in (torch.int32, torch.int64):
         raise ValueError("slot maps must be int32 or int64")
     if kv_pool.stride(5) != 1 or kv_scale.stride(4) != 1:
         raise ValueError("KV pool rows and scales need a contiguous last dimension")
-    destination_slots = destination_slots.to(source_slots.dtype).contiguous()
-    source_slots = source_slots.contiguous()
+    if destination_slots.dtype != source_slots.dtype:
+        destination_slots = destination_slots.to(source_slots.dtype)
+    destination_slots, source_slots = destination_slots.contiguous(), source_slots.contiguous()
     from . import ops
 
     if ops.compiling():

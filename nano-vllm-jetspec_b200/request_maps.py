@@ -64,10 +64,10 @@ def build_request_maps(block_tables: torch.Tensor, cached_lens: torch.Tensor,
             or not free_pages.is_contiguous() or block_tables.stride(1) != 1
             or block_tables.stride(0) < block_tables.shape[1]):
         raise ValueError("lengths, free pages and table rows must be contiguous")
-    wide = torch.empty((2, max_tokens), dtype=torch.int64, device=device)
-    narrow = torch.empty(max_tokens + 2 * requests + 2, dtype=i32, device=device)
-    slots, positions = wide.unbind(0)
-    owners, cu, lens, taken = narrow.split((max_tokens, requests + 1, requests, 1))
+    slots, positions = torch.empty((2, max_tokens), dtype=torch.int64, device=device).unbind(0)
+    owners, cu, lens, taken = torch.empty(
+        max_tokens + 2 * requests + 2, dtype=i32, device=device).split_with_sizes(
+            (max_tokens, requests + 1, requests, 1))
     maps = RequestMaps(block_tables, slots, positions, owners, cu, lens, taken)
     from . import ops
 

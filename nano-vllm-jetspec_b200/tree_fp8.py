@@ -30,22 +30,24 @@ def packed_tree_attention_fp8(q, k_pool, v_pool, k_scale, v_scale, metadata, sca
     in ``q``'s dtype, or FP32 on request.  A row that sees no key gives zeros; one that sees a
     NaN row of the cache gives NaN.
     """
-    if q.ndim != 3 or q.shape[0] != metadata.total_queries:
+    shape, pool_shape, dtype = q.shape, k_pool.shape, q.dtype
+    if len(shape) != 3 or shape[0] != metadata.total_queries:
         raise ValueError("packed queries do not match the metadata")
-    if k_pool.ndim != 4 or k_pool.shape != v_pool.shape or k_pool.shape[1] != metadata.block_size:
+    if (len(pool_shape) != 4 or v_pool.shape != pool_shape
+            or pool_shape[1] != metadata.block_size):
         raise ValueError("packed K/V page geometry does not match metadata")
     check_layer(k_pool, v_pool, k_scale, v_scale)
-    total, q_heads, dim = q.shape
-    kv_heads = k_pool.shape[2]
-    if dim != k_pool.shape[3] or dim % 16 or not 16 <= dim <= MAX_HEAD_DIM:
+    total, q_heads, dim = shape
+    kv_heads = pool_shape[2]
+    if dim != pool_shape[3] or dim % 16 or not 16 <= dim <= MAX_HEAD_DIM:
         raise ValueError("head dim must be the pool's, a multiple of 16 up to 128")
     groups = num_queries_per_kv
     if (isinstance(groups, bool) or not isinstance(groups, int) or not 1 <= groups <= MAX_GROUPS
             or q_heads != kv_heads * groups):
         raise ValueError("invalid packed GQA head grouping")
-    if q.dtype != torch.bfloat16 and q.dtype != torch.float16:
+    if dtype != torch.bfloat16 and dtype != torch.float16:
         raise ValueError("8-bit cache attention takes BF16 or FP16 queries")
-    if output_dtype not in (None, q.dtype, torch.float32):
+    if output_dtype not in (None, dtype, torch.float32):
         raise ValueError("output dtype must match the queries or be FP32")
     if not 0 < scale < math.inf:
         raise ValueError("the softmax scale must be positive and finite")
@@ -56,7 +58,7 @@ def packed_tree_attention_fp8(q, k_pool, v_pool, k_scale, v_scale, metadata, sca
     if q.stride(2) != 1 or k_pool.stride(3) != 1 or v_pool.stride(3) != 1:
         raise ValueError("queries and pools need a contiguous head dimension")
     _check_metadata(metadata)
-    out = torch.empty(q.shape, dtype=output_dtype or q.dtype, device=device)
+    out = torch.empty(shape, dtype=output_dtype or dtype, device=device)
     if total == 0:
         return out
     from . import ops
