@@ -471,8 +471,10 @@ typedef struct JtTreeAttnFp8Params {
   int32_t table_width;
   int32_t dtype;                   /* JT_BF16 or JT_F16                                 */
   int32_t out_dtype;               /* dtype or JT_F32                                   */
-  int32_t min_nodes, max_nodes;    /* least (above 0) and largest node count of a request, as
-                                      far as the host knows them; 0, 0 when it does not  */
+  int32_t min_nodes, max_nodes;    /* least (above 0) and largest node count of a request when
+                                      the host knows them, 0, 0 when it does not (and not
+                                      used for a launch under stream capture): requests
+                                      outside them may be left out                         */
 } JtTreeAttnFp8Params;
 
 int jt_tree_attn_fp8_launch(const JtTreeAttnFp8Params* params, cudaStream_t stream);

@@ -398,22 +398,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return jt::MmaOp<__nv_bfloat16>::pack(lo, hi);
 }
 
-// exp2 of a score pair on the FMA pipe, relieving the special-function unit: 2^x = 2^j 2^f with
-// j = rint(x) from the float rounding trick and 2^f, |f| <= 1/2, from a cubic fitted to the
-// least relative error on that interval (8.4e-5, below the bf16 rounding of P).
-__device__ __forceinline__ float2 exp2_poly2(float2 x) {
-  x = make_float2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
-  const float2 t = __fadd2_rn(x, make_float2(12582912.f, 12582912.f));
-  const float2 j = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
-  const float2 f = __fadd2_rn(x, make_float2(-j.x, -j.y));
-  float2 q = __ffma2_rn(make_float2(0.05521299f, 0.05521299f), f,
-                        make_float2(0.24271414f, 0.24271414f));
-  q = __ffma2_rn(q, f, make_float2(0.69326216f, 0.69326216f));
-  q = __ffma2_rn(q, f, make_float2(0.9999196f, 0.9999196f));
-  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
-}
-
 // ---- the work line ----------------------------------------------------------------------
 struct Geometry {
   int groups, npt, npi;  // nodes per query tile, per item
@@ -610,11 +594,7 @@ __device__ __forceinline__ float half_exp(uint32_t s_addr, const float* kf, floa
     for (int k = 0; k < 16; ++k) {
       const float2 x = __ffma2_rn(
           make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), c2, n2);
-      float2 e;
-      if (!kWide && (k & 3) == 3)
-        e = exp2_poly2(x);
-      else
-        e = make_float2(jt::fast_exp2(x.x), jt::fast_exp2(x.y));
+      const float2 e = make_float2(jt::fast_exp2(x.x), jt::fast_exp2(x.y));
       sum[k & 1] = __fadd2_rn(sum[k & 1], e);
       ph[k] = pack_bf16(e.x, e.y);
       if constexpr (kWide) {
@@ -723,13 +703,18 @@ __device__ __forceinline__ void store_columns(const JtTreeAttnFp8Params& p, int6
   }
 }
 
-// Four output columns of one row from its unnormalised sums.
+// Four output columns of one row from its unnormalised sums, O / l 2^shift.
 template <bool kWide>
 __device__ __forceinline__ void store_row4(const JtTreeAttnFp8Params& p, int q_start, int h, int row,
-                                           int d, float4 o, float l) {
+                                           int d, float4 o, float l, float shift) {
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (l == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);  // the row sees no key
-  o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  if (l == 0.f) {  // the row sees no key
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    shift = 0.f;
+  }
+  // In two steps: 2^shift alone may leave fp32's range.
+  const float g = jt::fast_exp2(0.5f * shift);
+  o = make_float4(o.x * inv * g * g, o.y * inv * g * g, o.z * inv * g * g, o.w * inv * g * g);
   const int node = row / p.groups;
   const int64_t at = (static_cast<int64_t>(q_start) + node) * p.out_stride0 +
                      (static_cast<int64_t>(h) * p.groups + row - node * p.groups) * p.out_stride1 + d;
@@ -1608,6 +1593,11 @@ int launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, size_t s
 
 template <bool kWide, typename QT>
 int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
+  // A captured launch is replayed with other node counts than today's: it covers all sizes.
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  int rc = jt_cuda_check(cudaStreamIsCapturing(stream, &capture), "cudaStreamIsCapturing");
+  if (rc != JT_OK) return rc;
+  const bool known = p.max_nodes > 0 && capture == cudaStreamCaptureStatusNone;
   LoadPlan plan{};
   // TMA where a tile is whole boxes of whole pages: pages of whole tiles, or powers of two
   // from 16 keys (a bulk copy of scale bytes is at least 16), with 16-byte scale rows.
@@ -1623,9 +1613,10 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
   // Requests of up to 16 rows and larger trees take kernels of their own; each skips the other's
   // requests, and the host leaves out a kernel that it knows to be without any.
   const int grid = std::min(sms, kMaxCtas);
-  const int64_t most = p.max_nodes > 0 ? static_cast<int64_t>(p.max_nodes) * p.groups : kFewRows + 1;
-  if (std::max(p.min_nodes, 1) * static_cast<int64_t>(p.groups) <= kFewRows) {
-    const int rc = most <= 8 ? launch_few<1, kWide, QT>(p, plan, kmap, vmap, grid, stream)
+  const int64_t least = static_cast<int64_t>(known ? std::max(p.min_nodes, 1) : 1) * p.groups;
+  const int64_t most = known ? static_cast<int64_t>(p.max_nodes) * p.groups : kFewRows + 1;
+  if (least <= kFewRows) {
+    rc = most <= 8 ? launch_few<1, kWide, QT>(p, plan, kmap, vmap, grid, stream)
                              : launch_few<2, kWide, QT>(p, plan, kmap, vmap, grid, stream);
     if (rc != JT_OK || most <= kFewRows) return rc;
   }
@@ -1634,7 +1625,7 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
   if (!encode_queries(&qmap, carve(p.workspace, p.total_queries, p.groups, p.num_kv_heads).q_terms, rows,
                       p.num_kv_heads * Smem<kWide>::kTerms))
     return jt_fail(JT_ERR_CUDA, "tree_attn_fp8: cuTensorMapEncodeTiled rejected the query terms");
-  int rc = jt_cuda_check(cudaFuncSetAttribute(tree_attn_fp8_kernel<kWide>,
+  rc = jt_cuda_check(cudaFuncSetAttribute(tree_attn_fp8_kernel<kWide>,
                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
                                               Smem<kWide>::kBytes),
                          "tree_attn_fp8 smem attribute");

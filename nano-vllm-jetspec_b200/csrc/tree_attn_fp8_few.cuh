@@ -17,7 +17,8 @@
 // row's largest).  2^e of the key multiplies its scores; 2^f of its value is folded into the
 // exponent, y = x + f, P = 2^(y - M + 7) with M a lazy maximum of y (moved when exceeded by
 // 2^8): P stays within 2^15, f16's range, and what f16 drops lies 2^-31 below the largest term.
-// The sum takes 2^-f back: l = sum P 2^-f.  f16 and fp32 outputs add P's low parts (22 bits).
+// The sum has a lazy maximum m of its own, l = sum 2^(x - m): a key of small values may weigh
+// most.  out = O / l 2^(M - 7 - m).  f16 and fp32 outputs add P's low parts (22 bits).
 //
 // Work: as in the tensor core kernel, the items' tiles form one line cut evenly over the SMs.
 // Warp 0 loads (TMA, or cp.async rows where TMA cannot) through a ring of four 32 KB stages;
@@ -39,8 +40,8 @@ struct Few {
   static constexpr int kV = kFewStages * kTile8;
   static constexpr int kScale = 2 * kFewStages * kTile8;           // [stage][K, V][128] bytes
   static constexpr int kO = kScale + kFewStages * 256;             // [warp][row][pitch] float
-  static constexpr int kMl = kO + kWarps * kRows * kFewRowPitch * 4;  // [warp][row] float2
-  static constexpr int kMisc = kMl + kWarps * kRows * 8;           // scan; abort
+  static constexpr int kMl = kO + kWarps * kRows * kFewRowPitch * 4;  // [warp][row] m, l, M, -
+  static constexpr int kMisc = kMl + kWarps * kRows * 16;          // scan; abort
   static constexpr int kBar = kMisc + 512;
   static constexpr int kBytes = kBar + 8 * 2 * kFewStages + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory per CTA");
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
   const int g8 = lane >> 2, q4 = lane & 3;
   const float log2e = 1.4426950408889634f;
   float* o_place = reinterpret_cast<float*>(sbase + F::kO);
-  float2* ml_place = reinterpret_cast<float2*>(sbase + F::kMl);
+  float4* ml_place = reinterpret_cast<float4*>(sbase + F::kMl);
 #pragma unroll 1
   while (few_next(p, cur, it)) {  // to the end even after a wait that ran out: the warps meet
     const int rows = min(it.T * p.groups, F::kRows);
@@ -359,10 +360,10 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
       }
     }
     float o[NT][8][4];
-    float m[NT][2], l[NT][2];
+    float m[NT][2], l[NT][2], my[NT][2];  // of x, of y
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      m[t][0] = m[t][1] = -INFINITY;
+      m[t][0] = m[t][1] = my[t][0] = my[t][1] = -INFINITY;
       l[t][0] = l[t][1] = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -413,38 +414,45 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
       // A NaN value row makes the scores of its key NaN for the rows that see it.
       const float kf[2] = {scale_value(vb0 == 255u ? 255u : kb0), scale_value(vb1 == 255u ? 255u : kb1)};
       const float fe[2] = {static_cast<float>(static_cast<int>(vb0) - 127), static_cast<float>(static_cast<int>(vb1) - 127)};
-      const float back[2] = {scale_value(254u - min(vb0, 254u)), scale_value(254u - min(vb1, 254u))};  // 2^-f
       uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float y[2][2];  // [key g8, g8 + 8][row 2 q4, 2 q4 + 1]
+        float x[2][2];  // [key g8, g8 + 8][row 2 q4, 2 q4 + 1]
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            y[k][i] = fmaf((s[n][0][2 * k + i] + s[n][1][2 * k + i]) * kf[k], c_row[n][i], fe[k]);
+            x[k][i] = (s[n][0][2 * k + i] + s[n][1][2 * k + i]) * kf[k] * c_row[n][i];
         if (masked) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const int node = key0 + g8 + 8 * k - it.P;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              if (node >= 0 && !(node < 16 && (seen[n][i] >> node) & 1u)) y[k][i] = -INFINITY;
+              if (node >= 0 && !(node < 16 && (seen[n][i] >> node) & 1u)) x[k][i] = -INFINITY;
           }
         }
-        const bool moves = y[0][0] > m[n][0] + 8.f || y[1][0] > m[n][0] + 8.f ||
-                           y[0][1] > m[n][1] + 8.f || y[1][1] > m[n][1] + 8.f;
+        bool moves = false;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          moves |= fmaxf(x[0][i], x[1][i]) > m[n][i] + 8.f ||
+                   fmaxf(x[0][i] + fe[0], x[1][i] + fe[1]) > my[n][i] + 8.f;
         if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float mx = fmaxf(y[0][i], y[1][i]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            if (mx > m[n][i] + 8.f) {
-              const float alpha = m[n][i] == -INFINITY ? 1.f : jt::fast_exp2(m[n][i] - mx);
-              m[n][i] = mx;
-              l[n][i] *= alpha;
+            float top = fmaxf(x[0][i], x[1][i]), topy = fmaxf(x[0][i] + fe[0], x[1][i] + fe[1]);
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) {
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+              topy = fmaxf(topy, __shfl_xor_sync(0xffffffffu, topy, d));
+            }
+            if (top > m[n][i] + 8.f) {
+              if (m[n][i] != -INFINITY) l[n][i] *= jt::fast_exp2(m[n][i] - top);
+              m[n][i] = top;
+            }
+            if (topy > my[n][i] + 8.f) {
+              const float alpha = my[n][i] == -INFINITY ? 1.f : jt::fast_exp2(my[n][i] - topy);
+              my[n][i] = topy;
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 o[n][j][i] *= alpha;
@@ -456,11 +464,12 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
         float e[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float nm = m[n][i] == -INFINITY ? 0.f : 7.f - m[n][i];
+          const float nm = m[n][i] == -INFINITY ? 0.f : -m[n][i];
+          const float ny = my[n][i] == -INFINITY ? 0.f : 7.f - my[n][i];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            e[k][i] = jt::fast_exp2(y[k][i] + nm);
-            l[n][i] = fmaf(e[k][i], back[k], l[n][i]);
+            e[k][i] = jt::fast_exp2(x[k][i] + (fe[k] + ny));
+            l[n][i] += jt::fast_exp2(x[k][i] + nm);
           }
         }
 #pragma unroll
@@ -512,7 +521,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int row = 8 * n + 2 * q4 + i;
-        if (g8 == 0) ml_place[w * F::kRows + row] = make_float2(m[n][i], sum);
+        if (g8 == 0) ml_place[w * F::kRows + row] = make_float4(m[n][i], sum, my[n][i], 0.f);
         float2* dst = reinterpret_cast<float2*>(o_place + (w * F::kRows + row) * kFewRowPitch + 16 * g8);
 #pragma unroll
         for (int j = 0; j < 8; ++j) dst[j] = make_float2(o[n][j][i], o[n][j][2 + i]);
@@ -520,26 +529,32 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
     asm volatile("bar.sync 1, %0;\n" ::"n"(32 * F::kWarps) : "memory");
     const int row = (tid - 32) >> 5, d = 4 * lane;  // a warp a row
     for (int rw = row; rw < rows; rw += F::kWarps) {
-      float top = -INFINITY;
+      float top = -INFINITY, topy = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < F::kWarps; ++k) top = fmaxf(top, ml_place[k * F::kRows + rw].x);
+      for (int k = 0; k < F::kWarps; ++k) {
+        top = fmaxf(top, ml_place[k * F::kRows + rw].x);
+        topy = fmaxf(topy, ml_place[k * F::kRows + rw].z);
+      }
       float sum = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < F::kWarps; ++k) {
-        const float2 a = ml_place[k * F::kRows + rw];
-        // Keys without a maximum have a zero sum, or a NaN that has to stay.
-        const float f = a.x == -INFINITY ? 1.f : jt::fast_exp2(a.x - top);
+        const float4 a = ml_place[k * F::kRows + rw];
+        // Keys without a maximum have zero sums, or NaN ones that have to stay.
+        const float f = a.z == -INFINITY ? 1.f : jt::fast_exp2(a.z - topy);
         const float4 x = *reinterpret_cast<const float4*>(o_place + (k * F::kRows + rw) * kFewRowPitch + d);
-        sum = fmaf(a.y, f, sum);
+        sum = fmaf(a.y, a.x == -INFINITY ? 1.f : jt::fast_exp2(a.x - top), sum);
         acc = make_float4(fmaf(x.x, f, acc.x), fmaf(x.y, f, acc.y), fmaf(x.z, f, acc.z), fmaf(x.w, f, acc.w));
       }
       const Workspace ws = carve(p.workspace);
       if (it.slot >= 0) {
-        if (lane == 0) ws.ml[it.slot * 2ll * kM + rw] = make_float2(top, sum);
+        if (lane == 0) {
+          ws.ml[it.slot * 2ll * kM + rw] = make_float2(top, sum);
+          ws.ml[(it.slot * 2ll + 1) * kM + rw] = make_float2(topy, 0.f);
+        }
         ws.o[(it.slot * 2ll * kM + rw) * (kD / 4) + lane] = acc;
       } else if (d < p.head_dim) {
-        store_row4<kWide>(p, it.q_start, it.h, rw, d, acc, sum);
+        store_row4<kWide>(p, it.q_start, it.h, rw, d, acc, sum, topy - 7.f - top);
       }
     }
   }
@@ -557,23 +572,25 @@ __global__ void __launch_bounds__(32 * kFewRows) tree_attn_fp8_few_merge_kernel(
   if (!first.valid || first.finishes) return;
   if (row >= p.node_counts[first.r] * p.groups) return;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, my = -INFINITY, l = 0.f;
   for (int i = c; i < parts; ++i) {
     const int slot = i == c ? 2 * c + 1 : 2 * i;
     if (i != c && !w.meta[slot].valid) continue;  // a part shorter than the least cut
     const float2 ml = w.ml[slot * 2ll * kM + row];
+    const float oy = w.ml[(slot * 2ll + 1) * kM + row].x;
     const float4 o = w.o[(slot * 2ll * kM + row) * (kD / 4) + lane];
-    const float top = fmaxf(m, ml.x);
-    // A row whose keys were all NaN has no maximum but a NaN sum, which has to stay.
-    const float fa = m == -INFINITY ? 1.f : jt::fast_exp2(m - top);
-    const float fb = ml.x == -INFINITY ? 1.f : jt::fast_exp2(ml.x - top);
-    l = l * fa + ml.y * fb;
+    // A row whose keys were all NaN has no maximum but NaN sums, which have to stay.
+    auto factor = [](float own, float top) { return own == -INFINITY ? 1.f : jt::fast_exp2(own - top); };
+    const float top = fmaxf(m, ml.x), topy = fmaxf(my, oy);
+    const float fa = factor(my, topy), fb = factor(oy, topy);
+    l = l * factor(m, top) + ml.y * factor(ml.x, top);
     acc = make_float4(acc.x * fa + o.x * fb, acc.y * fa + o.y * fb, acc.z * fa + o.z * fb, acc.w * fa + o.w * fb);
     m = top;
+    my = topy;
     if (i != c && w.meta[slot].finishes) break;
   }
   if (4 * lane < p.head_dim)
-    store_row4<kWide>(p, p.cu_seqlens_q[first.r], first.h, row, 4 * lane, acc, l);
+    store_row4<kWide>(p, p.cu_seqlens_q[first.r], first.h, row, 4 * lane, acc, l, my - 7.f - m);
 }
 
 template <int NT, bool kWide, typename QT>
