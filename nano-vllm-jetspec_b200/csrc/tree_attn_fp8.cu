@@ -12,28 +12,41 @@
 //   would), and K goes from HBM to the tensor core untouched.  2^e multiplies the score
 //   column in the softmax.  Elements below 2^-10 of the row's largest lose low bits, at most
 //   2^-18 of that largest.
-// * PV runs in bf16: a warpgroup expands the V codes (exact in bf16, 2^f folded in) into the
+// * PV runs in bf16: four warps expand the V codes (exact in bf16, 2^f folded in) into the
 //   swizzled tile the MMA reads.  P is rounded to bf16 (8 bits, as in the 16-bit cache's
 //   kernel); f16 and fp32 outputs take P as hi + lo bf16 (16 bits).
 //
+// Requests of up to 16 rows (nodes x query heads of a KV head) would leave seven eighths of a
+// 128-row tile empty and take the kernel of tree_attn_fp8_few.cuh: 16 requests of 32 thousand
+// keys take 204 us there and 389 here with 4 rows each, 288 and 386 with 16, and 64 requests
+// of 500 to 4000 keys 95 and 128 with 4 rows, 124 and 122 with 16.
+//
 // Work: an item is (request, KV head, m-block), an m-block one or two 128-row query tiles;
-// the items' 128-key tiles, weighted by their tensor time, form one line that is cut into
-// equal parts, one per CTA, so every SM streams the same amount whatever the lengths.  Every
+// the items' 128-key tiles, weighted by their measured time, form one line that is cut into
+// equal parts, one per CTA, so every SM has the same to do whatever the lengths (weights of 1
+// and 2 for one and two query tiles and 3 for an item, by tensor time alone, left CTAs between
+// 411 and 735 us of the same mix).  Every
 // CTA scans the lengths itself and finds its part: no plan kernel, no queue.  An item cut
 // between CTAs leaves unnormalised fp32 partials that a second small kernel merges (a
 // programmatic dependent; it returns at once when nothing was cut).
 //
 // Two softmax streams per CTA keep the tensor core busy while the other one works.  With two
 // query tiles (trees of more than 128 rows) each stream owns a tile and both use every K / V
-// tile; with one, the streams take alternate key tiles of the same rows and their (max, sum,
-// O) are merged at the end.
+// tile; with one, each takes half of every key tile and their (max, sum, O) are merged at the
+// end.  A stream goes through its keys 64 at a time, in two score buffers with a warpgroup
+// each.
+//
+// Bound: the softmax.  32 trees of 64 nodes over 2048 keys (70.9 GFLOP, 173 MB): 140 us, where
+// the matrix products alone would take 42 and the bytes 27.  128 keys against 256 rows take a
+// CTA about 5.5 thousand cycles, of which the tensor core works 2.1; 16 softmax warps beside
+// four converters reach 3.5 in a loop of their own, and the rest is the chain scores -> P -> PV
+// -> scores with its waits.
 //
 //   warps 0, 2   MMA issuers, one per stream; TMEM (S0, S1, O0, O1: 128 columns each)
 //   warp 1       work pieces; TMA loads of K, V and scale bytes for prefix tiles
 //   warp 3       cp.async gathers of tiles that touch tree nodes or pages TMA cannot box
 //   warps 4-7    scale bytes -> key factors; V codes -> bf16 tile
-//   warps 8-23   softmax + epilogue: two warpgroups per stream, each with 64 of a tile's keys
-//                and one thread per row
+//   warps 8-23   softmax + epilogue: a warpgroup per score buffer, a thread per row
 //
 // Every mbarrier wait is bounded; one that runs out sets JT_DEVERR_TIMEOUT and the CTA's
 // abort flag, all roles leave their loops, drain what they started and free the TMEM.
@@ -302,6 +315,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(taddr),
+               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
@@ -537,11 +555,11 @@ __device__ __noinline__ uint2 mask_words(const uint32_t* bits, int off) {
   return make_uint2(out[0], out[1]);
 }
 
-// The largest of a row's 64 scores (times the keys' factors) of half a tile, and then, with the
+// The largest of a row's 64 scores (times the keys' factors) of a granule, and then, with the
 // row's running maximum known, their probabilities.  The scores are read from TMEM twice, 32 at
 // a time, rather than held: with 24 warps a thread has 80 registers, and four softmax warps per
-// scheduler hide each other's latencies, which two with the scores in registers do not (a
-// half tile took 712 cycles of a scheduler with two, 555 with four).
+// scheduler hide each other's latencies, which two with the scores in registers do not (the
+// mix above 750 us with two, 615 with four).
 __device__ __forceinline__ void load_scores(uint32_t s_addr, const float* kf, uint32_t (&v)[32]) {
   tmem_ld32(s_addr, v);
   tmem_wait_ld();
@@ -576,20 +594,18 @@ __device__ __forceinline__ float half_max(uint32_t s_addr, const float* kf) {
   }
   return mx;
 }
-// P = exp2(score * c_row - m), rounded to bf16, to the S columns the scores came from (its low
-// parts 32 columns on, for wide outputs); returns the fp32 sum.
-template <bool kWide>
-__device__ __forceinline__ float half_exp(uint32_t s_addr, const float* kf, float c_row, float neg_m) {
+// P = exp2(score * c_row - m) as high and low bf16 parts, to the S columns the scores came from
+// (the low parts 32 columns on); returns the fp32 sum.
+__device__ __forceinline__ float half_exp_wide(uint32_t s_addr, const float* kf, float c_row, float neg_m) {
   const float2 c2 = make_float2(c_row, c_row), n2 = make_float2(neg_m, neg_m);
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-  uint32_t low[kWide ? 16 : 1];
-#pragma unroll(kWide ? 2 : 1)
+  uint32_t low[16];
+#pragma unroll
   for (int q = 0; q < 2; ++q) {
     uint32_t v[32], ph[16];
     load_scores(s_addr + 32 * q, kf + 32 * q, v);
     // The first low parts go where the second scores were.
-    if constexpr (kWide)
-      if (q == 1) tmem_st16(s_addr + 32, low);
+    if (q == 1) tmem_st16(s_addr + 32, low);
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
       const float2 x = __ffma2_rn(
@@ -597,14 +613,44 @@ __device__ __forceinline__ float half_exp(uint32_t s_addr, const float* kf, floa
       const float2 e = make_float2(jt::fast_exp2(x.x), jt::fast_exp2(x.y));
       sum[k & 1] = __fadd2_rn(sum[k & 1], e);
       ph[k] = pack_bf16(e.x, e.y);
-      if constexpr (kWide) {
-        const float2 f = jt::MmaOp<__nv_bfloat16>::unpack(ph[k]);
-        low[k] = pack_bf16(e.x - f.x, e.y - f.y);
-      }
+      const float2 f = jt::MmaOp<__nv_bfloat16>::unpack(ph[k]);
+      low[k] = pack_bf16(e.x - f.x, e.y - f.y);
     }
     tmem_st16(s_addr + 16 * q, ph);
   }
-  if constexpr (kWide) tmem_st16(s_addr + 48, low);
+  tmem_st16(s_addr + 48, low);
+  return (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
+}
+// The same rounded to bf16, 16 columns at a time with the next 16 on their way (against 32 at a
+// time: 3 % of a mix).
+__device__ __forceinline__ float half_exp_narrow(uint32_t s_addr, const float* kf, float c_row, float neg_m) {
+  const float2 c2 = make_float2(c_row, c_row), n2 = make_float2(neg_m, neg_m);
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  uint32_t v[2][16];
+  tmem_ld16(s_addr, v[0]);
+  const float4* f4 = reinterpret_cast<const float4*>(kf);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tmem_wait_ld();
+    if (c < 3) tmem_ld16(s_addr + 16 * (c + 1), v[(c + 1) & 1]);
+    uint32_t ph[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float4 f = f4[4 * c + k];
+      const uint32_t* x = v[c & 1] + 4 * k;
+      const float2 xa = make_float2(__uint_as_float(x[0]), __uint_as_float(x[1]));
+      const float2 xb = make_float2(__uint_as_float(x[2]), __uint_as_float(x[3]));
+      const float2 a = __ffma2_rn(__fmul2_rn(xa, make_float2(f.x, f.y)), c2, n2);
+      const float2 b = __ffma2_rn(__fmul2_rn(xb, make_float2(f.z, f.w)), c2, n2);
+      const float2 ea = make_float2(jt::fast_exp2(a.x), jt::fast_exp2(a.y));
+      const float2 eb = make_float2(jt::fast_exp2(b.x), jt::fast_exp2(b.y));
+      sum[0] = __fadd2_rn(sum[0], ea);
+      sum[1] = __fadd2_rn(sum[1], eb);
+      ph[2 * k] = pack_bf16(ea.x, ea.y);
+      ph[2 * k + 1] = pack_bf16(eb.x, eb.y);
+    }
+    tmem_st8(s_addr + 8 * c, ph);
+  }
   return (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
 }
 
@@ -1358,7 +1404,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           m_run = m_new;
           const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
           l_run += careful ? half_exp_masked<kWide>(s_addr, f, c_row, neg_m, w.x, w.y)
-                           : half_exp<kWide>(s_addr, f, c_row, neg_m);
+                           : kWide ? half_exp_wide(s_addr, f, c_row, neg_m)
+                           : half_exp_narrow(s_addr, f, c_row, neg_m);
           if (__any_sync(0xffffffffu, moved && m_old != -INFINITY)) {
             // Rescale O once PV of the stream's previous granule has completed.  The wait is for
             // exactly the latest phase: the PV before it completed ahead of this granule's
