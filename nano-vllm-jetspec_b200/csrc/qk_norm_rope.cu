@@ -16,7 +16,9 @@
 // with 8 elements of the first half and their rotation partners of the second, so the
 // rotation needs no exchange and the norm (and the 8-bit maximum) is a few shuffles; a lane
 // group takes four heads of a token, which keeps enough bytes in flight and reads the
-// position, cos / sin and weights once for the four.
+// position, cos / sin and weights once for the four.  16381 tokens of 32 + 8 + 8 bf16 heads,
+// 8-bit cache: 80 us, 4.7 TB/s (CTAs of 64 threads fill an SM's registers; with 256, of which
+// two fit, 93 us).
 #include <algorithm>
 
 #include "common.cuh"
@@ -25,7 +27,7 @@ namespace {
 
 __device__ uint32_t g_norm_errors;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 64;
 
 enum StoreMode { kStoreNone = 0, kStoreSame = 1, kStoreFp8 = 2 };
 
