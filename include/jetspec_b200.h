@@ -436,10 +436,11 @@ int32_t jt_kv_fp8_commit_max_slots(void);
  * metadata with K / V rows held as e4m3 codes times a power-of-two scale per (slot, KV head):
  * value = code * 2^(byte - 127), scale byte 255 = NaN.  A single-token decode step is a tree
  * of one node.  Scores, softmax statistics and sums in fp32; probabilities rounded to bf16
- * for the PV product, or kept to 16 bits (hi + lo) when the output is f16 or fp32.  A query
+ * for the PV product, or kept to 16 bits (hi + lo) when the output is f16 or fp32 (requests
+ * of up to 16 rows, nodes x groups: f16, and 22 bits).  A query
  * row that sees no key gives zeros; a row that sees a key whose K or V scale is NaN gives
  * NaN; keys a row does not see never reach it, whatever their bytes hold.  V values past
- * bf16's range saturate.  Requests with no
+ * bf16's range saturate (requests of more than 16 rows).  Requests with no
  * nodes are allowed.  Strides of the pools and scales in bytes, of q and out in elements,
  * last dimensions contiguous; pool rows 16-byte aligned (head_dim a multiple of 16, at most
  * 128), at most 1024 nodes per tree (larger: device error bit 1, rows not written).

@@ -17,7 +17,7 @@
 // rotation needs no exchange and the norm (and the 8-bit maximum) is a few shuffles; a lane
 // group takes four heads of a token, which keeps enough bytes in flight and reads the
 // position, cos / sin and weights once for the four.  16381 tokens of 32 + 8 + 8 bf16 heads,
-// 8-bit cache: 80 us, 4.7 TB/s (CTAs of 64 threads fill an SM's registers; with 256, of which
+// 8-bit cache: 78 us, 4.9 TB/s (CTAs of 64 threads fill an SM's registers; with 256, of which
 // two fit, 93 us).
 #include <algorithm>
 
