@@ -24,7 +24,7 @@
 // Work: as in the tensor core kernel, the items' tiles form one line cut evenly over the SMs.
 // Warp 0 loads (TMA, or cp.async rows where TMA cannot) through a ring of four 32 KB stages;
 // each of the other warps takes 16 keys of a tile with its own maxima and sums, and the warps
-// meet at the end of a piece.  Eight such warps with up to 224 registers beat sixteen with 96 (two
+// meet at the end of a piece.  Eight such warps of 136 registers beat sixteen of 96 (two
 // tiles in hand): 202 to 240 us for 16 requests of 32 thousand keys.
 
 constexpr int kFewStages = 4;
