@@ -461,7 +461,9 @@ typedef struct JtTreeAttnFp8Params {
   const int64_t* tree_slots;       /* [total_queries]                                   */
   const float* qq_bias;            /* [sum T_r^2] 0 / -inf                              */
   const int64_t* qq_bias_offsets;  /* [num_requests + 1]                                */
-  void* workspace;                 /* device scratch, 256-byte aligned                     */
+  void* workspace;                 /* device scratch, 256-byte aligned; the launch's kernels
+                                      hand their state on through it, so launches that share
+                                      one are issued by one thread at a time, on one stream */
   int64_t workspace_bytes;
   int64_t num_blocks;
   int64_t q_stride0, q_stride1, out_stride0, out_stride1, table_stride0;

@@ -16,7 +16,7 @@ DTYPE_CODES = {torch.bfloat16: _lib.JT_BF16, torch.float16: _lib.JT_F16,
                torch.float32: _lib.JT_F32}
 
 _workspaces: dict = {}
-_workspace_lock = threading.Lock()
+_stream_locks: dict = {}
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -36,22 +36,36 @@ def stream_handle(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(raw_stream(device))
 
 
-def workspace(device: torch.device, nbytes: int, stream: int | None = None) -> torch.Tensor:
+def workspace(device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
     """Device scratch of at least ``nbytes`` reserved per (device, stream, size).
 
     Workspaces are never freed or resized: a CUDA graph that captured a launch keeps
     pointing at the same bytes for as long as the process lives.  Launches on one
     stream are ordered, so they can share the bytes; another stream gets its own.
     """
-    if stream is None:
-        stream = raw_stream(device)
     key = (device.index, stream, int(nbytes))
-    with _workspace_lock:
-        buffer = _workspaces.get(key)
-        if buffer is None:
-            buffer = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
-            _workspaces[key] = buffer
+    buffer = _workspaces.get(key)
+    if buffer is None:
+        buffer = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+        _workspaces[key] = buffer
     return buffer
+
+
+def with_workspace(device: torch.device, nbytes: int, stream: int, launch):
+    """``launch(address)`` with ``nbytes`` of scratch; returns what it returns.
+
+    An operator of several kernels hands its state from one to the next through the scratch,
+    and the ctypes call that enqueues them gives up the interpreter lock.  The stream's own
+    lock, held until all of them are enqueued, keeps another thread's launches on the same
+    stream (and so in the same scratch) from coming between.  Re-entrant: a finaliser that
+    runs inside completes its own launches first.
+    """
+    key = (device.index, stream)
+    lock = _stream_locks.get(key)
+    if lock is None:
+        lock = _stream_locks.setdefault(key, threading.RLock())
+    with lock:
+        return launch(workspace(device, nbytes, stream).data_ptr())
 
 
 def ptr(tensor: torch.Tensor | None) -> int | None:

@@ -99,7 +99,6 @@ def _launch_attention(out, q, k_pool, v_pool, k_scale, v_scale, m, scale, groups
             raise ValueError("8-bit cache attention: invalid geometry")
         _WORKSPACE_SIZES[shape] = nbytes
     stream = _launch.raw_stream(device)
-    scratch = _launch.workspace(device, nbytes, stream)
     qs, os_, ks, vs = q.stride(), out.stride(), k_pool.stride(), v_pool.stride()
     kss, vss = k_scale.stride(), v_scale.stride()
     p = _lib.JtTreeAttnFp8Params(
@@ -107,9 +106,14 @@ def _launch_attention(out, q, k_pool, v_pool, k_scale, v_scale, m, scale, groups
         v_scale.data_ptr(), m.cu_seqlens_q.data_ptr(), m.query_to_request.data_ptr(),
         m.query_local_row.data_ptr(), m.prefix_lens.data_ptr(), m.node_counts.data_ptr(),
         m.block_tables.data_ptr(), m.tree_slots.data_ptr(), m.qq_bias.data_ptr(),
-        m.qq_bias_offsets.data_ptr(), scratch.data_ptr(), nbytes,
+        m.qq_bias_offsets.data_ptr(), None, nbytes,
         blocks, qs[0], qs[1], os_[0], os_[1], m.block_tables.stride(0), ks[0], ks[1], ks[2],
         vs[0], vs[1], vs[2], kss[0], kss[1], vss[0], vss[1], scale, requests, total, kv_heads,
         groups, dim, block_size, m.block_tables.shape[1], codes[q.dtype], codes[out.dtype],
         *_node_range(m))
-    _lib.check(lib.jt_tree_attn_fp8_launch(ctypes.byref(p), stream))
+
+    def launch(scratch):
+        p.workspace = scratch
+        return lib.jt_tree_attn_fp8_launch(ctypes.byref(p), stream)
+
+    _lib.check(_launch.with_workspace(device, nbytes, stream, launch))

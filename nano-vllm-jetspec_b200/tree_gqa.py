@@ -105,7 +105,7 @@ def launch_tree_attention_eager(out, q, k_pool, v_pool, metadata, scale, groups,
     total = int(metadata.total_queries)
     kv_heads = int(k_pool.shape[2])
     head_dim = int(q.shape[-1])
-    scratch = None
+    nbytes = 0
     stream = _launch.raw_stream(device)
     if q.dtype != torch.float32:
         shape = (num_requests, total, kv_heads, int(groups), head_dim)
@@ -114,7 +114,6 @@ def launch_tree_attention_eager(out, q, k_pool, v_pool, metadata, scale, groups,
             size = ctypes.c_size_t(0)
             _lib.check(lib.jt_tree_attn_workspace_size(*shape, ctypes.byref(size)))
             nbytes = _WORKSPACE_SIZES.setdefault(shape, int(size.value))
-        scratch = _launch.workspace(device, nbytes, stream)
     p = _lib.JtTreeAttnParams()
     p.out, p.q, p.k_pool, p.v_pool = out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr()
     p.cu_seqlens_q = metadata.cu_seqlens_q.data_ptr()
@@ -142,9 +141,13 @@ def launch_tree_attention_eager(out, q, k_pool, v_pool, metadata, scale, groups,
     p.v_stride0, p.v_stride1, p.v_stride2 = v_pool.stride(0), v_pool.stride(1), v_pool.stride(2)
     p.scale = float(scale)
     p.split_keys = int(split_keys)
-    p.workspace = None if scratch is None else scratch.data_ptr()
-    p.workspace_bytes = 0 if scratch is None else scratch.numel()
-    _lib.check(lib.jt_tree_attn_launch(ctypes.byref(p), ctypes.c_void_p(stream)))
+    p.workspace_bytes = nbytes
+
+    def launch(scratch):
+        p.workspace = scratch
+        return lib.jt_tree_attn_launch(ctypes.byref(p), ctypes.c_void_p(stream))
+
+    _lib.check(_launch.with_workspace(device, nbytes, stream, launch) if nbytes else launch(None))
     return out
 
 

@@ -1,0 +1,94 @@
+"""Scratch of the operators that hand state from kernel to kernel: who may use which bytes when.
+
+No GPU: the library, the stream lookup and the capture query are stood in for, and the fake
+launch records the scratch that it was given and how long the call lasted.
+"""
+from __future__ import annotations
+
+import threading
+import time
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from jetspec_b200 import _launch, _lib, tree_fp8, tree_gqa
+
+KV_HEADS, GROUPS, DIM, BLOCK = 2, 4, 64, 16
+
+
+class FakeLibrary:
+    """Sizes by a rule like the real ones'; launches that take a while and note (start, end,
+    scratch address, scratch bytes)."""
+
+    def __init__(self, seconds=0.0):
+        self.seconds, self.calls = seconds, []
+
+    def _launch(self, p, stream):
+        start = time.perf_counter()
+        time.sleep(self.seconds)
+        p = p._obj
+        self.calls.append((start, time.perf_counter(), p.workspace, p.workspace_bytes))
+        return _lib.JT_OK
+
+    jt_tree_attn_fp8_launch = jt_tree_attn_launch = _launch
+
+    def jt_tree_attn_fp8_workspace_size(self, requests, total, heads, groups, dim):
+        return 4096 + 512 * total
+
+    def jt_tree_attn_workspace_size(self, requests, total, heads, groups, dim, out):
+        out._obj.value = 4096 + 512 * total
+        return _lib.JT_OK
+
+
+def metadata(total):
+    i32, i64 = torch.int32, torch.int64
+    return SimpleNamespace(
+        cu_seqlens_q=torch.tensor([0, total], dtype=i32),
+        query_to_request=torch.zeros(total, dtype=i32), query_local_row=torch.arange(total).int(),
+        prefix_lens=torch.zeros(1, dtype=i32), node_counts=torch.tensor([total], dtype=i32),
+        block_tables=torch.zeros((1, 1), dtype=i32), tree_slots=torch.arange(total, dtype=i64),
+        qq_bias=torch.zeros(total * total), qq_bias_offsets=torch.zeros(2, dtype=i64),
+        block_size=BLOCK, num_requests=1, total_queries=total, node_counts_host=(total,))
+
+
+def call_fp8(total):
+    q = torch.zeros((total, KV_HEADS * GROUPS, DIM), dtype=torch.bfloat16)
+    pool = torch.zeros((4, BLOCK, KV_HEADS, DIM), dtype=torch.uint8)
+    scale = torch.zeros((4, KV_HEADS, BLOCK), dtype=torch.uint8)
+    tree_fp8._launch_attention(torch.empty_like(q), q, pool, pool, scale, scale, metadata(total),
+                               0.125, GROUPS)
+
+
+def call_16bit(total):
+    q = torch.zeros((total, KV_HEADS * GROUPS, DIM), dtype=torch.bfloat16)
+    pool = torch.zeros((4, BLOCK, KV_HEADS, DIM), dtype=torch.bfloat16)
+    tree_gqa.launch_tree_attention_eager(torch.empty_like(q), q, pool, pool, metadata(total),
+                                         0.125, GROUPS)
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    lib = FakeLibrary()
+    monkeypatch.setattr(_lib, "load_library", lambda *a: lib)
+    monkeypatch.setattr(_launch, "raw_stream", lambda device: 77)
+    monkeypatch.setattr(tree_fp8, "_WORKSPACE_SIZES", {})
+    monkeypatch.setattr(tree_gqa, "_WORKSPACE_SIZES", {})
+    return lib
+
+
+@pytest.mark.parametrize("call", [call_fp8, call_16bit])
+def test_threads_on_one_stream_do_not_share_scratch_at_a_time(fake, call):
+    """Two calls whose launches interleave must not hold the same bytes: one's second kernel
+    would read what the other's first kernel wrote."""
+    fake.seconds = 0.02
+    threads = [threading.Thread(target=call, args=(5,)) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    calls = sorted(fake.calls)
+    assert len(calls) == 4
+    for i, (_, end, address, _) in enumerate(calls):
+        for start, _, other, _ in calls[i + 1:]:
+            assert other != address or start >= end

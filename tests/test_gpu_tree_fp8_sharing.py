@@ -1,0 +1,40 @@
+"""packed_tree_attention_fp8 called from several threads and captures: what they share."""
+from __future__ import annotations
+
+import threading
+
+import pytest
+import torch
+
+import jetspec_b200 as jb
+
+from helpers import bits_equal
+from test_gpu_tree_fp8 import DEVICE, Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("counts", [[40, 3, 64], [2, 1, 4]])
+def test_threads_on_one_stream(counts):
+    """Equal shapes, other data: every call gives what it gives alone."""
+    prefixes = [900, 4000, 33]
+    cases = [Case(prefixes, counts, seed=40 + i) for i in range(2)]
+    want = [case.run() for case in cases]
+    torch.cuda.synchronize()
+    wrong, failed = [0, 0], []
+
+    def work(i):
+        try:
+            for _ in range(10):
+                outs = [cases[i].run() for _ in range(30)]
+                wrong[i] += sum(not bits_equal(out, want[i]) for out in outs)
+        except BaseException as error:  # reported by the main thread
+            failed.append(error)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and wrong == [0, 0]
+    assert jb.read_device_errors() == 0
