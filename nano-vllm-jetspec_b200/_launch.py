@@ -39,9 +39,8 @@ def stream_handle(device: torch.device) -> ctypes.c_void_p:
 def workspace(device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
     """Device scratch of at least ``nbytes`` reserved per (device, stream, size).
 
-    Workspaces are never freed or resized: a CUDA graph that captured a launch keeps
-    pointing at the same bytes for as long as the process lives.  Launches on one
-    stream are ordered, so they can share the bytes; another stream gets its own.
+    Launches on one stream are ordered, so they can share the bytes; another stream gets its
+    own.
     """
     key = (device.index, stream, int(nbytes))
     buffer = _workspaces.get(key)
@@ -59,7 +58,15 @@ def with_workspace(device: torch.device, nbytes: int, stream: int, launch):
     lock, held until all of them are enqueued, keeps another thread's launches on the same
     stream (and so in the same scratch) from coming between.  Re-entrant: a finaliser that
     runs inside completes its own launches first.
+
+    A captured call shares nothing: its graph may replay beside other work, on any stream.
+    Its scratch is allocated for the call; under torch.cuda.graph (and whatever captures
+    through it) that is memory of the graph's own pool, which the allocator hands to later
+    calls of the same capture and to nobody else while the graph lives.
     """
+    if torch._C._cuda_isCurrentStreamCapturing():
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return launch(scratch.data_ptr())
     key = (device.index, stream)
     lock = _stream_locks.get(key)
     if lock is None:

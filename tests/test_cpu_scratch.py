@@ -21,6 +21,8 @@ class FakeLibrary:
     """Sizes by a rule like the real ones'; launches that take a while and note (start, end,
     scratch address, scratch bytes)."""
 
+    capturing = False
+
     def __init__(self, seconds=0.0):
         self.seconds, self.calls = seconds, []
 
@@ -72,6 +74,8 @@ def fake(monkeypatch):
     lib = FakeLibrary()
     monkeypatch.setattr(_lib, "load_library", lambda *a: lib)
     monkeypatch.setattr(_launch, "raw_stream", lambda device: 77)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: lib.capturing,
+                        raising=False)
     monkeypatch.setattr(tree_fp8, "_WORKSPACE_SIZES", {})
     monkeypatch.setattr(tree_gqa, "_WORKSPACE_SIZES", {})
     return lib
@@ -92,3 +96,31 @@ def test_threads_on_one_stream_do_not_share_scratch_at_a_time(fake, call):
     for i, (_, end, address, _) in enumerate(calls):
         for start, _, other, _ in calls[i + 1:]:
             assert other != address or start >= end
+
+
+@pytest.mark.parametrize("call", [call_fp8, call_16bit])
+def test_a_captured_call_takes_scratch_of_its_own(fake, call, monkeypatch):
+    """A graph replays whenever its owner likes: beside eager calls on the stream that it was
+    captured on, and beside graphs captured there after it.  Its scratch has to come from the
+    allocator at the capture (from the graph's own pool), not from what calls share."""
+    made = []
+    empty = torch.empty
+
+    def counted(*args, **kwargs):
+        tensor = empty(*args, **kwargs)
+        if tensor.dtype == torch.uint8:
+            made.append(tensor)  # kept: no address comes twice
+        return tensor
+
+    monkeypatch.setattr(torch, "empty", counted)
+    call(5)
+    call(5)
+    fake.capturing = True
+    call(5)
+    call(5)
+    fake.capturing = False
+    call(5)
+    used = [c[2] for c in fake.calls]
+    assert used[0] == used[1] == used[4]
+    assert len(set(used)) == 3
+    assert set(used[2:4]) <= {t.data_ptr() for t in made}

@@ -38,3 +38,30 @@ def test_threads_on_one_stream(counts):
         t.join()
     assert not failed and wrong == [0, 0]
     assert jb.read_device_errors() == 0
+
+
+@pytest.mark.parametrize("counts", [[40, 3, 64], [2, 1, 4]])
+def test_graphs_replay_beside_each_other_and_beside_eager_calls(counts):
+    """Captured one after the other on one stream, replayed on three at the same time."""
+    cases = [Case([9000, 4000, 33], counts, seed=50 + i) for i in range(3)]
+    want = [case.run() for case in cases]
+    graphs, outs = [], []
+    capture = torch.cuda.Stream()
+    for case in cases[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=capture):
+            outs.append(case.run())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(capture):
+        beside = []
+        for _ in range(20):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            beside += [cases[2].run() for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(bits_equal(out, want[2]) for out in beside)
+    assert bits_equal(outs[0], want[0]) and bits_equal(outs[1], want[1])
+    assert jb.read_device_errors() == 0
