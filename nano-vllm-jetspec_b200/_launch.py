@@ -15,8 +15,7 @@ from . import _lib
 DTYPE_CODES = {torch.bfloat16: _lib.JT_BF16, torch.float16: _lib.JT_F16,
                torch.float32: _lib.JT_F32}
 
-_workspaces: dict = {}
-_stream_locks: dict = {}
+_workspaces: dict = {}  # (device index, stream) -> _Workspace
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -36,28 +35,35 @@ def stream_handle(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(raw_stream(device))
 
 
-def workspace(device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
-    """Device scratch of at least ``nbytes`` reserved per (device, stream, size).
+def remember(sizes: dict, shape: tuple, nbytes: int) -> int:
+    """Keeps a launch shape's workspace size, of a bounded number of shapes."""
+    if len(sizes) >= 4096:
+        sizes.clear()
+    return sizes.setdefault(shape, nbytes)
 
-    Launches on one stream are ordered, so they can share the bytes; another stream gets its
-    own.
-    """
-    key = (device.index, stream, int(nbytes))
-    buffer = _workspaces.get(key)
-    if buffer is None:
-        buffer = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
-        _workspaces[key] = buffer
-    return buffer
+
+class _Workspace:
+    """Scratch of one (device, stream) and the lock that its users hold while they enqueue."""
+    __slots__ = ("lock", "buffer", "nbytes", "address")
+
+    def __init__(self):
+        self.lock = threading.RLock()
+        self.buffer, self.nbytes, self.address = None, 0, None
 
 
 def with_workspace(device: torch.device, nbytes: int, stream: int, launch):
-    """``launch(address)`` with ``nbytes`` of scratch; returns what it returns.
+    """``launch(address)`` with ``nbytes`` of device scratch; returns what it returns.
+
+    Launches on one stream are ordered, so they share one buffer; another stream has its own.
+    It grows to the largest request seen, by a quarter at least so that ragged sizes settle
+    soon; the smaller one goes back to the allocator, which gives it to later work of the same
+    stream only.
 
     An operator of several kernels hands its state from one to the next through the scratch,
     and the ctypes call that enqueues them gives up the interpreter lock.  The stream's own
     lock, held until all of them are enqueued, keeps another thread's launches on the same
-    stream (and so in the same scratch) from coming between.  Re-entrant: a finaliser that
-    runs inside completes its own launches first.
+    stream from coming between.  Re-entrant: a finaliser that runs inside completes its own
+    launches first.
 
     A captured call shares nothing: its graph may replay beside other work, on any stream.
     Its scratch is allocated for the call; under torch.cuda.graph (and whatever captures
@@ -68,11 +74,16 @@ def with_workspace(device: torch.device, nbytes: int, stream: int, launch):
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
         return launch(scratch.data_ptr())
     key = (device.index, stream)
-    lock = _stream_locks.get(key)
-    if lock is None:
-        lock = _stream_locks.setdefault(key, threading.RLock())
-    with lock:
-        return launch(workspace(device, nbytes, stream).data_ptr())
+    held = _workspaces.get(key)
+    if held is None:
+        held = _workspaces.setdefault(key, _Workspace())
+    with held.lock:
+        if nbytes > held.nbytes:
+            size = max(nbytes, held.nbytes + held.nbytes // 4)
+            held.buffer, held.nbytes = None, 0  # freed first: the two need not fit together
+            held.buffer = torch.empty(size, dtype=torch.uint8, device=device)
+            held.nbytes, held.address = size, held.buffer.data_ptr()
+        return launch(held.address)
 
 
 def ptr(tensor: torch.Tensor | None) -> int | None:

@@ -97,7 +97,7 @@ def _launch_attention(out, q, k_pool, v_pool, k_scale, v_scale, m, scale, groups
         nbytes = lib.jt_tree_attn_fp8_workspace_size(*shape)
         if nbytes < 0:
             raise ValueError("8-bit cache attention: invalid geometry")
-        _WORKSPACE_SIZES[shape] = nbytes
+        _launch.remember(_WORKSPACE_SIZES, shape, nbytes)
     stream = _launch.raw_stream(device)
     qs, os_, ks, vs = q.stride(), out.stride(), k_pool.stride(), v_pool.stride()
     kss, vss = k_scale.stride(), v_scale.stride()

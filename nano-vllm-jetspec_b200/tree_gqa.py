@@ -113,7 +113,7 @@ def launch_tree_attention_eager(out, q, k_pool, v_pool, metadata, scale, groups,
         if nbytes is None:
             size = ctypes.c_size_t(0)
             _lib.check(lib.jt_tree_attn_workspace_size(*shape, ctypes.byref(size)))
-            nbytes = _WORKSPACE_SIZES.setdefault(shape, int(size.value))
+            nbytes = _launch.remember(_WORKSPACE_SIZES, shape, int(size.value))
     p = _lib.JtTreeAttnParams()
     p.out, p.q, p.k_pool, p.v_pool = out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr()
     p.cu_seqlens_q = metadata.cu_seqlens_q.data_ptr()

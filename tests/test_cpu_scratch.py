@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import threading
 import time
+import weakref
 from types import SimpleNamespace
 
 import pytest
@@ -124,3 +125,37 @@ def test_a_captured_call_takes_scratch_of_its_own(fake, call, monkeypatch):
     assert used[0] == used[1] == used[4]
     assert len(set(used)) == 3
     assert set(used[2:4]) <= {t.data_ptr() for t in made}
+
+
+@pytest.mark.parametrize("call", [call_fp8, call_16bit])
+def test_scratch_stays_bounded_over_many_sizes(fake, call, monkeypatch):
+    """A serving loop meets every total of packed nodes; what stays allocated after it must not
+    grow with their number."""
+    made = []
+    empty = torch.empty
+
+    def counted(*args, **kwargs):
+        tensor = empty(*args, **kwargs)
+        if tensor.dtype == torch.uint8:
+            made.append((weakref.ref(tensor), tensor.numel()))
+        return tensor
+
+    monkeypatch.setattr(torch, "empty", counted)
+    stream = object()  # one that no other call has used
+    monkeypatch.setattr(_launch, "raw_stream", lambda device: hash(stream))
+    totals = [*range(1, 200, 3), *range(200, 1, -7)]
+    for total in totals:
+        call(total)
+    largest = max(c[3] for c in fake.calls)
+    assert [c[3] for c in fake.calls] == [4096 + 512 * t for t in totals]
+    held = sum(n for ref, n in made if ref() is not None)
+    assert largest <= held <= 2 * largest
+    assert len(made) <= 24  # allocations, not one per size
+
+
+def test_remembered_sizes_stay_bounded():
+    sizes = {}
+    for total in range(10000):
+        assert _launch.remember(sizes, (1, total), 3 * total) == 3 * total
+        assert sizes[1, total] == 3 * total
+    assert len(sizes) <= 4096

@@ -65,3 +65,22 @@ def test_graphs_replay_beside_each_other_and_beside_eager_calls(counts):
     assert all(bits_equal(out, want[2]) for out in beside)
     assert bits_equal(outs[0], want[0]) and bits_equal(outs[1], want[1])
     assert jb.read_device_errors() == 0
+
+
+def test_memory_stays_bounded_over_many_batch_sizes():
+    """Every total of packed nodes from 1 to 48: one scratch buffer of the stream, not 48."""
+    cases = [Case([64] * n, [1] * n, kv_heads=1, groups=2, dim=16, block=64, seed=n)
+             for n in (1, 48)]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        cases[1].run()
+        held = torch.cuda.memory_allocated(DEVICE)
+        for n in range(1, 48):
+            case = Case([64] * n, [1] * n, kv_heads=1, groups=2, dim=16, block=64, seed=n)
+            case.run()
+            del case
+        assert torch.cuda.memory_allocated(DEVICE) - held < 1 << 20
+        want = cases[0].run()
+    stream.synchronize()
+    assert bits_equal(want, cases[0].run())
