@@ -44,11 +44,11 @@ def remember(sizes: dict, shape: tuple, nbytes: int) -> int:
 
 class _Workspace:
     """Scratch of one (device, stream) and the lock that its users hold while they enqueue."""
-    __slots__ = ("lock", "buffer", "nbytes", "address")
+    __slots__ = ("lock", "buffer", "nbytes")
 
     def __init__(self):
         self.lock = threading.RLock()
-        self.buffer, self.nbytes, self.address = None, 0, None
+        self.buffer, self.nbytes = None, 0
 
 
 def with_workspace(device: torch.device, nbytes: int, stream: int, launch):
@@ -82,8 +82,9 @@ def with_workspace(device: torch.device, nbytes: int, stream: int, launch):
             size = max(nbytes, held.nbytes + held.nbytes // 4)
             held.buffer, held.nbytes = None, 0  # freed first: the two need not fit together
             held.buffer = torch.empty(size, dtype=torch.uint8, device=device)
-            held.nbytes, held.address = size, held.buffer.data_ptr()
-        return launch(held.address)
+            held.nbytes = size
+        buffer = held.buffer  # kept through the launch, whatever a finaliser's call does
+        return launch(buffer.data_ptr())
 
 
 def ptr(tensor: torch.Tensor | None) -> int | None:

@@ -96,7 +96,8 @@ struct Smem {
   static constexpr int kV8 = kK + kKRing * kTile8;
   static constexpr int kV16 = kV8 + kVRing * kTile8;
   static constexpr int kScale = kV16 + 2 * kTile16;          // [kScaleRing][K, V][128] bytes
-  static constexpr int kKf = kScale + kScaleRing * 256;       // [2][128] float
+  static constexpr int kBad = kScale + kScaleRing * 256;      // [kScaleRing][4] words: keys without a place
+  static constexpr int kKf = kBad + kScaleRing * 16;          // [2][128] float
   static constexpr int kX = kKf + 2 * kN * 4;                 // [stream][half][128] float2: max, sum
   static constexpr int kMx = kX + 4 * kM * 8;                 // [stream][128] float: maxima
   static constexpr int kItem = kMx + 2 * kM * 4;              // [2][16] int
@@ -157,6 +158,10 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 }
 __device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(bytes)
                : "memory");
 }
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
@@ -642,8 +647,9 @@ __device__ __forceinline__ float half_exp_narrow(uint32_t s_addr, const float* k
   return (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
 }
 
-// The same for tiles with masked keys or a NaN row (the last one or two of an item): masked
-// scores are -inf, every exponential is exp2, which keeps a NaN.  Rolled over 8 columns: a few
+// The same for tiles with masked keys, a NaN row or a key without a place in the pool (the last
+// one or two of an item, and few others): masked scores are -inf, and those of keys whose factor
+// is negative, which stands for no place; every exponential is exp2, which keeps a NaN.  Rolled over 8 columns: a few
 // hundred instructions that run seldom cost more to fetch than to execute.
 __device__ __noinline__ float half_max_masked(uint32_t s_addr, const float* kf, uint32_t m0,
                                               uint32_t m1) {
@@ -656,7 +662,8 @@ __device__ __noinline__ float half_max_masked(uint32_t s_addr, const float* kf, 
     const uint32_t bits = (c < 4 ? m0 : m1) >> (8 * (c & 3));
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      mx = fmaxf(mx, (bits >> k) & 1u ? __uint_as_float(v[k]) * kf[8 * c + k] : -INFINITY);
+      mx = fmaxf(mx, (bits >> k) & 1u && !(kf[8 * c + k] < 0.f) ? __uint_as_float(v[k]) * kf[8 * c + k]
+                                                                  : -INFINITY);
   }
   return mx;
 }
@@ -677,7 +684,8 @@ __device__ __noinline__ float half_exp_masked(uint32_t s_addr, const float* kf, 
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int col = 2 * k + i;
-          const float x = ((q ? m1 : m0) >> col) & 1u ? __uint_as_float(v[col]) : -INFINITY;
+          const bool seen = ((q ? m1 : m0) >> col) & 1u && !(kf[32 * q + col] < 0.f);
+          const float x = seen ? __uint_as_float(v[col]) : -INFINITY;
           e[i] = jt::fast_exp2(fmaf(x, c_row, neg_m));
           sum += e[i];
         }
@@ -698,7 +706,8 @@ __device__ __noinline__ float half_exp_masked(uint32_t s_addr, const float* kf, 
       float e[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float x = (bits >> k) & 1u ? __uint_as_float(v[k]) * kf[8 * c + k] : -INFINITY;
+        const float f = kf[8 * c + k];
+        const float x = (bits >> k) & 1u && !(f < 0.f) ? __uint_as_float(v[k]) * f : -INFINITY;
         e[k] = jt::fast_exp2(fmaf(x, c_row, neg_m));
         sum += e[k];
       }
@@ -1133,17 +1142,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t full = JT_BAR((is_v ? kBarVFull : kBarKFull) + slot);
           const uint32_t dst = base + (is_v ? L::kV8 : L::kK) + slot * kTile8;
           const uint32_t sc_slot = g % kScaleRing, sc_full = JT_BAR(kBarScale + sc_slot);
+          volatile uint32_t* bad = reinterpret_cast<volatile uint32_t*>(sbase + L::kBad) + 4 * sc_slot;
           mbar_arrive_tx(full, kTile8);
-          if (!is_v) mbar_arrive_tx(sc_full, 2 * kN);
+          if (!is_v) {
+            mbar_expect_tx(sc_full, 2 * kN);
+            bad[0] = bad[1] = bad[2] = bad[3] = 0;
+          }
 #pragma unroll 1
           for (int i = 0; i < kN; i += plan.box) {
             const int pos = kb + i, off = pos % p.block_size;
             int page = __ldg(table + pos / p.block_size);
             if (page < 0 || page >= p.num_blocks) {
+              // The box's keys are left out.  Page -1 lies outside the map: zeros.
               atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
               page = -1;
+              if (!is_v) {
+#pragma unroll 1
+                for (int k = i; k < i + plan.box; k += 16) bad[k >> 5] |= 0xffffu << (k & 31);
+              }
             }
-            // Page -1 lies outside the map: the box is filled with zeros.
             tma_load_4d(dst + i * kD, is_v ? &vmap : &kmap, 0, it.h, off, page, full);
             if (!is_v) {
               const int64_t pg = max(page, 0);
@@ -1153,7 +1170,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           note(is_v ? 4 + slot : slot, true, g / ring);
-          if (!is_v) note(8 + sc_slot, true, g / kScaleRing);
+          if (!is_v) {
+            mbar_arrive(sc_full);  // with the missing keys written
+            note(8 + sc_slot, true, g / kScaleRing);
+          }
         };
         if (lane == 0) {
           // K 0, K 1, then V t and K t + 2: the order in which they are used.
@@ -1235,12 +1255,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait_shared_at_least(base + L::kMisc + 12, g + 1, abort);
           __syncwarp();
           unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256 + lane;
+          uint32_t* bad = reinterpret_cast<uint32_t*>(sbase + L::kBad) + 4 * (g % kScaleRing);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             gather_row(base + L::kK + ks * kTile8, 32 * i + lane, k_src[i], ok[i] ? chunks : 0);
             gather_row(base + L::kV8 + vs * kTile8, 32 * i + lane, v_src[i], ok[i] ? chunks : 0);
             sc[32 * i] = static_cast<unsigned char>(kb[i]);
             sc[kN + 32 * i] = static_cast<unsigned char>(vb[i]);
+            const uint32_t none = __ballot_sync(0xffffffffu, !ok[i]);
+            if (lane == 0) bad[i] = none;
           }
           asm volatile("cp.async.wait_all;\n" ::: "memory");
           fence_proxy_async();
@@ -1276,12 +1299,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         warp_wait(JT_BAR(kBarScale + g % kScaleRing), (g / kScaleRing) & 1, abort);
         const unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256 + ct;
         const uint32_t kb = sc[0], vb = sc[kN];
+        // Keys without a place in the pool: a negative factor, which the masked forms leave out.
+        const uint32_t bad = reinterpret_cast<const uint32_t*>(sbase + L::kBad)[4 * (g % kScaleRing) + cw];
         if (g >= 2) warp_wait(JT_BAR(kBarBEmpty + buf), ((g >> 1) & 1) ^ 1, abort);
-        kf[buf * kN + ct] = vb == 255u ? scale_value(255u) : scale_value(kb);
+        kf[buf * kN + ct] = (bad >> lane) & 1u ? -1.f : vb == 255u ? scale_value(255u) : scale_value(kb);
         const uint2 mine = v_multipliers(vb);
-        const bool nan = __any_sync(0xffffffffu, kb == 255u || vb == 255u);
+        const bool rare = bad != 0 || __any_sync(0xffffffffu, kb == 255u || vb == 255u);
         const bool big = __any_sync(0xffffffffu, vb > 134u);  // needs the second multiplier
-        if (lane == 0) flag[buf * 4 + cw] = nan;
+        if (lane == 0) flag[buf * 4 + cw] = rare;
         warp_arrive(JT_BAR(kBarFac + buf));
         warp_wait(JT_BAR(kBarVFull + g % kVRing), (g / kVRing) & 1, abort);
         // This warp's 32 rows x 8 chunks in 8 rounds, four rounds' loads in flight at a time.

@@ -39,7 +39,8 @@ struct Few {
   static constexpr int kRows = 8 * NT;
   static constexpr int kV = kFewStages * kTile8;
   static constexpr int kScale = 2 * kFewStages * kTile8;           // [stage][K, V][128] bytes
-  static constexpr int kO = kScale + kFewStages * 256;             // [warp][row][pitch] float
+  static constexpr int kBad = kScale + kFewStages * 256;           // [stage][4] words: keys without a place
+  static constexpr int kO = kBad + kFewStages * 16;                // [warp][row][pitch] float
   static constexpr int kMl = kO + kWarps * kRows * kFewRowPitch * 4;  // [warp][row] m, l, M, -
   static constexpr int kMisc = kMl + kWarps * kRows * 16;          // scan; abort
   static constexpr int kBar = kMisc + 512;
@@ -231,6 +232,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
         const uint32_t full = full0 + 8 * stage;
         const uint32_t kdst = base + stage * kTile8, vdst = kdst + F::kV;
         unsigned char* sc = sbase + F::kScale + stage * 256;
+        uint32_t* none = reinterpret_cast<uint32_t*>(sbase + F::kBad) + 4 * stage;
         const bool tma = plan.tma && kb + kN <= it.P;
         if (tma && (tile * boxes) >> 5 != batch) {
           batch = (tile * boxes) >> 5;
@@ -257,8 +259,14 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
           if (lane == 0) mbar_arrive_tx(full, 2 * kTile8 + 2 * kN);
           __syncwarp();
           const int page = __shfl_sync(0xffffffffu, pages, (tile * boxes + lane) & 31);
+          const uint32_t out = __ballot_sync(0xffffffffu, lane < boxes && page < 0);
+          if (lane < 4) {
+            // This word's 32 keys lie in one box, or in two of 16.
+            const uint32_t b = out >> (32 * lane / plan.box);
+            none[lane] = plan.box >= 32 ? (b & 1u ? ~0u : 0u) : (b & 1u ? 0xffffu : 0u) | (b & 2u ? ~0xffffu : 0u);
+          }
           if (lane < boxes) {
-            // Page -1 lies outside the map: the box is filled with zeros.
+            // Page -1 lies outside the map: zeros.
             const int i = lane * plan.box, off = (kb + i) % p.block_size;
             tma_load_4d(kdst + i * kD, &kmap, 0, it.h, off, page, full);
             tma_load_4d(vdst + i * kD, &vmap, 0, it.h, off, page, full);
@@ -280,6 +288,8 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
             gather_row(vdst, row, vp + page * p.v_stride0 + off * p.v_stride1 + it.h * p.v_stride2, ok ? chunks : 0);
             sc[row] = ok ? __ldg(ksc + page * p.ks_stride0 + it.h * p.ks_stride1 + off) : 127;
             sc[kN + row] = ok ? __ldg(vsc + page * p.vs_stride0 + it.h * p.vs_stride1 + off) : 127;
+            const uint32_t out = __ballot_sync(0xffffffffu, !ok);
+            if (lane == 0) none[i] = out;
           }
           asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(full) : "memory");
           mbar_arrive(full);
@@ -374,12 +384,15 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
     for (int t = 0; t < it.n; ++t) {
       const uint32_t g = g0 + t, stage = g % kFewStages;
       const int key0 = (it.t0 + t) * kN + 16 * w;
-      const bool masked = (it.t0 + t + 1) * kN > it.P;
       mbar_wait(full0 + 8 * stage, (g / kFewStages) & 1, abort);
       __syncwarp();
       const unsigned char* kt = sbase + stage * kTile8 + 16 * w * 128;
       const unsigned char* vt = kt + F::kV;
       const unsigned char* sc = sbase + F::kScale + stage * 256 + 16 * w;
+      // Keys without a place in the pool are left out, like tree nodes that a row does not see.
+      const uint32_t none = (reinterpret_cast<const uint32_t*>(sbase + F::kBad)[4 * stage + (w >> 1)] >>
+                             (16 * (w & 1))) & 0xffffu;
+      const bool masked = (it.t0 + t + 1) * kN > it.P || none != 0;
       // S^T
       float s[NT][2][4];
 #pragma unroll
@@ -429,7 +442,8 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
             const int node = key0 + g8 + 8 * k - it.P;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              if (node >= 0 && !(node < 16 && (seen[n][i] >> node) & 1u)) x[k][i] = -INFINITY;
+              if ((none >> (g8 + 8 * k)) & 1u || (node >= 0 && !(node < 16 && (seen[n][i] >> node) & 1u)))
+                x[k][i] = -INFINITY;
           }
         }
         bool moves = false;
