@@ -96,13 +96,13 @@ struct Smem {
   static constexpr int kV8 = kK + kKRing * kTile8;
   static constexpr int kV16 = kV8 + kVRing * kTile8;
   static constexpr int kScale = kV16 + 2 * kTile16;          // [kScaleRing][K, V][128] bytes
-  static constexpr int kBad = kScale + kScaleRing * 256;      // [kScaleRing][4] words: keys without a place
-  static constexpr int kKf = kBad + kScaleRing * 16;          // [2][128] float
+  static constexpr int kLost = kScale + kScaleRing * 256;     // [kScaleRing][4] words: keys without a place
+  static constexpr int kKf = kLost + kScaleRing * 16;         // [2][128] float
   static constexpr int kX = kKf + 2 * kN * 4;                 // [stream][half][128] float2: max, sum
   static constexpr int kMx = kX + 4 * kM * 8;                 // [stream][128] float: maxima
   static constexpr int kItem = kMx + 2 * kM * 4;              // [2][16] int
-  static constexpr int kFlag = kItem + 2 * 64;                // [2][4] int
-  static constexpr int kMisc = kFlag + 32;                    // TMEM base, abort, free slots
+  static constexpr int kFlag = kItem + 2 * 64;                // [2][4] int2: rare forms; keys without a place
+  static constexpr int kMisc = kFlag + 64;                    // TMEM base, abort, free slots
   static constexpr int kBar = kMisc + 32;
   static constexpr int kBytes = kBar + 8 * 64 + 1024;         // + alignment slack
   static_assert(kBytes <= 227 * 1024, "shared memory per CTA");
@@ -529,6 +529,19 @@ __device__ __noinline__ void gather_row(uint32_t dst, int row, const char* src, 
                     c < chunks ? 16 : 0);
 }
 
+// Marks keys lo to hi - 1 of a tile, in sixteens, as without a place in the pool.  Out of line,
+// and the words are cleared by their reader: what the loading lane runs for every tile counts
+// (words that it writes for each: 2.5 % of a serving mix).
+__device__ __noinline__ void lose_keys(uint32_t words, int lo, int hi) {
+  atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
+#pragma unroll 1
+  for (int k = lo; k < hi; k += 16)
+    asm volatile("{\n .reg .b32 w;\n ld.shared.u32 w, [%0];\n or.b32 w, w, %1;\n st.shared.u32 [%0], w;\n}\n" ::"r"(
+                     words + 4 * (k >> 5)),
+                 "r"(0xffffu << (k & 31))
+                 : "memory");
+}
+
 // How tiles reach shared memory, decided on the host from the layout.
 struct LoadPlan {
   int tma;   // prefix tiles by TMA boxes of `box` keys, their scale bytes by bulk copies
@@ -648,9 +661,9 @@ __device__ __forceinline__ float half_exp_narrow(uint32_t s_addr, const float* k
 }
 
 // The same for tiles with masked keys, a NaN row or a key without a place in the pool (the last
-// one or two of an item, and few others): masked scores are -inf, and those of keys whose factor
-// is negative, which stands for no place; every exponential is exp2, which keeps a NaN.  Rolled over 8 columns: a few
-// hundred instructions that run seldom cost more to fetch than to execute.
+// one or two of an item, and few others): masked scores are -inf, every exponential is exp2,
+// which keeps a NaN.  Rolled over 8 columns: a few hundred instructions that run seldom cost
+// more to fetch than to execute.
 __device__ __noinline__ float half_max_masked(uint32_t s_addr, const float* kf, uint32_t m0,
                                               uint32_t m1) {
   float mx = -INFINITY;
@@ -662,8 +675,7 @@ __device__ __noinline__ float half_max_masked(uint32_t s_addr, const float* kf, 
     const uint32_t bits = (c < 4 ? m0 : m1) >> (8 * (c & 3));
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      mx = fmaxf(mx, (bits >> k) & 1u && !(kf[8 * c + k] < 0.f) ? __uint_as_float(v[k]) * kf[8 * c + k]
-                                                                  : -INFINITY);
+      mx = fmaxf(mx, (bits >> k) & 1u ? __uint_as_float(v[k]) * kf[8 * c + k] : -INFINITY);
   }
   return mx;
 }
@@ -684,8 +696,7 @@ __device__ __noinline__ float half_exp_masked(uint32_t s_addr, const float* kf, 
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int col = 2 * k + i;
-          const bool seen = ((q ? m1 : m0) >> col) & 1u && !(kf[32 * q + col] < 0.f);
-          const float x = seen ? __uint_as_float(v[col]) : -INFINITY;
+          const float x = ((q ? m1 : m0) >> col) & 1u ? __uint_as_float(v[col]) : -INFINITY;
           e[i] = jt::fast_exp2(fmaf(x, c_row, neg_m));
           sum += e[i];
         }
@@ -706,8 +717,7 @@ __device__ __noinline__ float half_exp_masked(uint32_t s_addr, const float* kf, 
       float e[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float f = kf[8 * c + k];
-        const float x = (bits >> k) & 1u && !(f < 0.f) ? __uint_as_float(v[k]) * f : -INFINITY;
+        const float x = (bits >> k) & 1u ? __uint_as_float(v[k]) * kf[8 * c + k] : -INFINITY;
         e[k] = jt::fast_exp2(fmaf(x, c_row, neg_m));
         sum += e[k];
       }
@@ -877,6 +887,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   if (tid == 0) misc[1] = misc[2] = misc[3] = 0;
+  if (tid < 4 * kScaleRing) reinterpret_cast<uint32_t*>(sbase + L::kLost)[tid] = 0;
   if (tid < kNumBars) {
     mbar_init(JT_BAR(tid), bar_count(tid));
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -1142,24 +1153,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t full = JT_BAR((is_v ? kBarVFull : kBarKFull) + slot);
           const uint32_t dst = base + (is_v ? L::kV8 : L::kK) + slot * kTile8;
           const uint32_t sc_slot = g % kScaleRing, sc_full = JT_BAR(kBarScale + sc_slot);
-          volatile uint32_t* bad = reinterpret_cast<volatile uint32_t*>(sbase + L::kBad) + 4 * sc_slot;
           mbar_arrive_tx(full, kTile8);
-          if (!is_v) {
-            mbar_expect_tx(sc_full, 2 * kN);
-            bad[0] = bad[1] = bad[2] = bad[3] = 0;
-          }
+          if (!is_v) mbar_expect_tx(sc_full, 2 * kN);
 #pragma unroll 1
           for (int i = 0; i < kN; i += plan.box) {
             const int pos = kb + i, off = pos % p.block_size;
             int page = __ldg(table + pos / p.block_size);
             if (page < 0 || page >= p.num_blocks) {
               // The box's keys are left out.  Page -1 lies outside the map: zeros.
-              atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
+              lose_keys(base + L::kLost + 16 * sc_slot, i, is_v ? i : i + plan.box);
               page = -1;
-              if (!is_v) {
-#pragma unroll 1
-                for (int k = i; k < i + plan.box; k += 16) bad[k >> 5] |= 0xffffu << (k & 31);
-              }
             }
             tma_load_4d(dst + i * kD, is_v ? &vmap : &kmap, 0, it.h, off, page, full);
             if (!is_v) {
@@ -1255,7 +1258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait_shared_at_least(base + L::kMisc + 12, g + 1, abort);
           __syncwarp();
           unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256 + lane;
-          uint32_t* bad = reinterpret_cast<uint32_t*>(sbase + L::kBad) + 4 * (g % kScaleRing);
+          uint32_t* lost = reinterpret_cast<uint32_t*>(sbase + L::kLost) + 4 * (g % kScaleRing);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             gather_row(base + L::kK + ks * kTile8, 32 * i + lane, k_src[i], ok[i] ? chunks : 0);
@@ -1263,7 +1266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             sc[32 * i] = static_cast<unsigned char>(kb[i]);
             sc[kN + 32 * i] = static_cast<unsigned char>(vb[i]);
             const uint32_t none = __ballot_sync(0xffffffffu, !ok[i]);
-            if (lane == 0) bad[i] = none;
+            if (none != 0 && lane == 0) lost[i] = none;
           }
           asm volatile("cp.async.wait_all;\n" ::: "memory");
           fence_proxy_async();
@@ -1282,7 +1285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int ct = tid - 128, cw = warp - 4;  // this thread's key; this warp's 32 rows
     uint32_t g0 = 0;
     float* kf = reinterpret_cast<float*>(sbase + L::kKf);
-    volatile int* flag = reinterpret_cast<volatile int*>(sbase + L::kFlag);
+    int2* flag = reinterpret_cast<int2*>(sbase + L::kFlag);
     // V: eight lanes of a warp take four 16-byte chunks of rows r and r ^ 5, so that both the
     // swizzled loads and the swizzled stores of the eight touch different banks.
     const int quad = lane >> 3, sub = lane & 7;
@@ -1299,14 +1302,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         warp_wait(JT_BAR(kBarScale + g % kScaleRing), (g / kScaleRing) & 1, abort);
         const unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256 + ct;
         const uint32_t kb = sc[0], vb = sc[kN];
-        // Keys without a place in the pool: a negative factor, which the masked forms leave out.
-        const uint32_t bad = reinterpret_cast<const uint32_t*>(sbase + L::kBad)[4 * (g % kScaleRing) + cw];
+        uint32_t* lost_word = reinterpret_cast<uint32_t*>(sbase + L::kLost) + 4 * (g % kScaleRing) + cw;
+        const uint32_t lost = *lost_word;
         if (g >= 2) warp_wait(JT_BAR(kBarBEmpty + buf), ((g >> 1) & 1) ^ 1, abort);
-        kf[buf * kN + ct] = (bad >> lane) & 1u ? -1.f : vb == 255u ? scale_value(255u) : scale_value(kb);
+        kf[buf * kN + ct] = vb == 255u ? scale_value(255u) : scale_value(kb);
         const uint2 mine = v_multipliers(vb);
-        const bool rare = bad != 0 || __any_sync(0xffffffffu, kb == 255u || vb == 255u);
+        const bool rare = lost != 0 || __any_sync(0xffffffffu, kb == 255u || vb == 255u);
         const bool big = __any_sync(0xffffffffu, vb > 134u);  // needs the second multiplier
-        if (lane == 0) flag[buf * 4 + cw] = rare;
+        __syncwarp();
+        if (lane == 0) {
+          flag[buf * 4 + cw] = make_int2(rare, static_cast<int>(lost));
+          if (lost != 0) *lost_word = 0;
+        }
         warp_arrive(JT_BAR(kBarFac + buf));
         warp_wait(JT_BAR(kBarVFull + g % kVRing), (g / kVRing) & 1, abort);
         // This warp's 32 rows x 8 chunks in 8 rounds, four rounds' loads in flight at a time.
@@ -1361,7 +1368,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t other_bar = JT_BAR(kBarMx + (2 * s + (buf ^ 1)) * 4 + (warp & 3));
     const float* kf = reinterpret_cast<const float*>(sbase + L::kKf);
     const Workspace ws = carve(p.workspace, p.total_queries, ge.groups, p.num_kv_heads);
-    const volatile int* flag = reinterpret_cast<const volatile int*>(sbase + L::kFlag);
     float2* xch = reinterpret_cast<float2*>(sbase + L::kX);
     float* m_row = reinterpret_cast<float*>(sbase + L::kMx) + s * kM + row;
     const int local = row / ge.groups, head_in = row - local * ge.groups;
@@ -1397,8 +1403,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         if (live) {
           const float* f = kf + (g & 1) * kN + kHalf * half;
-          careful |= (flag[(g & 1) * 4] | flag[(g & 1) * 4 + 1] | flag[(g & 1) * 4 + 2] |
-                      flag[(g & 1) * 4 + 3]) != 0;
+          const int4* rare = reinterpret_cast<const int4*>(sbase + L::kFlag + 32 * (g & 1));
+          const int4 r0 = rare[half];
+          w.x &= ~static_cast<uint32_t>(r0.y);
+          w.y &= ~static_cast<uint32_t>(r0.w);
+          careful |= (r0.x | r0.z) != 0;
           const float mx = c_row * (careful ? half_max_masked(s_addr, f, w.x, w.y) : half_max(s_addr, f));
           // The rows' running maximum goes from granule to granule, between the two warps that
           // share the rows.  It is lazy: it moves only when a granule exceeds it by 2^8, so P

@@ -225,6 +225,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
       }
       const int32_t* table = p.block_tables + static_cast<int64_t>(it.r) * p.table_stride0;
       int batch = -1, pages = -1;  // a lane's box of 32 consecutive ones, looked up together
+      uint32_t lost = 0;           // those of them whose page lies outside the pool
 #pragma unroll 1
       for (int t = 0; t < it.n; ++t) {
         const uint32_t g = g0 + t, stage = g % kFewStages;
@@ -238,10 +239,12 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
           batch = (tile * boxes) >> 5;
           const int pos = (32 * batch + lane) * plan.box;
           pages = pos < it.P ? __ldg(table + pos / p.block_size) : -1;
-          if (pos < it.P && (pages < 0 || pages >= p.num_blocks)) {
+          const bool bad = pos < it.P && (pages < 0 || pages >= p.num_blocks);
+          if (bad) {
             atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
             pages = -1;
           }
+          lost = __ballot_sync(0xffffffffu, bad);
         }
         KeyPlace at[4];
         if (!tma) {
@@ -259,10 +262,11 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
           if (lane == 0) mbar_arrive_tx(full, 2 * kTile8 + 2 * kN);
           __syncwarp();
           const int page = __shfl_sync(0xffffffffu, pages, (tile * boxes + lane) & 31);
-          const uint32_t out = __ballot_sync(0xffffffffu, lane < boxes && page < 0);
-          if (lane < 4) {
+          if (lost == 0) {
+            if (lane == 0) *reinterpret_cast<int4*>(none) = make_int4(0, 0, 0, 0);
+          } else if (lane < 4) {
             // This word's 32 keys lie in one box, or in two of 16.
-            const uint32_t b = out >> (32 * lane / plan.box);
+            const uint32_t b = lost >> (((tile * boxes) & 31) + 32 * lane / plan.box);
             none[lane] = plan.box >= 32 ? (b & 1u ? ~0u : 0u) : (b & 1u ? 0xffffu : 0u) | (b & 2u ? ~0xffffu : 0u);
           }
           if (lane < boxes) {
