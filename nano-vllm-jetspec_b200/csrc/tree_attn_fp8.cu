@@ -430,10 +430,7 @@ __device__ __forceinline__ ItemInfo item_info(const Geometry& ge, int P, int T, 
 __device__ __noinline__ int2 load_request(const JtTreeAttnFp8Params& p, int r, bool flag) {
   int P = __ldg(p.prefix_lens + r), T = __ldg(p.node_counts + r);
   const int64_t capacity = static_cast<int64_t>(p.table_width) * p.block_size;
-  if (T > kMaxNodes) {
-    if (flag) atomicOr(&g_attn_fp8_errors, JT_DEVERR_TREE_TOO_LARGE);
-    T = 0;
-  }
+  if (T > kMaxNodes) T = 0;  // clear_refused
   if (P < 0 || P > capacity) {
     if (flag) atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
     P = P < 0 ? 0 : static_cast<int>(capacity);
@@ -497,6 +494,39 @@ __host__ __device__ __forceinline__ Workspace carve(void* base, int64_t nodes = 
                    reinterpret_cast<uint8_t*>(q + factor_bytes(nodes * groups, heads) + mask_bytes(nodes))};
 }
 
+// Zeros for the rows of requests that no kernel of the launch takes, and the error bit that says
+// why: what else they would hold is whatever lay in the caller's memory.  One warp per CTA of
+// one of the launch's kernels, which share the requests out.
+__device__ __noinline__ void clear_refused(const JtTreeAttnFp8Params& p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t stride = gridDim.x;
+  for (int64_t first = blockIdx.x; first < p.num_requests; first += 32 * stride) {
+    const int64_t r = first + lane * stride;
+    int T = 0, q0 = 0;
+    if (r < p.num_requests) {
+      T = __ldg(p.node_counts + r);
+      q0 = __ldg(p.cu_seqlens_q + r);
+    }
+    const bool large = T > kMaxNodes;
+    if (large) atomicOr(&g_attn_fp8_errors, JT_DEVERR_TREE_TOO_LARGE);
+    uint32_t todo = __ballot_sync(0xffffffffu, large);
+    for (; todo != 0; todo &= todo - 1) {
+      const int src = __ffs(todo) - 1;
+      const int64_t q = __shfl_sync(0xffffffffu, q0, src), n = __shfl_sync(0xffffffffu, T, src);
+      const int64_t lo = max(q, static_cast<int64_t>(0));
+      const int64_t hi = min(q + n, static_cast<int64_t>(p.total_queries));
+      const int heads = p.num_kv_heads * p.groups, size = p.out_dtype == JT_F32 ? 4 : 2;
+      const int words = p.head_dim * size / 16;  // per head, 16 bytes each
+      for (int64_t i = lane; i < (hi - lo) * heads * words; i += 32) {
+        const int64_t row = i / (heads * words);
+        const int rest = static_cast<int>(i - row * (heads * words)), head = rest / words;
+        char* dst = static_cast<char*>(p.out) + ((lo + row) * p.out_stride0 + head * p.out_stride1) * size;
+        reinterpret_cast<uint4*>(dst)[rest - head * words] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  }
+}
+
 // Page and offset of key position `pos` of a piece, page -1 past its keys or out of the pool.
 struct KeyPlace {
   int64_t page;
@@ -546,6 +576,7 @@ __device__ __noinline__ void lose_keys(uint32_t words, int lo, int hi) {
 struct LoadPlan {
   int tma;   // prefix tiles by TMA boxes of `box` keys, their scale bytes by bulk copies
   int box;
+  int alone;  // the few-row kernel runs without the other one
 };
 
 // Visibility words of 64 keys for a row, from its node's bits: bit b of the first word is the key
@@ -951,6 +982,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();  // the scan area is free
   // From here on the query terms are complete, and so is every earlier use of the workspace.
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  if (warp == kThreads / 32 - 1) clear_refused(p);
 
   // Pieces: a two-entry ring in shared memory, filled one piece ahead by warp 1's first lane.
   volatile int* item_ring = reinterpret_cast<volatile int*>(sbase + L::kItem);
@@ -1685,6 +1717,7 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
   const int64_t least = static_cast<int64_t>(known ? std::max(p.min_nodes, 1) : 1) * p.groups;
   const int64_t most = known ? static_cast<int64_t>(p.max_nodes) * p.groups : kFewRows + 1;
   if (least <= kFewRows) {
+    plan.alone = most <= kFewRows;
     rc = most <= 8 ? launch_few<1, kWide, QT>(p, plan, kmap, vmap, grid, stream)
                              : launch_few<2, kWide, QT>(p, plan, kmap, vmap, grid, stream);
     if (rc != JT_OK || most <= kFewRows) return rc;

@@ -314,6 +314,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
 
   // -------------------------------------------------------------------- keys
   const int w = warp - 1;
+  if (w == F::kWarps - 1 && plan.alone) clear_refused(p);
   const int g8 = lane >> 2, q4 = lane & 3;
   const float log2e = 1.4426950408889634f;
   float* o_place = reinterpret_cast<float*>(sbase + F::kO);

@@ -1,0 +1,51 @@
+"""Requests that packed_tree_attention_fp8 does not take: their rows are zeros and a device error bit
+is set, whatever the output's memory held; the other requests' rows are what they are alone.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import jetspec_b200 as jb
+from jetspec_b200 import tree_fp8
+
+from helpers import bits_equal
+from test_gpu_tree_fp8 import DEVICE, Case
+from test_gpu_tree_fp8_few import namespace
+
+pytestmark = pytest.mark.gpu
+
+
+def run(case, meta, dtype=torch.bfloat16):
+    """The launch into memory that holds sevens, with sevens before and after it."""
+    shape = (case.q.shape[0] + 16, *case.q.shape[1:])
+    memory = torch.full(shape, 7.0, dtype=dtype, device=DEVICE)
+    out = memory[8:-8]
+    tree_fp8._launch_attention(out, case.q, case.k, case.v, case.ks, case.vs, meta, case.scale,
+                               case.batch.groups)
+    torch.cuda.synchronize()
+    assert (memory[:8] == 7).all() and (memory[-8:] == 7).all()
+    return out
+
+
+def rows(case, r):
+    o = case.meta.cu_seqlens_q.tolist()
+    return slice(o[r], o[r + 1])
+
+
+@pytest.mark.parametrize("counts", [[3, 1030, 40], [1100], [64, 1025, 2000, 1]])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_trees_of_more_than_1024_nodes(counts, dtype):
+    """Known too large on the device only: the host's counts are not given."""
+    case = Case([200 + i for i in range(len(counts))], counts, kv_heads=1, groups=2, seed=31)
+    meta = namespace(case.meta, node_counts_host=None)
+    jb.read_device_errors()
+    got = run(case, meta, dtype)
+    assert jb.read_device_errors() == 2
+    small = [r for r, n in enumerate(counts) if n <= 1024]
+    for r, n in enumerate(counts):
+        if n > 1024:
+            assert (got[rows(case, r)] == 0).all()
+    if small:
+        case.run = lambda **kw: got
+        case.check(small)
