@@ -444,7 +444,8 @@ int32_t jt_kv_fp8_commit_max_slots(void);
  * bf16's range saturate (requests of more than 16 rows).  Requests with no
  * nodes are allowed.  Strides of the pools and scales in bytes, of q and out in elements,
  * last dimensions contiguous; pool rows 16-byte aligned (head_dim a multiple of 16, at most
- * 128), at most 1024 nodes per tree (larger: device error bit 1, the rows are zeros).
+ * 128), at most 1024 nodes per tree (larger: device error bit 1, the rows are zeros).  A request
+ * whose nodes leave [0, total_queries) sets device error bit 0; its rows in range are zeros.
  */
 typedef struct JtTreeAttnFp8Params {
   void* out;                       /* [total_queries, q_heads, head_dim], out_dtype      */

@@ -430,7 +430,9 @@ __device__ __forceinline__ ItemInfo item_info(const Geometry& ge, int P, int T, 
 __device__ __noinline__ int2 load_request(const JtTreeAttnFp8Params& p, int r, bool flag) {
   int P = __ldg(p.prefix_lens + r), T = __ldg(p.node_counts + r);
   const int64_t capacity = static_cast<int64_t>(p.table_width) * p.block_size;
-  if (T > kMaxNodes) T = 0;  // clear_refused
+  // Refused: clear_refused.
+  const int q0 = __ldg(p.cu_seqlens_q + r);
+  if (T > kMaxNodes || q0 < 0 || T > p.total_queries - q0) T = 0;
   if (P < 0 || P > capacity) {
     if (flag) atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
     P = P < 0 ? 0 : static_cast<int>(capacity);
@@ -507,9 +509,10 @@ __device__ __noinline__ void clear_refused(const JtTreeAttnFp8Params& p) {
       T = __ldg(p.node_counts + r);
       q0 = __ldg(p.cu_seqlens_q + r);
     }
-    const bool large = T > kMaxNodes;
+    const bool large = T > kMaxNodes, astray = T > 0 && (q0 < 0 || T > p.total_queries - q0);
     if (large) atomicOr(&g_attn_fp8_errors, JT_DEVERR_TREE_TOO_LARGE);
-    uint32_t todo = __ballot_sync(0xffffffffu, large);
+    if (astray) atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
+    uint32_t todo = __ballot_sync(0xffffffffu, large || astray);
     for (; todo != 0; todo &= todo - 1) {
       const int src = __ffs(todo) - 1;
       const int64_t q = __shfl_sync(0xffffffffu, q0, src), n = __shfl_sync(0xffffffffu, T, src);

@@ -49,3 +49,35 @@ def test_trees_of_more_than_1024_nodes(counts, dtype):
     if small:
         case.run = lambda **kw: got
         case.check(small)
+
+
+@pytest.mark.parametrize("groups,counts,known", [(1, (5, 9, 4), True), (4, (5, 9, 4), False),
+                                                 (4, (50, 90, 40), True), (4, (50, 3, 1), False)])
+def test_nodes_past_the_packed_rows(groups, counts, known):
+    """Device counts and offsets that leave the rows of the call: nothing is written past them."""
+    case = Case([300, 40, 900], counts, kv_heads=2, groups=groups, seed=32)
+    total, m = sum(counts), case.meta
+    late = total - counts[2] + 3  # the last request begins three rows on
+    bias = torch.cat([m.qq_bias.view(-1), m.qq_bias.new_zeros(4096)])
+    for cu, bad in (([0, counts[0], late, total], [2]), ([-2, counts[0], total - counts[2], total], [0]),
+                    ([0, counts[0], total, total], [2])):
+        meta = namespace(m, cu_seqlens_q=torch.tensor(cu, dtype=torch.int32, device=DEVICE),
+                         qq_bias=bias, **({} if known else {"node_counts_host": None}))
+        jb.read_device_errors()
+        got = run(case, meta)
+        assert jb.read_device_errors() == 1
+        good = [r for r in range(3) if r not in bad]
+        for r in bad:
+            lo, hi = max(cu[r], 0), min(cu[r] + counts[r], total)
+            assert (got[lo:hi] == 0).all()
+        case.run = lambda **kw: got
+        case.check(good)
+    counts_up = m.node_counts.clone()
+    counts_up[2] += 6
+    meta = namespace(m, node_counts=counts_up, qq_bias=bias,
+                     **({} if known else {"node_counts_host": None}))
+    got = run(case, meta)
+    assert jb.read_device_errors() == 1
+    assert (got[rows(case, 2)] == 0).all()
+    case.run = lambda **kw: got
+    case.check([0, 1])
