@@ -478,8 +478,9 @@ typedef struct JtTreeAttnFp8Params {
   int32_t out_dtype;               /* dtype or JT_F32                                   */
   int32_t min_nodes, max_nodes;    /* least (above 0) and largest node count of a request when
                                       the host knows them, 0, 0 when it does not (and not
-                                      used for a launch under stream capture): requests
-                                      outside them may be left out                         */
+                                      used for a launch under stream capture).  They decide
+                                      which kernels run: a request whose rows none of them
+                                      takes sets device error bit 0, its rows are zeros    */
 } JtTreeAttnFp8Params;
 
 int jt_tree_attn_fp8_launch(const JtTreeAttnFp8Params* params, cudaStream_t stream);

@@ -54,6 +54,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "common.cuh"
 
@@ -498,8 +499,9 @@ __host__ __device__ __forceinline__ Workspace carve(void* base, int64_t nodes = 
 
 // Zeros for the rows of requests that no kernel of the launch takes, and the error bit that says
 // why: what else they would hold is whatever lay in the caller's memory.  One warp per CTA of
-// one of the launch's kernels, which share the requests out.
-__device__ __noinline__ void clear_refused(const JtTreeAttnFp8Params& p) {
+// one of the launch's kernels, which share the requests out.  `least` and `most`: the rows that
+// the launched kernels take.
+__device__ __noinline__ void clear_refused(const JtTreeAttnFp8Params& p, int least, int most) {
   const int lane = threadIdx.x & 31;
   const int64_t stride = gridDim.x;
   for (int64_t first = blockIdx.x; first < p.num_requests; first += 32 * stride) {
@@ -509,7 +511,9 @@ __device__ __noinline__ void clear_refused(const JtTreeAttnFp8Params& p) {
       T = __ldg(p.node_counts + r);
       q0 = __ldg(p.cu_seqlens_q + r);
     }
-    const bool large = T > kMaxNodes, astray = T > 0 && (q0 < 0 || T > p.total_queries - q0);
+    const bool large = T > kMaxNodes;
+    const bool astray = T > 0 && (q0 < 0 || T > p.total_queries - q0 ||
+                                  (!large && (T * p.groups < least || T * p.groups > most)));
     if (large) atomicOr(&g_attn_fp8_errors, JT_DEVERR_TREE_TOO_LARGE);
     if (astray) atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
     uint32_t todo = __ballot_sync(0xffffffffu, large || astray);
@@ -579,7 +583,7 @@ __device__ __noinline__ void lose_keys(uint32_t words, int lo, int hi) {
 struct LoadPlan {
   int tma;   // prefix tiles by TMA boxes of `box` keys, their scale bytes by bulk copies
   int box;
-  int alone;  // the few-row kernel runs without the other one
+  int alone;  // the kernel of few rows or the one of many runs without the other
 };
 
 // Visibility words of 64 keys for a row, from its node's bits: bit b of the first word is the key
@@ -985,7 +989,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();  // the scan area is free
   // From here on the query terms are complete, and so is every earlier use of the workspace.
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  if (warp == kThreads / 32 - 1) clear_refused(p);
+  if (warp == kThreads / 32 - 1) clear_refused(p, plan.alone ? kFewRows + 1 : 1, INT_MAX);
 
   // Pieces: a two-entry ring in shared memory, filled one piece ahead by warp 1's first lane.
   volatile int* item_ring = reinterpret_cast<volatile int*>(sbase + L::kItem);
@@ -1725,6 +1729,7 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
                              : launch_few<2, kWide, QT>(p, plan, kmap, vmap, grid, stream);
     if (rc != JT_OK || most <= kFewRows) return rc;
   }
+  plan.alone = least > kFewRows;
   const int64_t rows = static_cast<int64_t>(p.total_queries) * p.groups;
   CUtensorMap qmap{};
   if (!encode_queries(&qmap, carve(p.workspace, p.total_queries, p.groups, p.num_kv_heads).q_terms, rows,

@@ -82,15 +82,15 @@ struct FewCursor {
   int r, h, P, T;
   bool more;
 };
-__device__ __forceinline__ int2 few_request(const JtTreeAttnFp8Params& p, int r, bool flag) {
+__device__ __forceinline__ int2 few_request(const JtTreeAttnFp8Params& p, int r, bool flag, int most) {
   int2 q = load_request(p, r, flag);
-  if (q.y * p.groups > kFewRows) q.y = 0;  // the other kernel's
+  if (q.y * p.groups > most) q.y = 0;  // the other kernel's, or clear_refused
   return q;
 }
 __device__ __forceinline__ int few_cost(int P, int T) {
   return T == 0 ? 0 : ((P + T + kN - 1) >> 7) + kFewItemCost;
 }
-__device__ __noinline__ bool few_next(const JtTreeAttnFp8Params& p, FewCursor& c, FewPiece& it) {
+__device__ __noinline__ bool few_next(const JtTreeAttnFp8Params& p, FewCursor& c, FewPiece& it, int most) {
   while (c.more) {
     const int n = (c.P + c.T + kN - 1) >> 7;
     const ItemInfo info{c.P + c.T, n, 0, 1, n + kFewItemCost};
@@ -110,7 +110,7 @@ __device__ __noinline__ bool few_next(const JtTreeAttnFp8Params& p, FewCursor& c
       c.h = 0;
       c.T = 0;
       while (c.T == 0 && ++c.r < p.num_requests) {
-        const int2 q = few_request(p, c.r, false);
+        const int2 q = few_request(p, c.r, false, most);
         c.P = q.x;
         c.T = q.y;
       }
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
   const int r_lo = min(tid * per, R), r_hi = min(r_lo + per, R);
   int64_t mine = 0;
   for (int r = r_lo; r < r_hi; ++r) {
-    const int2 q = few_request(p, r, blockIdx.x == 0);
+    const int2 q = few_request(p, r, blockIdx.x == 0, F::kRows);
     mine += static_cast<int64_t>(few_cost(q.x, q.y)) * p.num_kv_heads;
   }
   int64_t incl = mine;
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
   if (has_part && mine > 0 && my_start <= cur.x0 && cur.x0 < my_start + mine) {
     int64_t s = my_start;
     for (int r = r_lo; r < r_hi; ++r) {
-      const int2 q = few_request(p, r, false);
+      const int2 q = few_request(p, r, false, F::kRows);
       const int64_t c = static_cast<int64_t>(few_cost(q.x, q.y)) * p.num_kv_heads;
       if (cur.x0 < s + c) {
         scan[32] = r;
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
   cur.more = has_part;
   if (has_part) {
     cur.r = static_cast<int>(scan[32]);
-    const int2 q = few_request(p, cur.r, false);
+    const int2 q = few_request(p, cur.r, false, F::kRows);
     cur.P = q.x;
     cur.T = q.y;
     const int64_t s = scan[33], c = few_cost(q.x, q.y);
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
     bool dead = false, gathered = false;
     uint32_t issued = 0;
 #pragma unroll 1
-    while (!dead && few_next(p, cur, it)) {
+    while (!dead && few_next(p, cur, it, F::kRows)) {
       if (it.slot >= 0) {
         const int which = it.slot & 1;
         meta_valid[which] = 1;
@@ -314,14 +314,14 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
 
   // -------------------------------------------------------------------- keys
   const int w = warp - 1;
-  if (w == F::kWarps - 1 && plan.alone) clear_refused(p);
+  if (w == F::kWarps - 1 && plan.alone) clear_refused(p, 1, F::kRows);
   const int g8 = lane >> 2, q4 = lane & 3;
   const float log2e = 1.4426950408889634f;
   float* o_place = reinterpret_cast<float*>(sbase + F::kO);
   float4* ml_place = reinterpret_cast<float4*>(sbase + F::kMl);
 #pragma unroll 1
-  while (few_next(p, cur, it)) {  // to the end even after a wait that ran out: the warps meet
-    const int rows = min(it.T * p.groups, F::kRows);
+  while (few_next(p, cur, it, F::kRows)) {  // to the end even after a wait that ran out: the warps meet
+    const int rows = it.T * p.groups;
     // Q fragments: row g8 of each n-tile, dims 32 q4 .. 32 q4 + 31, as f16 of row / 2^e.
     uint32_t qf[NT][16];
     float c_row[NT][2];  // factors of rows 2 q4 and 2 q4 + 1

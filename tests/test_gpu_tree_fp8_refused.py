@@ -81,3 +81,34 @@ def test_nodes_past_the_packed_rows(groups, counts, known):
     assert (got[rows(case, 2)] == 0).all()
     case.run = lambda **kw: got
     case.check([0, 1])
+
+
+@pytest.mark.parametrize("groups,host,device,taken", [
+    (4, (4, 4, 3), (1, 9, 1), (0, 2)),          # only few rows known: a tree of 36 is not taken
+    (4, (2, 2, 1), (1, 3, 1), (0, 2)),          # up to 8 rows known: nor is one of 12
+    (4, (40, 20, 30), (44, 3, 43), (0, 2)),     # only large trees known: nor one of 12
+    (4, (40, 20, 30), (20, 30, 40), (0, 1, 2)),  # other counts that the same kernel takes
+    (4, (3, 40, 5), (40, 3, 5), (0, 1, 2)),     # both kernels run: all are taken
+])
+def test_host_counts_that_are_not_the_devices(groups, host, device, taken):
+    case = Case([300, 40, 900], device, kv_heads=2, groups=groups, seed=33)
+    assert sum(host) == sum(device)
+    meta = namespace(case.meta, node_counts_host=host)
+    jb.read_device_errors()
+    got = run(case, meta)
+    assert jb.read_device_errors() == (0 if len(taken) == 3 else 1)
+    for r in range(3):
+        if r not in taken:
+            assert (got[rows(case, r)] == 0).all()
+    case.run = lambda **kw: got
+    case.check(list(taken))
+
+
+def test_a_tree_above_1024_nodes_where_few_rows_are_known():
+    case = Case([300, 40], [1030, 2], kv_heads=2, groups=1, seed=34)
+    jb.read_device_errors()
+    got = run(case, namespace(case.meta, node_counts_host=(8, 2)))
+    assert jb.read_device_errors() == 2
+    assert (got[:1030] == 0).all()
+    case.run = lambda **kw: got
+    case.check([1])
