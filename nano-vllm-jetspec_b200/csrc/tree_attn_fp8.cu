@@ -498,9 +498,9 @@ __host__ __device__ __forceinline__ Workspace carve(void* base, int64_t nodes = 
 }
 
 // Zeros for the rows of requests that no kernel of the launch takes, and the error bit that says
-// why: what else they would hold is whatever lay in the caller's memory.  One warp per CTA of
-// one of the launch's kernels, which share the requests out.  `least` and `most`: the rows that
-// the launched kernels take.
+// why: what else they would hold is whatever lay in the caller's memory.  `least` and `most`: the
+// rows that the launched kernels take.  A warp per CTA of the launch's last merge kernel, ahead of
+// its wait (nothing else writes these rows): beside the attention's own warps it cost 2 to 3 %.
 __device__ __noinline__ void clear_refused(const JtTreeAttnFp8Params& p, int least, int most) {
   const int lane = threadIdx.x & 31;
   const int64_t stride = gridDim.x;
@@ -583,7 +583,6 @@ __device__ __noinline__ void lose_keys(uint32_t words, int lo, int hi) {
 struct LoadPlan {
   int tma;   // prefix tiles by TMA boxes of `box` keys, their scale bytes by bulk copies
   int box;
-  int alone;  // the kernel of few rows or the one of many runs without the other
 };
 
 // Visibility words of 64 keys for a row, from its node's bits: bit b of the first word is the key
@@ -989,7 +988,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();  // the scan area is free
   // From here on the query terms are complete, and so is every earlier use of the workspace.
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  if (warp == kThreads / 32 - 1) clear_refused(p, plan.alone ? kFewRows + 1 : 1, INT_MAX);
 
   // Pieces: a two-entry ring in shared memory, filled one piece ahead by warp 1's first lane.
   volatile int* item_ring = reinterpret_cast<volatile int*>(sbase + L::kItem);
@@ -1579,7 +1577,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // slots 2(c + 1), 2(c + 2), ... up to the one that finishes it.
 template <bool kWide>
 __global__ void __launch_bounds__(kM) tree_attn_fp8_merge_kernel(
-    const __grid_constant__ JtTreeAttnFp8Params p, const int parts) {
+    const __grid_constant__ JtTreeAttnFp8Params p, const int parts, const int least) {
+  if (blockIdx.y == 0 && threadIdx.x < 32) clear_refused(p, least, INT_MAX);
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const Workspace w = carve(p.workspace);
   const int c = blockIdx.x, tile = blockIdx.y >> 3, cg0 = (blockIdx.y & 7) * 4, row = threadIdx.x;
@@ -1724,12 +1723,10 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
   const int64_t least = static_cast<int64_t>(known ? std::max(p.min_nodes, 1) : 1) * p.groups;
   const int64_t most = known ? static_cast<int64_t>(p.max_nodes) * p.groups : kFewRows + 1;
   if (least <= kFewRows) {
-    plan.alone = most <= kFewRows;
-    rc = most <= 8 ? launch_few<1, kWide, QT>(p, plan, kmap, vmap, grid, stream)
-                             : launch_few<2, kWide, QT>(p, plan, kmap, vmap, grid, stream);
+    rc = most <= 8 ? launch_few<1, kWide, QT>(p, plan, kmap, vmap, grid, true, stream)
+                   : launch_few<2, kWide, QT>(p, plan, kmap, vmap, grid, most <= kFewRows, stream);
     if (rc != JT_OK || most <= kFewRows) return rc;
   }
-  plan.alone = least > kFewRows;
   const int64_t rows = static_cast<int64_t>(p.total_queries) * p.groups;
   CUtensorMap qmap{};
   if (!encode_queries(&qmap, carve(p.workspace, p.total_queries, p.groups, p.num_kv_heads).q_terms, rows,
@@ -1751,7 +1748,8 @@ int launch(const JtTreeAttnFp8Params& p, int sms, cudaStream_t stream) {
                         "tree_attn_fp8 launch", p, kmap, vmap, qmap, plan);
   if (rc != JT_OK) return rc;
   return launch_dependent(tree_attn_fp8_merge_kernel<kWide>, dim3(grid, 8 * Smem<kWide>::kTiles), kM,
-                          0, stream, "tree_attn_fp8 merge launch", p, grid);
+                          0, stream, "tree_attn_fp8 merge launch", p, grid,
+                           static_cast<int>(least > kFewRows ? kFewRows + 1 : 1));
 }
 
 }  // namespace

@@ -314,7 +314,6 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
 
   // -------------------------------------------------------------------- keys
   const int w = warp - 1;
-  if (w == F::kWarps - 1 && plan.alone) clear_refused(p, 1, F::kRows);
   const int g8 = lane >> 2, q4 = lane & 3;
   const float log2e = 1.4426950408889634f;
   float* o_place = reinterpret_cast<float*>(sbase + F::kO);
@@ -583,7 +582,9 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
 // a later one, a warp per row.
 template <bool kWide>
 __global__ void __launch_bounds__(32 * kFewRows) tree_attn_fp8_few_merge_kernel(
-    const __grid_constant__ JtTreeAttnFp8Params p, const int parts) {
+    const __grid_constant__ JtTreeAttnFp8Params p, const int parts, const int most) {
+  // With no kernel after it for the requests that this one does not take.
+  if (most > 0 && threadIdx.x < 32) clear_refused(p, 1, most);
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const Workspace w = carve(p.workspace);
   const int c = blockIdx.x, row = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -614,7 +615,7 @@ __global__ void __launch_bounds__(32 * kFewRows) tree_attn_fp8_few_merge_kernel(
 
 template <int NT, bool kWide, typename QT>
 int launch_few(const JtTreeAttnFp8Params& p, const LoadPlan& plan, const CUtensorMap& kmap,
-               const CUtensorMap& vmap, int grid, cudaStream_t stream) {
+               const CUtensorMap& vmap, int grid, bool alone, cudaStream_t stream) {
   auto kernel = tree_attn_fp8_few_kernel<NT, kWide, QT>;
   int rc = jt_cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                               Few<NT>::kBytes),
@@ -624,5 +625,5 @@ int launch_few(const JtTreeAttnFp8Params& p, const LoadPlan& plan, const CUtenso
   rc = jt_cuda_check(cudaGetLastError(), "tree_attn_fp8 few rows launch");
   if (rc != JT_OK) return rc;
   return launch_dependent(tree_attn_fp8_few_merge_kernel<kWide>, dim3(grid), 32 * kFewRows, 0, stream,
-                          "tree_attn_fp8 few rows merge launch", p, grid);
+                          "tree_attn_fp8 few rows merge launch", p, grid, alone ? Few<NT>::kRows : 0);
 }
