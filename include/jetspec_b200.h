@@ -440,7 +440,9 @@ int32_t jt_kv_fp8_commit_max_slots(void);
  * of up to 16 rows, nodes x groups: f16, and 22 bits).  A query
  * row that sees no key gives zeros; a row that sees a key whose K or V scale is NaN gives
  * NaN; keys a row does not see never reach it, whatever their bytes hold.  A key whose page or
- * slot lies outside the pool is left out and sets device error bit 0.  V values past
+ * slot lies outside the pool is left out and sets device error bit 0.  A NaN code of K makes NaN of
+ * the rows that see its key, one of V of their element (of the whole row from the 128-key tile on
+ * in which the prefix ends).  V values past
  * bf16's range saturate (requests of more than 16 rows).  Requests with no
  * nodes are allowed.  Strides of the pools and scales in bytes, of q and out in elements,
  * last dimensions contiguous; pool rows 16-byte aligned (head_dim a multiple of 16, at most

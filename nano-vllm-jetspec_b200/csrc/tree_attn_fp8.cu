@@ -374,12 +374,35 @@ __device__ __forceinline__ uint2 v_multipliers(uint32_t b) {
 // Four e4m3 codes as bf16 pairs of value * 2^-120: the code's exponent and mantissa fields
 // dropped into bf16's (subnormal codes become bf16 subnormals of the same value).  The pairs
 // are codes (0, 2) and (1, 3), which saves the byte permutes: the V tile's columns, and so O's,
-// hold the head dims in the order 0, 2, 1, 3 of every four, undone where O is written out.  The
-// code 0x7f (NaN), which no row of this cache holds, reads as 480: finite, so bytes of keys
-// no row sees never reach the product.
+// hold the head dims in the order 0, 2, 1, 3 of every four, undone where O is written out.  A NaN
+// code (0x7f, 0xff), which this package's writer never makes, comes out as 480.  set_nan_codes puts
+// the NaN where it belongs in tiles whose keys every row sees; in the others it would reach the
+// rows that do not see the key as 0 x NaN: there the merge kernel gives it to the rows that do.
 __device__ __forceinline__ void widen(uint32_t w, uint32_t& even, uint32_t& odd) {
   even = (w & 0x007f007fu) * 16u + (w & 0x00800080u) * 256u;
   odd = ((w >> 4) & 0x07f007f0u) | (w & 0x80008000u);
+}
+// The high bit of the bytes that hold a NaN code (other bits: noise).
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u; }
+__device__ __forceinline__ uint32_t nan_codes(uint4 w) {
+  return (nan_codes(w.x) | nan_codes(w.y) | nan_codes(w.z) | nan_codes(w.w)) & 0x80808080u;
+}
+// NaN where the codes of a converter warp's 32 V rows are NaN, in their bf16 rows: a row per lane.
+__device__ __noinline__ void set_nan_codes(const unsigned char* src, unsigned char* dst) {
+  const int row = threadIdx.x & 31;
+#pragma unroll 1
+  for (int c = 0; c < 16; ++c) {  // eight codes: two words
+    const uint2 w = *reinterpret_cast<const uint2*>(src + row * 128 + (((c >> 1) ^ (row & 7)) << 4) + 8 * (c & 1));
+    const uint32_t t[2] = {nan_codes(w.x), nan_codes(w.y)};
+    uint4* o = reinterpret_cast<uint4*>(dst + (c >> 3) * kHalf16 + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+    if (((t[0] | t[1]) & 0x80808080u) == 0) continue;
+    uint4 v = *o;
+    v.x |= ((t[0] >> 7) & 0x00010001u) * 0x7fffu;
+    v.y |= ((t[0] >> 15) & 0x00010001u) * 0x7fffu;
+    v.z |= ((t[1] >> 7) & 0x00010001u) * 0x7fffu;
+    v.w |= ((t[1] >> 15) & 0x00010001u) * 0x7fffu;
+    *o = v;
+  }
 }
 __device__ __forceinline__ constexpr int o_column(int d) {  // column of head dim d in O
   return (d & ~3) | ((d & 1) << 1) | ((d >> 1) & 1);
@@ -466,7 +489,9 @@ struct Piece {
 };
 // A piece's partial slot in the workspace, or -1 for a whole item.
 struct PieceMeta {
-  int valid, finishes, r, h, mb, pad[3];
+  int valid, finishes, r, h, mb;
+  int nan;  // the CTA has met NaN codes of V in tiles with masked keys
+  int pad[2];
 };
 struct Workspace {
   PieceMeta* meta;   // [2 * kMaxCtas]
@@ -564,6 +589,55 @@ __device__ __noinline__ void gather_row(uint32_t dst, int row, const char* src, 
   for (int c = 0; c < 8; ++c)
     jt::cp_async_16(dst + row * 128 + ((c ^ (row & 7)) << 4), c < chunks ? src + 16 * c : src,
                     c < chunks ? 16 : 0);
+}
+
+// V codes that are NaN in tiles with masked keys: whoever meets one notes it for the CTA's pieces,
+// and the merge kernel makes NaN of the rows that see its key, node by node.  Asked in the
+// attention's own epilogue the question took 3 % of a serving mix, asked in the few-row kernel's
+// loop 1.5 % of a long decode.
+__device__ __noinline__ void note_nan_codes(const JtTreeAttnFp8Params& p) {
+  PieceMeta* m = carve(p.workspace).meta + 2 * blockIdx.x;
+  m[0].nan = m[1].nan = 1;
+}
+__device__ __noinline__ bool sees_nan_code(const JtTreeAttnFp8Params& p, int r, int2 request, int h, int j) {
+  const int P = request.x, q_start = __ldg(p.cu_seqlens_q + r), key_end = P + j + 1;
+  const int32_t* table = p.block_tables + static_cast<int64_t>(r) * p.table_stride0;
+  const float* bias = p.qq_bias + __ldg(p.qq_bias_offsets + r) + static_cast<int64_t>(j) * request.y;
+#pragma unroll 1
+  for (int pos = P / kN * kN; pos < key_end; ++pos) {
+    if (pos >= P && bias[pos - P] != 0.f) continue;
+    const KeyPlace at = locate_key(p, table, pos, P, key_end, q_start);
+    if (at.page < 0) continue;
+    const uint4* row = reinterpret_cast<const uint4*>(static_cast<const char*>(p.v_pool) + at.page * p.v_stride0 +
+                                                      at.off * p.v_stride1 + h * p.v_stride2);
+#pragma unroll 1
+    for (int c = 0; c < p.head_dim / 16; ++c)
+      if (nan_codes(row[c]) != 0) return true;
+  }
+  return false;
+}
+// The same for every node and KV head of the requests of `least` to `most` rows, by one block.
+// Rows of cut items are merged by other blocks, which make NaN of the same ones.
+__device__ __noinline__ void spread_nan_codes(const JtTreeAttnFp8Params& p, int least, int most) {
+  const int size = p.out_dtype == JT_F32 ? 4 : 2, words = p.head_dim * size / 16;
+#pragma unroll 1
+  for (int r = 0; r < p.num_requests; ++r) {
+    const int2 q = load_request(p, r, false);
+    if (q.y * p.groups < least || q.y * p.groups > most) continue;
+    const int64_t q_start = __ldg(p.cu_seqlens_q + r);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < q.y * p.num_kv_heads; i += blockDim.x) {
+      const int j = i / p.num_kv_heads, h = i - j * p.num_kv_heads;
+      if (!sees_nan_code(p, r, q, h, j)) continue;
+#pragma unroll 1
+      for (int k = 0; k < p.groups * words; ++k) {
+        const int head = h * p.groups + k / words;
+        char* dst = static_cast<char*>(p.out) + ((q_start + j) * p.out_stride0 + head * p.out_stride1) * size;
+        // NaN as one 32-bit value and as two of either 16-bit type.
+        reinterpret_cast<uint4*>(dst)[k % words] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+      }
+    }
+  }
 }
 
 // Marks keys lo to hi - 1 of a tile, in sixteens, as without a place in the pool.  Out of line,
@@ -1163,7 +1237,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         mine = (mine & ~(1u << bit)) | (by_tma ? 1u << bit : 0u);
         parity = (parity & ~(1u << bit)) | ((phase & 1u) << bit);
       };
-      if (lane == 0) publish(0);
+      if (lane == 0) {
+        PieceMeta* m = carve(p.workspace).meta + 2 * blockIdx.x;
+        m[0].nan = m[1].nan = 0;
+        publish(0);
+      }
       const char* ksc = static_cast<const char*>(p.k_scale);
       const char* vsc = static_cast<const char*>(p.v_scale);
       for (uint32_t seq = 0;; ++seq) {
@@ -1356,6 +1434,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // This warp's 32 rows x 8 chunks in 8 rounds, four rounds' loads in flight at a time.
         const unsigned char* src = sbase + L::kV8 + (g % kVRing) * kTile8 + cw * (32 * 128);
         unsigned char* dst = sbase + L::kV16 + buf * kTile16 + v_half * kHalf16 + cw * (32 * 128);
+        uint32_t nan = 0;
 #pragma unroll 1
         for (int i0 = 0; i0 < 8; i0 += 4) {
           uint4 w[4];
@@ -1371,6 +1450,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int row = ((i0 + i) >> 1) * 8 + ((sub & 4) ? (pr ^ 5) : pr);
             const uint32_t m = __shfl_sync(0xffffffffu, mine.x, row);
             uint32_t o[8];
+            nan |= nan_codes(w[i]);
             widen(w[i].x, o[0], o[1]);
             widen(w[i].y, o[2], o[3]);
             widen(w[i].z, o[4], o[5]);
@@ -1388,6 +1468,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<uint4*>(row_dst + ((c0 ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
             *reinterpret_cast<uint4*>(row_dst + (((c0 + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
           }
+        }
+        if (__any_sync(0xffffffffu, nan != 0)) {
+          if ((it.t0 + t + 1) * kN <= it.P)
+            set_nan_codes(src, sbase + L::kV16 + buf * kTile16 + cw * (32 * 128));
+          else
+            note_nan_codes(p);
         }
         fence_proxy_async();
         warp_arrive(JT_BAR(kBarBFull + buf));
@@ -1583,6 +1669,7 @@ __global__ void __launch_bounds__(kM) tree_attn_fp8_merge_kernel(
   const Workspace w = carve(p.workspace);
   const int c = blockIdx.x, tile = blockIdx.y >> 3, cg0 = (blockIdx.y & 7) * 4, row = threadIdx.x;
   const PieceMeta first = w.meta[2 * c + 1];
+  if (first.nan != 0 && blockIdx.y == 0) spread_nan_codes(p, kFewRows + 1, INT_MAX);
   if (!first.valid || first.finishes || 4 * cg0 >= p.head_dim) return;
   const int npt = kM / p.groups, npi = npt * Smem<kWide>::kTiles;
   const int T = p.node_counts[first.r];
@@ -1593,9 +1680,11 @@ __global__ void __launch_bounds__(kM) tree_attn_fp8_merge_kernel(
 #pragma unroll
   for (int k = 0; k < 16; ++k) acc[k] = 0.f;
   float m = -INFINITY, l = 0.f;
+  int nan = 0;
   for (int i = c; i < parts; ++i) {
     const int slot = i == c ? 2 * c + 1 : 2 * i;
     if (i != c && !w.meta[slot].valid) continue;  // a part shorter than the least cut
+    nan |= w.meta[slot].nan;
     const float2 ml = w.ml[(slot * 2ll + tile) * kM + row];
     float4 o[4];
 #pragma unroll
@@ -1615,6 +1704,8 @@ __global__ void __launch_bounds__(kM) tree_attn_fp8_merge_kernel(
     m = top;
     if (i != c && w.meta[slot].finishes) break;
   }
+  if (nan != 0 && sees_nan_code(p, first.r, load_request(p, first.r, false), first.h, j))
+    l = __uint_as_float(0x7fc00000u);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int h = first.h * p.groups + (row - local * p.groups);
   const int64_t at = (static_cast<int64_t>(p.cu_seqlens_q[first.r]) + j) * p.out_stride0 +

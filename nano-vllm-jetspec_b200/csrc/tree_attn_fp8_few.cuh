@@ -66,11 +66,16 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
   return r;
 }
-// A NaN code of a key that some row does not see must not reach that row as 0 x NaN.
+// A NaN code of a key that some row does not see must not reach that row as 0 x NaN: V's come out
+// as 448 in the tiles that hold such keys, and note_nan_codes sees to the rows that do see it.
 __device__ __forceinline__ uint32_t finite_f16x2(uint32_t v) {
   uint32_t r;
   asm("min.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(v), "r"(0x5f005f00u));  // 448
   return r;
+}
+
+__device__ __noinline__ void note_nan_keys(const JtTreeAttnFp8Params& p, uint4 a, uint4 b, uint4 c, uint4 d) {
+  if ((nan_codes(a) | nan_codes(b) | nan_codes(c) | nan_codes(d)) != 0) note_nan_codes(p);
 }
 
 struct FewPiece {
@@ -209,8 +214,9 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
     const unsigned char* ksc = static_cast<const unsigned char*>(p.k_scale);
     const unsigned char* vsc = static_cast<const unsigned char*>(p.v_scale);
     const int chunks = p.head_dim / 16, boxes = plan.tma ? kN / plan.box : 1;
+    if (lane == 0) meta[0].nan = meta[1].nan = 0;  // before any tile: note_nan_codes
     bool dead = false, gathered = false;
-    uint32_t issued = 0;
+    uint32_t issued = 0, marked = ~0u;  // stages whose words of missing keys may not be zero
 #pragma unroll 1
     while (!dead && few_next(p, cur, it, F::kRows)) {
       if (it.slot >= 0) {
@@ -262,13 +268,6 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
           if (lane == 0) mbar_arrive_tx(full, 2 * kTile8 + 2 * kN);
           __syncwarp();
           const int page = __shfl_sync(0xffffffffu, pages, (tile * boxes + lane) & 31);
-          if (lost == 0) {
-            if (lane == 0) *reinterpret_cast<int4*>(none) = make_int4(0, 0, 0, 0);
-          } else if (lane < 4) {
-            // This word's 32 keys lie in one box, or in two of 16.
-            const uint32_t b = lost >> (((tile * boxes) & 31) + 32 * lane / plan.box);
-            none[lane] = plan.box >= 32 ? (b & 1u ? ~0u : 0u) : (b & 1u ? 0xffffu : 0u) | (b & 2u ? ~0xffffu : 0u);
-          }
           if (lane < boxes) {
             // Page -1 lies outside the map: zeros.
             const int i = lane * plan.box, off = (kb + i) % p.block_size;
@@ -279,10 +278,19 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
             bulk_load(sdst, ksc + pg * p.ks_stride0 + it.h * p.ks_stride1 + off, plan.box, full);
             bulk_load(sdst + kN, vsc + pg * p.vs_stride0 + it.h * p.vs_stride1 + off, plan.box, full);
           }
+          if (lost != 0 || (marked >> stage) & 1u) {
+            if (lane < 4) {
+              // This word's 32 keys lie in one box, or in two of 16.
+              const uint32_t b = lost >> (((tile * boxes) & 31) + 32 * lane / plan.box);
+              none[lane] = plan.box >= 32 ? (b & 1u ? ~0u : 0u) : (b & 1u ? 0xffffu : 0u) | (b & 2u ? ~0xffffu : 0u);
+            }
+            marked = (marked & ~(1u << stage)) | (lost != 0 ? 1u << stage : 0u);
+          }
           if (lane != 0) mbar_arrive(full);
           mbar_arrive(full);
         } else {
           gathered = true;
+          marked |= 1u << stage;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const bool ok = at[i].page >= 0;
@@ -396,7 +404,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
       // Keys without a place in the pool are left out, like tree nodes that a row does not see.
       const uint32_t none = (reinterpret_cast<const uint32_t*>(sbase + F::kBad)[4 * stage + (w >> 1)] >>
                              (16 * (w & 1))) & 0xffffu;
-      const bool masked = (it.t0 + t + 1) * kN > it.P || none != 0;
+      const bool tail = (it.t0 + t + 1) * kN > it.P, masked = tail || none != 0;
       // S^T
       float s[NT][2][4];
 #pragma unroll
@@ -425,6 +433,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
         const int key = 2 * q4 + (i & 1) + 8 * (i >> 1);
         v[i] = *reinterpret_cast<const uint4*>(vt + key * 128 + ((g8 ^ (key & 7)) << 4));
       }
+      if (tail) note_nan_keys(p, v[0], v[1], v[2], v[3]);
       const uint32_t kb0 = sc[g8], kb1 = sc[g8 + 8], vb0 = sc[kN + g8], vb1 = sc[kN + g8 + 8];
       __syncwarp();
       if (lane == 0) mbar_arrive(empty0 + 8 * stage);
@@ -513,7 +522,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
           const uint32_t ab = __byte_perm(vw[0], vw[1], sel), cd = __byte_perm(vw[2], vw[3], sel);
           uint32_t a0 = e4m3x2_f16x2(ab), a1 = e4m3x2_f16x2(ab >> 16);
           uint32_t a2 = e4m3x2_f16x2(cd), a3 = e4m3x2_f16x2(cd >> 16);
-          if (masked) {
+          if (tail) {
             a0 = finite_f16x2(a0);
             a1 = finite_f16x2(a1);
             a2 = finite_f16x2(a2);
@@ -589,13 +598,16 @@ __global__ void __launch_bounds__(32 * kFewRows) tree_attn_fp8_few_merge_kernel(
   const Workspace w = carve(p.workspace);
   const int c = blockIdx.x, row = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PieceMeta first = w.meta[2 * c + 1];
+  if (first.nan != 0) spread_nan_codes(p, 1, kFewRows);
   if (!first.valid || first.finishes) return;
   if (row >= p.node_counts[first.r] * p.groups) return;
+  int nan = 0;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float m = -INFINITY, my = -INFINITY, l = 0.f;
   for (int i = c; i < parts; ++i) {
     const int slot = i == c ? 2 * c + 1 : 2 * i;
     if (i != c && !w.meta[slot].valid) continue;  // a part shorter than the least cut
+    nan |= w.meta[slot].nan;
     const float2 ml = w.ml[slot * 2ll * kM + row];
     const float oy = w.ml[(slot * 2ll + 1) * kM + row].x;
     const float4 o = w.o[(slot * 2ll * kM + row) * (kD / 4) + lane];
@@ -609,6 +621,8 @@ __global__ void __launch_bounds__(32 * kFewRows) tree_attn_fp8_few_merge_kernel(
     my = topy;
     if (i != c && w.meta[slot].finishes) break;
   }
+  if (nan != 0 && sees_nan_code(p, first.r, load_request(p, first.r, false), first.h, row / p.groups))
+    l = __uint_as_float(0x7fc00000u);
   if (4 * lane < p.head_dim)
     store_row4<kWide>(p, p.cu_seqlens_q[first.r], first.h, row, 4 * lane, acc, l, my - 7.f - m);
 }
