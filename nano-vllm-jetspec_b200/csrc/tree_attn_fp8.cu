@@ -5,30 +5,31 @@
 // then the T tree nodes), visible when the position is below P, or is node n <= j with zero
 // bias.  With k = K 2^e, v = V 2^f (K, V codes):
 //   s = scale * 2^e * sum_d q_d K_d,   p = exp(s - max),   out = sum p 2^f V / sum p
-// * Scores on 8-bit operands without loss: a bf16 query element, scaled by the row's power of
-//   two, is the sum of two e4m3 values (4 significant bits each, the second one signed: 8
-//   bits), an f16 one of three.  Q enters as two or three e4m3 tiles against the same K tile
-//   (kind::f8f6f4 runs at twice the bf16 rate, so two terms cost what one bf16 product
-//   would), and K goes from HBM to the tensor core untouched.  2^e multiplies the score
-//   column in the softmax.  Elements below 2^-10 of the row's largest lose low bits, at most
-//   2^-18 of that largest.
+// * Scores on 8-bit operands: a bf16 query element, scaled by the row's power of two, is the sum
+//   of two e4m3 values (4 significant bits each, the second one signed: 8 bits), an f16 one of
+//   three.  Q enters as two or three e4m3 tiles against the same K tile (kind::f8f6f4 runs at
+//   twice the bf16 rate, so two terms cost what one bf16 product would), and K goes from HBM to
+//   the tensor core untouched.  2^e multiplies the score column in the softmax.  Exact but for
+//   elements below 2^-9.8 (f16: 2^-6.8) of the row's largest: with that one scaled into
+//   (224, 448] the terms end at e4m3's least spacing 2^-9, so they lose at most half of it,
+//   2^-10 / 224 = 2^-17.8 of the largest.
 // * PV runs in bf16: four warps expand the V codes (exact in bf16, 2^f folded in) into the
 //   swizzled tile the MMA reads.  P is rounded to bf16 (8 bits, as in the 16-bit cache's
 //   kernel); f16 and fp32 outputs take P as hi + lo bf16 (16 bits).
 //
 // Requests of up to 16 rows (nodes x query heads of a KV head) would leave seven eighths of a
-// 128-row tile empty and take the kernel of tree_attn_fp8_few.cuh: 16 requests of 32 thousand
-// keys take 204 us there and 389 here with 4 rows each, 288 and 386 with 16, and 64 requests
-// of 500 to 4000 keys 95 and 128 with 4 rows, 124 and 122 with 16.
+// 128-row tile empty and take the kernel of tree_attn_fp8_few.cuh.  In one process 16 requests of
+// 30 to 32 thousand keys take 210 us there and 401 here with 4 rows each, 282 and 404 with 16, and
+// 64 requests of 500 to 4000 keys 115 and 160 with 4 rows, 156 and 164 with 16.
 //
 // Work: an item is (request, KV head, m-block), an m-block one or two 128-row query tiles;
 // the items' 128-key tiles, weighted by their measured time, form one line that is cut into
 // equal parts, one per CTA, so every SM has the same to do whatever the lengths (weights of 1
 // and 2 for one and two query tiles and 3 for an item, by tensor time alone, left CTAs between
-// 411 and 735 us of the same mix).  Every
-// CTA scans the lengths itself and finds its part: no plan kernel, no queue.  An item cut
-// between CTAs leaves unnormalised fp32 partials that a second small kernel merges (a
-// programmatic dependent; it returns at once when nothing was cut).
+// 411 and 735 us of the same mix).  Every CTA scans the lengths itself and finds its part: no plan
+// kernel, no queue.  An item cut between CTAs leaves unnormalised fp32 partials that a second small
+// kernel merges (a programmatic dependent, which also writes the rows of refused requests and of
+// NaN codes).
 //
 // Two softmax streams per CTA keep the tensor core busy while the other one works.  With two
 // query tiles (trees of more than 128 rows) each stream owns a tile and both use every K / V
@@ -36,11 +37,14 @@
 // end.  A stream goes through its keys 64 at a time, in two score buffers with a warpgroup
 // each.
 //
-// Bound: the softmax.  32 trees of 64 nodes over 2048 keys (70.9 GFLOP, 173 MB): 140 us, where
-// the matrix products alone would take 42 and the bytes 27.  128 keys against 256 rows take a
-// CTA about 5.5 thousand cycles, of which the tensor core works 2.1; 16 softmax warps beside
-// four converters reach 3.5 in a loop of their own, and the rest is the chain scores -> P -> PV
-// -> scores with its waits.
+// Bound: no unit, but the chain scores -> P -> PV -> scores with its waits.  32 trees of 64 nodes
+// over 2048 keys (70.9 GFLOP, 173 MB): 137 to 143 us by box, where the matrix products alone would
+// take 42 and the bytes 27.  128 keys against 256 rows take a CTA about 5.5 thousand cycles, of
+// which the tensor core works 2.1 and 16 softmax warps beside four converters 3.5 in a loop of
+// their own.  That is not what such trees have to cost: the 16-bit cache's kernel takes 112 us on
+// them (a serving mix: 326, here 473).  Work that it does not have: the key factors in both passes
+// over the scores, the expansion of V by four warps, and with one query tile half a key tile and an
+// O per stream.  So the 8-bit cache saves bytes here, and time where the bytes count (long decode).
 //
 //   warps 0, 2   MMA issuers, one per stream; TMEM (S0, S1, O0, O1: 128 columns each)
 //   warp 1       work pieces; TMA loads of K, V and scale bytes for prefix tiles

@@ -2,12 +2,14 @@
 // KV head <= 16: plain decode, chains of a few drafts).  Included by tree_attn_fp8.cu.
 //
 // Every byte of K and V is used by at most 16 rows, so the kernel is bound by HBM: per 128-key
-// tile an SM has 1360 cycles at the measured copy rate, and all that matters is to spend fewer
-// (it takes 1600: 16 requests of 32 thousand keys 177 us, 5.6 TB/s, and 190 with the merge).
-// The tensor core kernel needs 3400 (V expanded to bf16 through shared memory, 128-row MMAs with
-// 4 live rows).  Here both products run as register mma.m16n8k16 on f16 with the keys (K) and the
-// dims (V) on the 16 side and the query rows on the 8 side, so that up to 8 rows waste nothing,
-// and the codes go from shared memory to MMA fragments in registers:
+// tile an SM has 1360 cycles at the measured copy rate, and all that matters is to spend fewer.
+// It takes 1650: 16 requests of 30 to 32 thousand keys, 4 rows each, 183 us, 5.4 TB/s, and 184 to
+// 198 by box with the merge and the launches (the 16-bit cache: 340).  The tensor core kernel needs
+// 3400 (V expanded to bf16 through shared memory, 128-row MMAs with 4 live rows).  Launches whose
+// node counts the host does not know (captured and compiled ones) take the form of 16 rows, 286 us
+// for the same requests.  Here both products run as register mma.m16n8k16 on f16 with the keys (K)
+// and the dims (V) on the 16 side and the query rows on the 8 side, so that up to 8 rows waste
+// nothing, and the codes go from shared memory to MMA fragments in registers:
 //   S^T = K Q^T   a lane holds 32 consecutive dims of keys g and g + 8 (g = lane / 4), two 16-byte
 //                 loads a key, each 4-byte word the A fragment of one k-step after two exact
 //                 e4m3x2 -> f16x2 conversions; Q's dims are permuted alike.
@@ -24,8 +26,8 @@
 // Work: as in the tensor core kernel, the items' tiles form one line cut evenly over the SMs.
 // Warp 0 loads (TMA, or cp.async rows where TMA cannot) through a ring of four 32 KB stages;
 // each of the other warps takes 16 keys of a tile with its own maxima and sums, and the warps
-// meet at the end of a piece.  Eight such warps of 136 registers beat sixteen of 96 (two
-// tiles in hand): 202 to 240 us for 16 requests of 32 thousand keys.
+// meet at the end of a piece.  Eight such warps (146 registers for up to 8 rows) beat sixteen of
+// 96 (two tiles in hand) by 16 %.
 
 constexpr int kFewStages = 4;
 constexpr int kFewItemCost = 4;      // an item's fixed cost in tiles

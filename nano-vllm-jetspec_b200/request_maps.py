@@ -3,8 +3,10 @@
 The reference builds them on the host (BlockManager's page lists and the runner's
 prepare_prefill / prepare_decode loops, nanovllm/engine/block_manager.py,
 nanovllm/engine/model_runner.py) and uploads them every round.  ``build_request_maps`` takes
-the lengths and a free list that already live on the GPU, so a round whose lengths come out
-of the device-side acceptance walk needs no host in between.
+the lengths and a free list that already live on the GPU, so the maps of a round whose lengths
+come out of the device-side acceptance walk need no host in between.  What is left to the host:
+the free list has no cursor on the device (the next round's list begins ``pages_taken`` further
+on), and ``PackedTreeMetadata``'s builders take page tables of the host.
 """
 from __future__ import annotations
 

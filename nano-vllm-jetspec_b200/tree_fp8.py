@@ -28,7 +28,10 @@ def packed_tree_attention_fp8(q, k_pool, v_pool, k_scale, v_scale, metadata, sca
     kv_heads, dim] e4m3 with ``k_scale`` / ``v_scale`` [pages, kv_heads, block_size];
     ``metadata`` a ``PackedTreeMetadata``.  fp32 scores, softmax and sums; returns the output
     in ``q``'s dtype, or FP32 on request.  A row that sees no key gives zeros; one that sees a
-    NaN row of the cache gives NaN.
+    NaN row of the cache gives NaN.  A key whose page or slot lies outside the pool is left out;
+    requests that cannot be taken (trees above 1024 nodes, rows outside the packed ones, device
+    counts that the host's rule out) give zeros.  Both set a device error bit
+    (``read_device_errors``).
     """
     shape, pool_shape, dtype = q.shape, k_pool.shape, q.dtype
     if len(shape) != 3 or shape[0] != metadata.total_queries:
