@@ -90,7 +90,9 @@ typedef struct JtTreeAttnParams {
   int64_t v_stride0, v_stride1, v_stride2;
   float scale;
   int32_t split_keys;              /* 0 = automatic; else keys per split (multiple of 1024) */
-  void* workspace;                 /* device scratch, >= jt_tree_attn_workspace_size     */
+  void* workspace;                 /* device scratch, >= jt_tree_attn_workspace_size; launches
+                                      that share one come from one thread at a time, on one
+                                      stream                                               */
   size_t workspace_bytes;
 } JtTreeAttnParams;
 

@@ -393,6 +393,7 @@ __device__ __forceinline__ uint32_t nan_codes(uint4 w) {
 }
 // NaN where the codes of a converter warp's 32 V rows are NaN, in their bf16 rows: a row per lane.
 __device__ __noinline__ void set_nan_codes(const unsigned char* src, unsigned char* dst) {
+  __syncwarp();  // the rows were written by other lanes
   const int row = threadIdx.x & 31;
 #pragma unroll 1
   for (int c = 0; c < 16; ++c) {  // eight codes: two words
