@@ -38,7 +38,7 @@
 // each.
 //
 // Bound: no unit, but the chain scores -> P -> PV -> scores with its waits.  32 trees of 64 nodes
-// over 2048 keys (70.9 GFLOP, 173 MB): 137 to 143 us by box, where the matrix products alone would
+// over 2048 keys (70.9 GFLOP, 173 MB): 137 to 143 us by card, where the matrix products alone would
 // take 42 and the bytes 27.  128 keys against 256 rows take a CTA about 5.5 thousand cycles, of
 // which the tensor core works 2.1 and 16 softmax warps beside four converters 3.5 in a loop of
 // their own.  That is not what such trees have to cost: the 16-bit cache's kernel takes 112 us on

@@ -4,7 +4,7 @@
 // Every byte of K and V is used by at most 16 rows, so the kernel is bound by HBM: per 128-key
 // tile an SM has 1360 cycles at the measured copy rate, and all that matters is to spend fewer.
 // It takes 1650: 16 requests of 30 to 32 thousand keys, 4 rows each, 183 us, 5.4 TB/s, and 184 to
-// 198 by box with the merge and the launches (the 16-bit cache: 340).  The tensor core kernel needs
+// 198 by card with the merge and the launches (the 16-bit cache: 340).  The tensor core kernel needs
 // 3400 (V expanded to bf16 through shared memory, 128-row MMAs with 4 live rows).  Launches whose
 // node counts the host does not know (captured and compiled ones) take the form of 16 rows, 286 us
 // for the same requests.  Here both products run as register mma.m16n8k16 on f16 with the keys (K)
