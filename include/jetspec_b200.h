@@ -449,7 +449,8 @@ int32_t jt_kv_fp8_commit_max_slots(void);
  * nodes are allowed.  Strides of the pools and scales in bytes, of q and out in elements,
  * last dimensions contiguous; pool rows 16-byte aligned (head_dim a multiple of 16, at most
  * 128), at most 1024 nodes per tree (larger: device error bit 1, the rows are zeros).  A request
- * whose nodes leave [0, total_queries) sets device error bit 0; its rows in range are zeros.
+ * whose nodes leave [0, total_queries), or whose bias has not T_r^2 entries by its offsets, sets
+ * device error bit 0; its rows in range are zeros.
  */
 typedef struct JtTreeAttnFp8Params {
   void* out;                       /* [total_queries, q_heads, head_dim], out_dtype      */

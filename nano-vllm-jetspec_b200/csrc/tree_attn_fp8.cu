@@ -393,7 +393,6 @@ __device__ __forceinline__ uint32_t nan_codes(uint4 w) {
 }
 // NaN where the codes of a converter warp's 32 V rows are NaN, in their bf16 rows: a row per lane.
 __device__ __noinline__ void set_nan_codes(const unsigned char* src, unsigned char* dst) {
-  __syncwarp();  // the rows were written by other lanes
   const int row = threadIdx.x & 31;
 #pragma unroll 1
   for (int c = 0; c < 16; ++c) {  // eight codes: two words
@@ -455,13 +454,19 @@ __device__ __forceinline__ ItemInfo item_info(const Geometry& ge, int P, int T, 
   it.cost = it.n * it.weight + kItemCost;
   return it;
 }
+// Whether T nodes from packed row q0 on leave the call's rows, or their square the request's share
+// of the bias.
+__device__ __forceinline__ bool astray(const JtTreeAttnFp8Params& p, int T, int q0, int64_t biases) {
+  return T > 0 && (q0 < 0 || T > p.total_queries - q0 || static_cast<int64_t>(T) * T > biases);
+}
 // A request as the kernels take it: no nodes when it has none or is refused.
 __device__ __noinline__ int2 load_request(const JtTreeAttnFp8Params& p, int r, bool flag) {
+  // Loaded together: calls of this are a chain that short launches wait for.
   int P = __ldg(p.prefix_lens + r), T = __ldg(p.node_counts + r);
-  const int64_t capacity = static_cast<int64_t>(p.table_width) * p.block_size;
-  // Refused: clear_refused.
   const int q0 = __ldg(p.cu_seqlens_q + r);
-  if (T > kMaxNodes || q0 < 0 || T > p.total_queries - q0) T = 0;
+  const int64_t b0 = __ldg(p.qq_bias_offsets + r), b1 = __ldg(p.qq_bias_offsets + r + 1);
+  const int64_t capacity = static_cast<int64_t>(p.table_width) * p.block_size;
+  if (T > kMaxNodes || astray(p, T, q0, b1 - b0)) T = 0;  // refused: clear_refused
   if (P < 0 || P > capacity) {
     if (flag) atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
     P = P < 0 ? 0 : static_cast<int>(capacity);
@@ -537,16 +542,18 @@ __device__ __noinline__ void clear_refused(const JtTreeAttnFp8Params& p, int lea
   for (int64_t first = blockIdx.x; first < p.num_requests; first += 32 * stride) {
     const int64_t r = first + lane * stride;
     int T = 0, q0 = 0;
+    int64_t biases = 0;
     if (r < p.num_requests) {
       T = __ldg(p.node_counts + r);
       q0 = __ldg(p.cu_seqlens_q + r);
+      biases = __ldg(p.qq_bias_offsets + r + 1) - __ldg(p.qq_bias_offsets + r);
     }
     const bool large = T > kMaxNodes;
-    const bool astray = T > 0 && (q0 < 0 || T > p.total_queries - q0 ||
-                                  (!large && (T * p.groups < least || T * p.groups > most)));
+    const bool out = astray(p, T, q0, biases) ||
+                     (T > 0 && !large && (T * p.groups < least || T * p.groups > most));
     if (large) atomicOr(&g_attn_fp8_errors, JT_DEVERR_TREE_TOO_LARGE);
-    if (astray) atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
-    uint32_t todo = __ballot_sync(0xffffffffu, large || astray);
+    if (out) atomicOr(&g_attn_fp8_errors, JT_DEVERR_OUT_OF_RANGE);
+    uint32_t todo = __ballot_sync(0xffffffffu, large || out);
     for (; todo != 0; todo &= todo - 1) {
       const int src = __ffs(todo) - 1;
       const int64_t q = __shfl_sync(0xffffffffu, q0, src), n = __shfl_sync(0xffffffffu, T, src);
@@ -916,8 +923,10 @@ __global__ void __launch_bounds__(256) tree_attn_fp8_split_kernel(
     uint32_t mine = 0;  // word `lane`
     if (r >= 0 && r < p.num_requests && j >= 0) {
       const int T = __ldg(p.node_counts + r);
-      if (j < T && T <= kMaxNodes) {
-        const float* bias = p.qq_bias + __ldg(p.qq_bias_offsets + r) + static_cast<int64_t>(j) * T;
+      const int q0 = __ldg(p.cu_seqlens_q + r);
+      const int64_t b0 = __ldg(p.qq_bias_offsets + r), b1 = __ldg(p.qq_bias_offsets + r + 1);
+      if (j < T && T <= kMaxNodes && !astray(p, T, q0, b1 - b0)) {
+        const float* bias = p.qq_bias + b0 + static_cast<int64_t>(j) * T;
 #pragma unroll 4
         for (int w = 0; 32 * w <= j; ++w) {
           const int n = 32 * w + lane;
@@ -1376,7 +1385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           wait_shared_at_least(base + L::kMisc + 8, g + 1, abort);
           wait_shared_at_least(base + L::kMisc + 12, g + 1, abort);
-          __syncwarp();
+          __syncwarp();  // the rows are other lanes' too
           unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256 + lane;
           uint32_t* lost = reinterpret_cast<uint32_t*>(sbase + L::kLost) + 4 * (g % kScaleRing);
 #pragma unroll
@@ -1390,7 +1399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           asm volatile("cp.async.wait_all;\n" ::: "memory");
           fence_proxy_async();
-          __syncwarp();
+          __syncwarp();  // the rows are other lanes' too
           if (lane == 0) {
             mbar_arrive(JT_BAR(kBarKFull + ks));
             mbar_arrive(JT_BAR(kBarVFull + vs));
@@ -1475,6 +1484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (__any_sync(0xffffffffu, nan != 0)) {
+          __syncwarp();  // the rows are other lanes' too
           if ((it.t0 + t + 1) * kN <= it.P)
             set_nan_codes(src, sbase + L::kV16 + buf * kTile16 + cw * (32 * 128));
           else
@@ -1623,7 +1633,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int c = c0; c < c1; ++c) {  // 16 columns
           uint32_t o0[16], o1[16];
-          __syncwarp();
+          __syncwarp();  // the rows are other lanes' too
           tmem_ld16(tmem + lanes + col_o(tile) + 16 * c, o0);
 #pragma unroll
           for (int k = 0; k < 16; ++k) o1[k] = 0u;

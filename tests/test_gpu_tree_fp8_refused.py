@@ -112,3 +112,24 @@ def test_a_tree_above_1024_nodes_where_few_rows_are_known():
     assert (got[:1030] == 0).all()
     case.run = lambda **kw: got
     case.check([1])
+
+
+@pytest.mark.parametrize("groups,counts", [(1, (5, 9, 4)), (4, (50, 3, 40))])
+@pytest.mark.parametrize("known", [True, False])
+@pytest.mark.parametrize("bad", [0, 2])
+def test_counts_that_the_bias_does_not_hold(groups, counts, known, bad):
+    """Offsets that give a request a smaller matrix than its nodes': it is refused, not read past."""
+    case = Case([300, 40, 900], counts, kv_heads=2, groups=groups, seed=35)
+    offsets = case.meta.qq_bias_offsets.clone()
+    if bad == 0:
+        offsets[0] += 1
+    else:
+        offsets[3] -= 1
+    meta = namespace(case.meta, qq_bias_offsets=offsets,
+                     **({} if known else {"node_counts_host": None}))
+    jb.read_device_errors()
+    got = run(case, meta)
+    assert jb.read_device_errors() == 1
+    assert (got[rows(case, bad)] == 0).all()
+    case.run = lambda **kw: got
+    case.check([r for r in range(3) if r != bad])
