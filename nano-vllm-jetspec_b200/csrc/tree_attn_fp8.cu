@@ -1385,7 +1385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           wait_shared_at_least(base + L::kMisc + 8, g + 1, abort);
           wait_shared_at_least(base + L::kMisc + 12, g + 1, abort);
-          __syncwarp();  // the rows are other lanes' too
+          __syncwarp();
           unsigned char* sc = sbase + L::kScale + (g % kScaleRing) * 256 + lane;
           uint32_t* lost = reinterpret_cast<uint32_t*>(sbase + L::kLost) + 4 * (g % kScaleRing);
 #pragma unroll
@@ -1399,7 +1399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           asm volatile("cp.async.wait_all;\n" ::: "memory");
           fence_proxy_async();
-          __syncwarp();  // the rows are other lanes' too
+          __syncwarp();
           if (lane == 0) {
             mbar_arrive(JT_BAR(kBarKFull + ks));
             mbar_arrive(JT_BAR(kBarVFull + vs));
@@ -1633,7 +1633,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int c = c0; c < c1; ++c) {  // 16 columns
           uint32_t o0[16], o1[16];
-          __syncwarp();  // the rows are other lanes' too
+          __syncwarp();
           tmem_ld16(tmem + lanes + col_o(tile) + 16 * c, o0);
 #pragma unroll
           for (int k = 0; k < 16; ++k) o1[k] = 0u;
